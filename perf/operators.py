@@ -328,11 +328,11 @@ def _sample(s):
     w = torch.round(torch.exp(x) * ONE).to(torch.int64)
     place = torch.arange(n, device=DEV)[None]
     k = torch.where(s["top_k"] > 0, s["top_k"], n)[:, None]
-    w = torch.where(place < torch.where(t > 0, k, 1), w, 0)
+    w = torch.where((w >= s["min_p"].double()[:, None] * ONE) & (place < torch.where(t > 0, k, 1)), w, 0)
     total = torch.cumsum(w, dim=1)
     p = s["top_p"].double()[:, None]
     goal = torch.where(p < 1, torch.ceil(p * total[:, -1:].double()).to(torch.int64).clamp(min=1), total[:, -1:])
-    w = torch.where((total - w < goal) & (w >= s["min_p"].double()[:, None] * ONE), w, 0)
+    w = torch.where(total - w < goal, w, 0)
     total = torch.cumsum(w, dim=1)
     left = total[:, -1:]
     r = torch.minimum((s["u"].double()[:, None] * left.double()).to(torch.int64), left - 1)
@@ -403,12 +403,11 @@ def _chance(s, r):
         return 1.0
     l = s["logits"][r].double()
     p = torch.sort(torch.softmax(l / t, 0), descending=True).values
-    best = p[0].item()
+    p = p[p >= low * p[0]]
     p = p[:int(k)] if k > 0 else p
     if 0 < top < 1:
         before = torch.cumsum(p, 0) - p
         p = p[before < top * p.sum()]
-    p = p[p >= low * best]
     c = torch.cumsum(p, 0)
     at = min(int(torch.searchsorted(c, float(s["u"][r]) * c[-1].item(), right=True)), p.numel() - 1)
     return (p[at] / c[-1]).item()
