@@ -44,6 +44,9 @@ EXPORTS = (
     "btl_add_rmsnorm_swiglu_workspace_bytes", "btl_linear_residual",
     "btl_add_rmsnorm_linear_group_ref",
     "btl_stream_create", "btl_stream_stage_words", "btl_stream_run", "btl_stream_destroy",
+    # include/bitserve.h
+    "btl_paged_rope_append", "btl_paged_read", "btl_paged_attention_workspace_bytes", "btl_paged_attention",
+    "btl_sample_workspace_bytes", "btl_sample",
 )
 
 
@@ -63,6 +66,20 @@ class BtlKvQ8(ctypes.Structure):
 class BtlStreamLayer(ctypes.Structure):
     """btl_stream_layer_t: the seven packed projections of one decoder layer."""
     _fields_ = [(nm, BtlPacked) for nm in ("q", "k", "v", "o", "gate", "up", "down")]
+
+
+class BtlKvPaged(ctypes.Structure):
+    """btl_kv_paged_t: one layer's Q8 cache in pages of a shared pool."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("n_kv_heads", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64)]
+
+
+class BtlPagedBatch(ctypes.Structure):
+    """btl_paged_batch_t: the sequences of one call."""
+    _fields_ = [("row_start", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int64), ("max_pages", ctypes.c_int64), ("rows", ctypes.c_int64),
+                ("max_rows", ctypes.c_int64), ("max_len", ctypes.c_int64)]
 
 
 class BitLinearError(RuntimeError):
@@ -131,6 +148,12 @@ def _load():
         "btl_stream_stage_words": (sz, [vp]),
         "btl_stream_run": (i32, [vp, vp, vp, vp, vp]),
         "btl_stream_destroy": (i32, [vp]),
+        "btl_paged_rope_append": (i32, [vp, vp, vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), vp, vp, i64, vp, vp]),
+        "btl_paged_read": (i32, [P(BtlKvPaged), P(BtlPagedBatch), vp, vp, i32, vp]),
+        "btl_paged_attention_workspace_bytes": (sz, [i64, P(BtlKvPaged), P(BtlPagedBatch)]),
+        "btl_paged_attention": (i32, [vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), vp, vp, sz, vp]),
+        "btl_sample_workspace_bytes": (sz, [i64, i64]),
+        "btl_sample": (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -194,6 +194,60 @@ extern "C" {
 }
 
 // ---------------------------------------------------------------------------
+// include/bitserve.h
+// ---------------------------------------------------------------------------
+
+/// `btl_kv_paged_t`: one layer's Q8 KV cache in pages of a shared pool (device
+/// arrays; k [n_pages, n_kv_heads, page_size, head_dim], v in blocks of 16 tokens
+/// [n_pages, n_kv_heads, page_size / 16, head_dim, 16], scales [n_pages, n_kv_heads,
+/// page_size]).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct btl_kv_paged_t {
+    pub k: *mut u8,
+    pub v: *mut u8,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub n_pages: i64,
+    pub n_kv_heads: i64,
+    pub page_size: i64,
+    pub head_dim: i64,
+}
+
+/// `btl_paged_batch_t`: the sequences of one call (device int32 arrays row_start
+/// [n_seqs + 1], pos [n_seqs], pages [n_seqs, max_pages]) and the host's bounds.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct btl_paged_batch_t {
+    pub row_start: *const i32,
+    pub pos: *const i32,
+    pub pages: *const i32,
+    pub n_seqs: i64,
+    pub max_pages: i64,
+    pub rows: i64,
+    pub max_rows: i64,
+    pub max_len: i64,
+}
+
+extern "C" {
+    pub fn btl_paged_rope_append(q: *const c_void, k: *const c_void, v: *const c_void, dtype: c_int, n_heads: i64,
+                                 cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t,
+                                 rope_cos: *const f32, rope_sin: *const f32, rope_len: i64, q_out: *mut c_void,
+                                 stream: *mut c_void) -> c_int;
+    pub fn btl_paged_read(cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t, k_out: *mut c_void,
+                          v_out: *mut c_void, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn btl_paged_attention_workspace_bytes(n_heads: i64, cache: *const btl_kv_paged_t,
+                                               batch: *const btl_paged_batch_t) -> usize;
+    pub fn btl_paged_attention(q: *const c_void, dtype: c_int, n_heads: i64, cache: *const btl_kv_paged_t,
+                               batch: *const btl_paged_batch_t, out: *mut c_void, ws: *mut c_void,
+                               ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn btl_sample_workspace_bytes(rows: i64, n: i64) -> usize;
+    pub fn btl_sample(logits: *const f32, rows: i64, n: i64, ld: i64, temperature: *const f32, top_k: *const i32,
+                      top_p: *const f32, min_p: *const f32, u: *const f32, ids: *mut i32, probs: *mut f32,
+                      ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> c_int;
+}
+
+// ---------------------------------------------------------------------------
 // the HIP runtime calls the safe wrapper needs (libamdhip64)
 // ---------------------------------------------------------------------------
 
