@@ -61,7 +61,7 @@ __device__ __forceinline__ int find_seq(const Paged& c, int row, int lane)
 // page id of a group of 16 positions (-1: none in the pool) and the group's place in the page
 __device__ __forceinline__ int page_of(const Paged& c, const int32_t* table, int grp, int* in_page)
 {
-    const int j = c.ppg_shift >= 0 ? grp >> c.ppg_shift : grp / c.ppg;
+    const int j = (int)__umulhi(2u * (uint32_t)grp, c.ppg_mul);  // grp / ppg
     *in_page = grp - j * c.ppg;
     const int id = table[j];
     return id >= 0 && id < c.n_pages ? id : -1;
@@ -205,7 +205,7 @@ hipError_t launch_paged_read(const PagedRead& a, hipStream_t st)
 }
 
 // ---------------------------------------------------------------------------
-// k_paged_attn
+// Attention: k_paged_tok, k_paged_tile
 // ---------------------------------------------------------------------------
 // Per KV head the rows of a sequence times the query heads of the group are one
 // list of query rows m = i * group + e; a wave takes 16 of them a column tile
@@ -221,22 +221,26 @@ hipError_t launch_paged_read(const PagedRead& a, hipStream_t st)
 // 16 (r / 4) + 4 t + r % 4 in row r, which makes the four tiles' results in one
 // lane -- rows 4 g .. 4 g + 3 -- the 16 neighbours 16 g .. 16 g + 15.  Those are,
 // as they stand, the second product's operand: its other side, 16 keys of one
-// value, is one 16-byte load of the blocked v.  Nothing crosses lanes but the
-// row maxima (two shuffles), and no operand goes through LDS.
+// value, is one 16-byte load of the blocked v.  Nothing crosses lanes on the way.
 //
 // A code u8 becomes the f16 1024 + u8 by one byte permute, less 1152 (exact).
 // Queries are scaled by a power of two per row to just under 2^15, softmax weights
 // times the value's scale by one per (row, largest value scale so far): what is
-// lost is below 2^-39 of the row's largest term, not below f16's smallest number.
+// lost is below 2^-30 of the row's largest term, not below f16's smallest number.
 //
-// The token form (TOK, at most 16 query rows) gives the keys of a chunk to its
-// four waves in turn and merges them in LDS; the tile form gives 16 NT query rows
-// to each of its four waves and every key to all of them.
+// The softmax is taken in one pass against a reference that follows the row's
+// largest score, but only when a score passes it by 2^6: then the sums so far are
+// scaled down.  A few times a row, so the common step has neither a maximum across
+// lanes nor a scaling of the outputs.
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 namespace {
+
+constexpr float kAhead = 6.0f;   // a score may pass the reference by this (log2)
+constexpr int kVUp = 8;          // weights times value scales stay below 2^(kAhead + 1 + kVUp) = 2^15
+constexpr int kLeastExp = -100;  // the least exponent of a value scale that weights are scaled by
 
 // four codes -> four f16 (code - 128)
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t* o)
@@ -256,16 +260,25 @@ __device__ __forceinline__ h8 widen8(uint32_t w0, uint32_t w1)
     return __builtin_bit_cast(h8, *(uint4*)o);
 }
 
+// The largest / the sum of a value over the four lanes n, n + 16, n + 32, n + 48,
+// in each of them.  Swapping rows of a register with rows of its copy leaves the
+// pairs' other values in the two results.
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ float xor16_max(float v)
 {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
 }
 
 __device__ __forceinline__ float xor16_sum(float v)
 {
-    v = __fadd_rn(v, __shfl_xor(v, 16, 64));
-    return __fadd_rn(v, __shfl_xor(v, 32, 64));
+    u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __fadd_rn(__uint_as_float(p.x), __uint_as_float(p.y));
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __fadd_rn(__uint_as_float(p.x), __uint_as_float(p.y));
 }
 
 // Keeps the f32 product v as it was rounded.  The compiler may turn an f16
@@ -277,14 +290,14 @@ __device__ __forceinline__ void as_rounded(float& v) { asm("" : "+v"(v)); }
 // 2^e, -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// exponent of |v|, kept in [-110, 127] (0, subnormal: -110; not finite: as 0)
+// exponent of |v|, at least kLeastExp (0, subnormal, not finite: that)
 __device__ __forceinline__ int expo(float v)
 {
     const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-    return b >= 0x7F800000u ? -110 : max((int)(b >> 23) - 127, -110);
+    return b >= 0x7F800000u ? kLeastExp : max((int)(b >> 23) - 127, kLeastExp);
 }
 
-// The rows' chunk or the whole output of one query row: v of 4 neighbouring values.
+// v's 4 neighbouring values of a row
 template <bool BF>
 __device__ __forceinline__ void store4(void* p, int64_t i, f4 v)
 {
@@ -298,344 +311,584 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f4 v)
     }
 }
 
+// row of a sequence that query row m belongs to: m / group
+__device__ __forceinline__ int row_of(const PagedAttn& a, int m) { return (int)__umulhi(2u * (uint32_t)m, a.group_mul); }
+
+// The query rows of a wave: NT tiles of 16, in PARTS f16 parts.
+template <int NJ, int NT, bool BF>
+struct Queries {
+    static constexpr int PARTS = BF ? 1 : 2;
+    float cq[NT];  // log2 units of one unit of the scaled product
+    h8 v[PARTS][NT][2 * NJ];
+
+    // rows m0 .. of a sequence, none past m_last (those repeat it); row0: the output row of m = 0
+    __device__ __forceinline__ void load(const PagedAttn& a, const Seq& q, int64_t row0, int m0, int m_last, int lane)
+    {
+        const int g = lane >> 4, n = lane & 15, hd = a.c.hd;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const int m = m0 + 16 * u + n;
+            const int mm = min(m, m_last);
+            const int i = row_of(a, mm);
+            const int64_t r = row0 + (int64_t)i * a.nh + (mm - i * a.group);
+            float f[NJ][16];
+            float am = 0.0f;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int d = 16 * (4 * j + g);
+                if (BF) {
+                    uint4 w[2] = {};
+                    if (d < hd) {
+                        w[0] = *(const uint4*)((const uint16_t*)a.q + r * hd + d);
+                        w[1] = *(const uint4*)((const uint16_t*)a.q + r * hd + d + 8);
+                    }
+                    widen16<XK_BF16>(w, f[j]);
+                } else {
+                    uint4 w[4] = {};
+                    if (d < hd)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] = *(const uint4*)((const float*)a.q + r * hd + d + 4 * x);
+                    widen16<XK_F32>(w, f[j]);
+                }
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    am = fmaxf(am, __builtin_fabsf(f[j][x]));
+                    bad |= !(__builtin_fabsf(f[j][x]) < __builtin_inff());
+                }
+            }
+            am = xor16_max(bad ? __builtin_inff() : am);
+            const bool fin = am < __builtin_inff();
+            const int sh = fin ? 14 - expo(am) : 0;
+            const float up = exp2i(sh);
+            cq[u] = fin ? __fmul_rn(a.scale_log2, exp2i(-sh)) : __builtin_nanf("");
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float y = fin ? __fmul_rn(f[j][x], up) : 0.0f;  // exact
+                    const _Float16 hi = (_Float16)y;
+                    v[0][u][2 * j + (x >> 3)][x & 7] = hi;
+                    if (PARTS == 2) v[PARTS - 1][u][2 * j + (x >> 3)][x & 7] = (_Float16)__fsub_rn(y, (float)hi);
+                }
+        }
+    }
+};
+
+// One column tile's running softmax and output.
+template <int DT>
+struct Running {
+    float ref, l;  // reference (log2; -inf before the first key), this lane's part of the sum
+    int ve;        // exponent of the value scales that the weights are scaled by
+    f4 o[DT];
+
+    __device__ __forceinline__ void clear()
+    {
+        ref = -__builtin_inff();
+        l = 0.0f;
+        ve = kLeastExp;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    __device__ __forceinline__ void scale(float f)
+    {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+
+    // the value scales up to exponent e are to come
+    __device__ __forceinline__ void raise(int e)
+    {
+        scale(__builtin_ldexpf(1.0f, ve - e));
+        ve = e;
+    }
+
+    // sc: the products of 16 keys with their scales (-inf: not seen); vs: value
+    // scales times 2^(kVUp - ve).  Leaves the weights, in f16 parts.
+    template <int PARTS>
+    __device__ __forceinline__ void weigh(const f4* sc, const f4* vs, float cq, h8 (*pw)[2])
+    {
+        float y[16];
+        float big = -__builtin_inff();
+        float at = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            y[x] = __fmaf_rn(sc[x >> 2][x & 3], cq, -at);
+            big = fmaxf(big, y[x]);
+        }
+        if (__any(big > kAhead || ref == -__builtin_inff())) {
+            const float mine = xor16_max(big);
+            const bool moves = mine > (ref == -__builtin_inff() ? -__builtin_inff() : kAhead);
+            const float to = moves ? __fadd_rn(at, mine) : ref;
+            const float down = ref == -__builtin_inff() ? 0.0f : (moves ? __builtin_amdgcn_exp2f(__fsub_rn(at, to)) : 1.0f);
+            l = __fmul_rn(l, down);
+            scale(down);
+            ref = to;
+            at = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) y[x] = __fmaf_rn(sc[x >> 2][x & 3], cq, -at);
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float p = __builtin_amdgcn_exp2f(y[x]);
+            l = __fadd_rn(l, p);
+            float w = __fmul_rn(p, vs[x >> 2][x & 3]);
+            if (PARTS == 2) as_rounded(w);
+            const _Float16 hi = (_Float16)w;
+            pw[0][x >> 3][x & 7] = hi;
+            if (PARTS == 2) pw[PARTS - 1][x >> 3][x & 7] = (_Float16)__fsub_rn(w, (float)hi);
+        }
+    }
+
+    // the largest finite value scale among 16, over the four lanes of a row
+    __device__ __forceinline__ static float largest(const f4* vs)
+    {
+        float m = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float v = __builtin_fabsf(vs[x >> 2][x & 3]);
+            m = v < __builtin_inff() ? fmaxf(m, v) : m;
+        }
+        return xor16_max(m);
+    }
+
+    // a step whose keys this lane's row sees below `vis` only (key: its first)
+    template <int PARTS>
+    __device__ __forceinline__ void weigh_masked(f4* sc, const f4* vs, int key, int vis, float cq, h8 (*pw)[2])
+    {
+        f4 vm[4];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const bool see = key + x < vis;
+            sc[x >> 2][x & 3] = see ? sc[x >> 2][x & 3] : -__builtin_inff();
+            vm[x >> 2][x & 3] = see ? vs[x >> 2][x & 3] : 0.0f;
+        }
+        const int e = max(ve, expo(largest(vm)));
+        if (__any(e != ve)) raise(e);
+        const float up = exp2i(kVUp - ve);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vm[t] *= up;
+        weigh<PARTS>(sc, vm, cq, pw);
+    }
+
+    // one unit of o
+    __device__ __forceinline__ float unit() const { return exp2i(ve - kVUp); }
+};
+
+struct True {
+    constexpr operator bool() const { return true; }
+};
+struct False {
+    constexpr operator bool() const { return false; }
+};
+
+// First slot, counted over all pages, of the group of 16 keys `grp` (past the last
+// one: of that) for KV head h; -1: its page is outside the pool.
+__device__ __forceinline__ int64_t group_slot(const Paged& c, const int32_t* table, int grp, int last_grp, int h)
+{
+    int in;
+    const int page = page_of(c, table, min(grp, last_grp), &in);
+    return page < 0 ? -1 : ((int64_t)page * c.nkv + h) * c.ps + 16 * in;
+}
+
+__device__ __forceinline__ int64_t pick(int x, int64_t s0, int64_t s1, int64_t s2, int64_t s3)
+{
+    s0 = x == 1 ? s1 : s0;
+    s0 = x == 2 ? s2 : s0;
+    return x == 3 ? s3 : s0;
+}
+
+// Where a workgroup works: its KV head, chunk of keys and sequence.
+struct Place {
+    int h, chunk, tile, s;
+};
+
+// blockIdx.x = h + nkv (chunk + chunks * tile): the head varies fastest.  Workgroups
+// go to the XCDs in turn, so with 8 KV heads the tiles and chunks of one head share
+// an XCD's L2.
+__device__ __forceinline__ Place place_of(const Paged& c, int chunks)
+{
+    Place p;
+    p.h = (int)(blockIdx.x % (unsigned)c.nkv);
+    const unsigned b = blockIdx.x / (unsigned)c.nkv;
+    p.chunk = (int)(b % (unsigned)chunks);
+    p.tile = (int)(b / (unsigned)chunks);
+    p.s = p.tile;
+    return p;
+}
+
+// The rows of a refused sequence.
+template <bool BF>
+__device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h, int wave, int lane)
+{
+    for (int i = wave; i < q.n; i += 4)
+        for (int x = lane; x < a.group * a.c.hd; x += 64)
+            store1<BF>(a.out, ((int64_t)(q.a + i) * a.nh + h * a.group) * a.c.hd + x, __builtin_nanf(""));
+}
+
 }  // namespace
 
-template <int NJ, int NT, bool TOK, bool BF>
-__global__ __launch_bounds__(256) void k_paged_attn(PagedAttn a)
+// The token form: at most 16 query rows of a sequence.  grid nkv * chunks * n_seqs,
+// block 256: the four waves take the chunk's keys in turn, 64 at a time, straight
+// from memory into the operands' registers, and are merged in LDS.  DT: 16-value
+// tiles of a head, hd / 16 or one more.
+template <int DT, bool BF>
+__global__ __launch_bounds__(256) void k_paged_tok(PagedAttn a)
 {
-    constexpr int DT = 4 * NJ;         // 16-value tiles of a head, at most
-    constexpr int PARTS = BF ? 1 : 2;  // f16 parts of a query and of a weight
-    constexpr int MT = TOK ? kTokRows : 64 * NT;
+    constexpr int NJ = (DT + 3) / 4;
+    constexpr int PARTS = BF ? 1 : 2;
+    __shared__ float s_o[4][16][16 * DT + 4];
+    __shared__ float s_m[4][16], s_l[4][16];
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
-    const int hd = c.hd, ndt = hd >> 4;
-    // the head varies fastest: neighbouring workgroups go to different XCDs, so with
-    // 8 KV heads the tiles and chunks of one head share that XCD's L2
-    const int h = (int)(blockIdx.x % (unsigned)c.nkv);
-    const unsigned bi = blockIdx.x / (unsigned)c.nkv;
-    const int chunks = TOK ? a.p.tok_n : a.p.tile_n, C = TOK ? a.p.tok_c : a.p.tile_c;
-    const int chunk = (int)(bi % (unsigned)chunks);
-    int tile = (int)(bi / (unsigned)chunks);
-
-    // the sequence and its tile
-    int s;
-    if (TOK) {
-        s = tile;
-        tile = 0;
-    } else {
-        int base = 0;
-        for (s = -1; base < c.n_seqs; base += 64) {
-            int mine = 0;
-            if (base + lane < c.n_seqs) {
-                const int64_t rows = (int64_t)seq_at(c, base + lane).n * a.group;
-                mine = rows > a.p.lo ? (int)((rows + MT - 1) / MT) : 0;
-            }
-            int upto = mine;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int o = __shfl_up(upto, off, 64);
-                upto += lane >= off ? o : 0;
-            }
-            const uint64_t past = __ballot(upto > tile);
-            if (past) {
-                const int at = __ffsll((unsigned long long)past) - 1;
-                s = base + at;
-                tile -= __builtin_amdgcn_readlane(upto - mine, at);
-                break;
-            }
-            tile -= __builtin_amdgcn_readlane(upto, 63);
-        }
-        if (s < 0) return;
-    }
-    s = __builtin_amdgcn_readfirstlane(s);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    const Seq q = seq_at(c, s);
+    const int hd = c.hd, ndt = hd >> 4, C = a.p.tok_c;
+    const Place at = place_of(c, a.p.tok_n);
+    const Seq q = seq_at(c, at.s);
     const int64_t M = (int64_t)q.n * a.group;
-    if (M == 0 || (TOK && M > a.p.lo)) return;
-    const int64_t row0 = (int64_t)q.a * a.nh + h * a.group;  // output row of m: row0 + (m / group) * nh + m % group
+    if (M == 0 || M > a.p.lo) return;
+    const int64_t row0 = (int64_t)q.a * a.nh + at.h * a.group;  // output row of m: row0 + (m / group) * nh + m % group
     if (!q.ok) {
-        if (chunk == 0 && tile == 0)
-            for (int i = wave; i < q.n; i += 4)
-                for (int x = lane; x < a.group * hd; x += 64)
-                    store1<BF>(a.out, (row0 + (int64_t)i * a.nh) * hd + x, __builtin_nanf(""));
+        if (at.chunk == 0) fill_nan<BF>(a, q, at.h, wave, lane);
         return;
     }
-    const int m_tile = tile * MT;
-    const int m_last = (int)min(M, (int64_t)m_tile + MT) - 1;
-    const int seen = q.p0 + m_last / a.group + 1;  // keys that the tile's last row sees
-    const int key0 = chunk * C, key1 = min(key0 + C, seen);
+    const int seen = q.p0 + q.n;  // keys that the last row sees
+    const int key0 = at.chunk * C, key1 = min(key0 + C, seen);
     if (key0 >= key1) return;
-    const int32_t* table = c.pages + (int64_t)s * c.max_pages;
-
-    // ---- queries
-    const int m_wave = m_tile + (TOK ? 0 : 16 * NT * wave);
-    int vis[NT];           // keys that this lane's query row sees
-    int64_t orow[NT];      // its output row, -1: none
-    float cq[NT];          // log2 units of one unit of the scaled product
-    h8 qv[PARTS][NT][2 * NJ];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-        const int m = m_wave + 16 * u + n;
-        const bool on = m <= m_last;
-        const int mm = on ? m : m_last;
-        const int i = mm / a.group;
-        vis[u] = q.p0 + i + 1;
-        const int64_t r = row0 + (int64_t)i * a.nh + (mm - i * a.group);
-        orow[u] = on ? r : -1;
-        float f[NJ][16];
-        float am = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int d = 16 * (4 * j + g);
-            if (BF) {
-                uint4 w[2] = {};
-                if (d < hd) {
-                    w[0] = *(const uint4*)((const uint16_t*)a.q + r * hd + d);
-                    w[1] = *(const uint4*)((const uint16_t*)a.q + r * hd + d + 8);
-                }
-                widen16<XK_BF16>(w, f[j]);
-            } else {
-                uint4 w[4] = {};
-                if (d < hd)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) w[x] = *(const uint4*)((const float*)a.q + r * hd + d + 4 * x);
-                widen16<XK_F32>(w, f[j]);
-            }
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                am = fmaxf(am, __builtin_fabsf(f[j][x]));
-                bad |= !(__builtin_fabsf(f[j][x]) < __builtin_inff());
-            }
-        }
-        am = xor16_max(bad ? __builtin_inff() : am);
-        const bool fin = am < __builtin_inff();
-        const int sh = fin ? min(14 - expo(am), 120) : 0;
-        const float up = exp2i(sh);
-        cq[u] = fin ? __fmul_rn(a.scale_log2, exp2i(-sh)) : __builtin_nanf("");
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float y = fin ? __fmul_rn(f[j][x], up) : 0.0f;
-                const _Float16 hi = (_Float16)y;
-                qv[0][u][2 * j + (x >> 3)][x & 7] = hi;
-                if (PARTS == 2) qv[PARTS - 1][u][2 * j + (x >> 3)][x & 7] = (_Float16)__fsub_rn(y, (float)hi);
-            }
-    }
-
-    // ---- keys
-    float mx[NT], l[NT];
-    int ve[NT];  // exponent that the weights are scaled by
-    f4 o[DT][NT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-        mx[u] = -__builtin_inff();
-        l[u] = 0.0f;
-        ve[u] = -110;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
     const int last_grp = (key1 - 1) >> 4;
-    const int vis_least = q.p0 + min(m_wave, m_last) / a.group + 1;
-    for (int kb = key0 + (TOK ? 64 * wave : 0); kb < key1; kb += TOK ? 256 : 64) {
-        // pages of this lane's groups: of the key row it loads, of the keys whose scales and values it takes
-        int ik, iv;
-        const int pk = page_of(c, table, min((kb >> 4) + (n >> 2), last_grp), &ik);
-        const int pv = page_of(c, table, min((kb >> 4) + g, last_grp), &iv);
-        const uint8_t* kp = c.k + (((int64_t)max(pk, 0) * c.nkv + h) * c.ps + 16 * ik + (n & 3)) * hd;
-        const int64_t sv = ((int64_t)max(pv, 0) * c.nkv + h) * c.ps + 16 * iv;
+
+    Queries<NJ, 1, BF> qs;
+    qs.load(a, q, row0, 0, (int)M - 1, lane);
+    Running<DT> r;
+    r.clear();
+    auto step = [&](int kb, auto masked) {
+        // a lane loads a key row of group n / 4, and takes the scales and values of group g
+        const int64_t s0 = group_slot(c, table, kb >> 4, last_grp, at.h), s1 = group_slot(c, table, (kb >> 4) + 1, last_grp, at.h),
+                      s2 = group_slot(c, table, (kb >> 4) + 2, last_grp, at.h), s3 = group_slot(c, table, (kb >> 4) + 3, last_grp, at.h);
+        const uint8_t* kp = c.k + (max(pick(n >> 2, s0, s1, s2, s3), (int64_t)0) + (n & 3)) * hd;
+        const int64_t own = pick(g, s0, s1, s2, s3), sv = max(own, (int64_t)0);
         const uint8_t* vp = c.v + sv * hd + 16 * n;
         uint4 kw[4][NJ];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int d = 16 * (4 * j + g);
-                kw[t][j] = *(const uint4*)(kp + 4 * t * hd + (d < hd ? d : 0));
-            }
-        f4 ksc[4], vsc[4];
+            for (int j = 0; j < NJ; ++j) kw[t][j] = *(const uint4*)(kp + 4 * t * hd + 16 * (4 * j + g < ndt ? 4 * j + g : 0));
+        f4 ks[4], vs[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            ksc[t] = *(const f4*)(c.ks + sv + 4 * t);
-            vsc[t] = *(const f4*)(c.vs + sv + 4 * t);
-            if (pv < 0) ksc[t] = f4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            ks[t] = *(const f4*)(c.ks + sv + 4 * t);
+            vs[t] = *(const f4*)(c.vs + sv + 4 * t);
         }
         uint4 vw[DT];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) vw[d] = d < ndt ? *(const uint4*)(vp + 256 * d) : uint4{};
+        for (int d = 0; d < DT; ++d) vw[d] = *(const uint4*)(vp + 256 * min(d, ndt - 1));
+        const float lost = own < 0 ? __builtin_nanf("") : 0.0f;
 
-        f4 sc[NT][4];
+        f4 sc[4];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) sc[u][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+            sc[t] = f4{lost, lost, lost, lost};
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const h8 k0 = widen8(kw[t][j].x, kw[t][j].y), k1 = widen8(kw[t][j].z, kw[t][j].w);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) {
-                        sc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qv[p][u][2 * j], sc[u][t], 0, 0, 0);
-                        sc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qv[p][u][2 * j + 1], sc[u][t], 0, 0, 0);
-                    }
-            }
-
-        h8 pw[PARTS][NT][2];
-        const int kl = kb + 16 * g;               // this lane's first key
-        const bool full = kb + 64 <= vis_least;  // every row of the wave sees every key
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            f4 vm[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                vm[t] = vsc[t];
-                sc[u][t] *= ksc[t];
-            }
-            if (!full) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool see = kl + 4 * t + e < vis[u];
-                        sc[u][t][e] = see ? sc[u][t][e] : -__builtin_inff();
-                        vm[t][e] = see ? vm[t][e] : 0.0f;
-                    }
-            }
-            float big = -__builtin_inff(), vmax = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    big = fmaxf(big, sc[u][t][e]);
-                    const float av = __builtin_fabsf(vm[t][e]);
-                    vmax = av < __builtin_inff() ? fmaxf(vmax, av) : vmax;
+                for (int p = 0; p < PARTS; ++p) {
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qs.v[p][0][2 * j], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qs.v[p][0][2 * j + 1], sc[t], 0, 0, 0);
                 }
-            const float mnew = fmaxf(mx[u], xor16_max(big));
-            const int enew = max(ve[u], expo(xor16_max(vmax)));
-            const float ref = mnew == -__builtin_inff() ? 0.0f : __fmul_rn(mnew, cq[u]);
-            const float alpha = mx[u] == -__builtin_inff() ? 0.0f
-                                                           : __builtin_amdgcn_exp2f(__fmaf_rn(mx[u], cq[u], -ref));
-            const float oscale = __builtin_ldexpf(alpha, ve[u] - enew);
-            l[u] = __fmul_rn(l[u], alpha);
+            }
+            sc[t] *= ks[t];
+        }
+        h8 pw[PARTS][2];
+        if (masked) {
+            const int vis = q.p0 + row_of(a, min(n, (int)M - 1)) + 1;  // keys that this lane's row sees
+            r.template weigh_masked<PARTS>(sc, vs, kb + 16 * g, vis, qs.cq[0], pw);
+        } else {
+            const int e = max(r.ve, expo(r.largest(vs)));
+            if (__any(e != r.ve)) r.raise(e);
+            const float up = exp2i(kVUp - r.ve);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][u] *= oscale;
-            mx[u] = mnew;
-            ve[u] = enew;
-            const float vup = exp2i(min(14 - enew, 124));
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(__fmaf_rn(sc[u][t][e], cq[u], -ref));
-                    l[u] = __fadd_rn(l[u], p);
-                    float w = __fmul_rn(p, __fmul_rn(vm[t][e], vup));
-                    if (PARTS == 2) as_rounded(w);
-                    const _Float16 hi = (_Float16)w;
-                    pw[0][u][t >> 1][4 * (t & 1) + e] = hi;
-                    if (PARTS == 2) pw[PARTS - 1][u][t >> 1][4 * (t & 1) + e] = (_Float16)__fsub_rn(w, (float)hi);
-                }
+            for (int t = 0; t < 4; ++t) vs[t] *= up;
+            r.template weigh<PARTS>(sc, vs, qs.cq[0], pw);
         }
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-            if (d < ndt) {
-                const h8 v0 = widen8(vw[d].x, vw[d].y), v1 = widen8(vw[d].z, vw[d].w);
+        for (int d = 0; d < DT; ++d) {
+            const h8 v0 = widen8(vw[d].x, vw[d].y), v1 = widen8(vw[d].z, vw[d].w);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) {
-                        o[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pw[p][u][0], o[d][u], 0, 0, 0);
-                        o[d][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pw[p][u][1], o[d][u], 0, 0, 0);
-                    }
+            for (int p = 0; p < PARTS; ++p) {
+                r.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pw[p][0], r.o[d], 0, 0, 0);
+                r.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pw[p][1], r.o[d], 0, 0, 0);
             }
+        }
+    };
+    int kb = key0 + 64 * wave;
+    for (; kb + 64 <= min(key1, q.p0 + 1); kb += 256) step(kb, False{});  // every row sees every key
+    for (; kb < key1; kb += 256) step(kb, True{});
+
+    const float l = xor16_sum(r.l), unit = r.unit();
+    if (g == 0) {
+        s_m[wave][n] = r.ref;
+        s_l[wave][n] = l;
     }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *(f4*)&s_o[wave][n][16 * d + 4 * g] = r.o[d] * unit;
+    __syncthreads();
+    const bool whole = seen <= C;  // the sequence is one chunk
+    for (int x = threadIdx.x; x < (int)M * (hd >> 2); x += 256) {
+        const int m = x / (hd >> 2), d = 4 * (x - m * (hd >> 2));
+        float top = fmaxf(fmaxf(s_m[0][m], s_m[1][m]), fmaxf(s_m[2][m], s_m[3][m]));
+        top = top == -__builtin_inff() ? 0.0f : top;
+        float sum = 0.0f;
+        f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float b = __builtin_amdgcn_exp2f(__fsub_rn(s_m[w][m], top));
+            sum = __fmaf_rn(b, s_l[w][m], sum);
+            const f4 ow = *(const f4*)&s_o[w][m][d];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, ow[e], v[e]);
+        }
+        const int i = row_of(a, m);
+        const int64_t row = row0 + (int64_t)i * a.nh + (m - i * a.group);
+        if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
+            store4<BF>(a.out, row * hd + d, v);
+        } else {
+            const int64_t part = row * a.parts + at.chunk;
+            store4<false>(a.part_o, part * hd + d, v);
+            if (d == 0) *(float2*)(a.part_ml + 2 * part) = make_float2(top, sum);
+        }
+    }
+}
 
-    // ---- out, or the chunk's part of it
-    const bool whole = q.p0 + q.n <= C;  // the sequence is one chunk
-#pragma unroll
-    for (int u = 0; u < NT; ++u) l[u] = xor16_sum(l[u]);
-    if (TOK) {
-        __shared__ float s_o[4][16][16 * DT + 4];
-        __shared__ float s_m[4][16], s_l[4][16];
-        const float down = exp2i(max(ve[0] - 14, -124));
-        const float m2 = mx[0] == -__builtin_inff() ? mx[0] : __fmul_rn(mx[0], cq[0]);
-        if (g == 0) {
-            s_m[wave][n] = m2;
-            s_l[wave][n] = l[0];
+// The tile form: 64 NT query rows of a sequence, 16 NT a wave, every key to all four
+// waves.  grid nkv * chunks * tiles, block 256.  Each wave widens a quarter of the
+// next 64 keys' codes while the present ones are worked on: they lie in LDS as
+// operand fragments (64 lanes x 16 bytes, read and written without conflicts), so a
+// code is widened once a workgroup instead of once a wave.
+template <int DT, int NT, bool BF>
+__global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
+{
+    constexpr int NJ = (DT + 3) / 4;
+    constexpr int PARTS = BF ? 1 : 2;
+    constexpr int MT = 64 * NT;
+    __shared__ __align__(16) h8 s_k[2][4][2 * NJ][64];
+    __shared__ __align__(16) h8 s_v[2][DT][2][64];
+    __shared__ __align__(16) float s_ks[2][64], s_vs[2][64];
+    __shared__ float s_top[2];
+    const Paged& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int hd = c.hd, ndt = hd >> 4, C = a.p.tile_c;
+    Place at = place_of(c, a.p.tile_n);
+
+    // the sequence that the tile belongs to: sequences of more than `lo` query rows have
+    // one for every MT of them
+    at.s = -1;
+    for (int base = 0; base < c.n_seqs; base += 64) {
+        int mine = 0;
+        if (base + lane < c.n_seqs) {
+            const int64_t rows = (int64_t)seq_at(c, base + lane).n * a.group;
+            mine = rows > a.p.lo ? (int)((rows + MT - 1) / MT) : 0;
         }
+        int upto = mine;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-            if (d < ndt) *(f4*)&s_o[wave][n][16 * d + 4 * g] = o[d][0] * down;
-        __syncthreads();
-        const int rows = m_last + 1;
-        for (int x = threadIdx.x; x < rows * (hd >> 2); x += 256) {
-            const int m = x / (hd >> 2), d = 4 * (x - m * (hd >> 2));
-            float top = s_m[0][m];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][m]);
-            top = top == -__builtin_inff() ? 0.0f : top;
-            float sum = 0.0f;
-            f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float b = __builtin_amdgcn_exp2f(__fsub_rn(s_m[w][m], top));
-                sum = __fmaf_rn(b, s_l[w][m], sum);
-                const f4 ow = *(const f4*)&s_o[w][m][d];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, ow[e], v[e]);
-            }
-            const int i = m / a.group;
-            const int64_t r = row0 + (int64_t)i * a.nh + (m - i * a.group);
-            if (whole) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
-                store4<BF>(a.out, r * hd + d, v);
-            } else {
-                const int64_t at = r * a.parts + chunk;
-                store4<false>(a.part_o, at * hd + d, v);
-                if (d == 0) *(float2*)(a.part_ml + 2 * at) = make_float2(top, sum);
-            }
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(upto, off, 64);
+            upto += lane >= off ? o : 0;
         }
+        const uint64_t past = __ballot(upto > at.tile);
+        if (past) {
+            const int hit = __ffsll((unsigned long long)past) - 1;
+            at.s = base + hit;
+            at.tile -= __builtin_amdgcn_readlane(upto - mine, hit);
+            break;
+        }
+        at.tile -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    at.s = __builtin_amdgcn_readfirstlane(at.s);
+    at.tile = __builtin_amdgcn_readfirstlane(at.tile);
+    if (at.s < 0) return;
+    const Seq q = seq_at(c, at.s);
+    const int64_t M = (int64_t)q.n * a.group;
+    const int64_t row0 = (int64_t)q.a * a.nh + at.h * a.group;
+    if (!q.ok) {
+        if (at.chunk == 0 && at.tile == 0) fill_nan<BF>(a, q, at.h, wave, lane);
         return;
     }
+    const int m_tile = at.tile * MT;
+    const int m_wave = m_tile + 16 * NT * wave;
+    const int m_last = (int)min(M, (int64_t)m_tile + MT) - 1;
+    const int seen = q.p0 + row_of(a, m_last) + 1;  // keys that the tile's last row sees
+    const int key0 = at.chunk * C, key1 = min(key0 + C, seen);
+    if (key0 >= key1) return;
+    const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
+    const int last_grp = (key1 - 1) >> 4;
+
+    // this wave's share of 64 keys: key tile t = wave of k, value tiles wave, wave + 4 of v,
+    // the scales (waves 0 and 1)
+    uint4 kw[NJ], vw[NJ];
+    float scale = 0.0f;
+    auto fetch = [&](int kb) {
+        const int64_t s0 = group_slot(c, table, kb >> 4, last_grp, at.h), s1 = group_slot(c, table, (kb >> 4) + 1, last_grp, at.h),
+                      s2 = group_slot(c, table, (kb >> 4) + 2, last_grp, at.h), s3 = group_slot(c, table, (kb >> 4) + 3, last_grp, at.h);
+        // offsets made anew from the lane each time: the compiler kept them across the
+        // loop as 64-bit addresses, and spilled
+        int ln = lane;
+        asm("" : "+v"(ln));
+        const int n = ln & 15, g = ln >> 4, g16 = 16 * g;
+        const int koff = ((n & 3) + 4 * wave) * hd, voff = 16 * n;
+        const int64_t kat = max(pick(n >> 2, s0, s1, s2, s3), (int64_t)0) * hd;
+        const int64_t own = pick(g, s0, s1, s2, s3), sv = max(own, (int64_t)0);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int ko = 64 * j + g16;
+            kw[j] = *(const uint4*)(c.k + (kat + (koff + (ko < hd ? ko : 0))));
+            vw[j] = *(const uint4*)(c.v + (sv * hd + (voff + 256 * min(wave + 4 * j, ndt - 1))));
+        }
+        const float v = (wave & 1 ? c.vs : c.ks)[sv + n];
+        scale = own < 0 ? __builtin_nanf("") : v;
+    };
+    auto put = [&](int b) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            s_k[b][wave][2 * j][lane] = widen8(kw[j].x, kw[j].y);
+            s_k[b][wave][2 * j + 1][lane] = widen8(kw[j].z, kw[j].w);
+            if (wave + 4 * j < DT) {
+                s_v[b][wave + 4 * j][0][lane] = widen8(vw[j].x, vw[j].y);
+                s_v[b][wave + 4 * j][1][lane] = widen8(vw[j].z, vw[j].w);
+            }
+        }
+        if (wave == 0) s_ks[b][lane] = scale;
+        if (wave == 1) {
+            s_vs[b][lane] = scale;
+            const uint32_t m = __float_as_uint(scale) & 0x7FFFFFFFu;
+            const uint32_t top = wave_max_dpp(m < 0x7F800000u ? m : 0u);  // of finite ones
+            if (lane == 0) s_top[b] = __uint_as_float(top);
+        }
+    };
+
+    Running<DT> r[NT];
+    Queries<NJ, NT, BF> qs;
+    auto step = [&](int kb, int b, auto masked) {
+        if (kb + 64 < key1) fetch(kb + 64);
+        f4 sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const f4 ks = *(const f4*)&s_ks[b][16 * g + 4 * t];
+#pragma unroll
+            for (int u = 0; u < NT; ++u) sc[u][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 2 * NJ; ++j) {
+                const h8 k = s_k[b][t][j][lane];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+                        sc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qs.v[p][u][j], sc[u][t], 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < NT; ++u) sc[u][t] *= ks;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f4 vs[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vs[t] = *(const f4*)&s_vs[b][16 * g + 4 * t];
+        h8 pw[NT][PARTS][2];
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                int m = m_wave + 16 * u + n;
+                asm("" : "+v"(m));  // not kept across the loop
+                const int vis = q.p0 + row_of(a, min(m, m_last)) + 1;  // keys that this lane's row sees
+                r[u].template weigh_masked<PARTS>(sc[u], vs, kb + 16 * g, vis, qs.cq[u], pw[u]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // every row sees every key, and so far saw the same: their ve are one
+            const int e = max(r[0].ve, expo(s_top[b]));
+            if (e != r[0].ve)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) r[u].raise(e);
+            const float up = exp2i(kVUp - r[0].ve);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) vs[t] *= up;
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                r[u].template weigh<PARTS>(sc[u], vs, qs.cq[u], pw[u]);
+                __builtin_amdgcn_sched_barrier(0);  // one tile's temporaries at a time
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const h8 v = s_v[b][d][x][lane];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+                        r[u].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[u][p][x], r[u].o[d], 0, 0, 0);
+            }
+        if (kb + 64 < key1) put(b ^ 1);
+        __syncthreads();
+    };
+
+    fetch(key0);
+    qs.load(a, q, row0, m_wave, m_last, lane);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) r[u].clear();
+    put(0);
+    __syncthreads();
+    const int vis_least = q.p0 + row_of(a, m_tile) + 1;
+    int b = 0, kb = key0;
+    for (; kb + 64 <= min(key1, vis_least); kb += 64, b ^= 1) step(kb, b, False{});
+    for (; kb < key1; kb += 64, b ^= 1) step(kb, b, True{});
+
+    const bool whole = q.p0 + q.n <= C;  // the sequence is one chunk
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        if (orow[u] < 0) continue;
-        const float down = exp2i(max(ve[u] - 14, -124));
-        const int64_t at = orow[u] * a.parts + chunk;
+        const float l = xor16_sum(r[u].l), unit = r[u].unit();
+        int m = m_wave + 16 * u + n;
+        asm("" : "+v"(m));
+        const int i = row_of(a, m);
+        if (m > m_last) continue;
+        const int64_t row = row0 + (int64_t)i * a.nh + (m - i * a.group), part = row * a.parts + at.chunk;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (d < ndt) {
-                f4 v = o[d][u] * down;
+                f4 v = r[u].o[d] * unit;
                 if (whole) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], l[u]);
-                    store4<BF>(a.out, orow[u] * hd + 16 * d + 4 * g, v);
+                    for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], l);
+                    store4<BF>(a.out, row * hd + 16 * d + 4 * g, v);
                 } else {
-                    store4<false>(a.part_o, at * hd + 16 * d + 4 * g, v);
+                    store4<false>(a.part_o, part * hd + 16 * d + 4 * g, v);
                 }
             }
         if (!whole && g == 0)
-            *(float2*)(a.part_ml + 2 * at) =
-                make_float2(mx[u] == -__builtin_inff() ? 0.0f : __fmul_rn(mx[u], cq[u]), l[u]);
+            *(float2*)(a.part_ml + 2 * part) = make_float2(r[u].ref == -__builtin_inff() ? 0.0f : r[u].ref, l);
     }
 }
 
 // ---------------------------------------------------------------------------
 // k_paged_merge
 // ---------------------------------------------------------------------------
-// grid (rows, ceil(nh / 4)), block 256, a wave per (row, head): the chunks' outputs
-// weighed by 2^(m_c - max m), in chunk order.
-template <bool BF>
+// The chunks' outputs of a (row, head) weighed by 2^(m_c - max m).  Its threads are
+// sets of 32 lanes, a chunk a set and 4 values a lane: W = 1: a wave a (row, head),
+// for few chunks; W = 4: a workgroup, its sets' sums added in order in LDS.
+// grid (rows, ceil(nh / (4 / W))), block 256.
+template <int W, bool BF>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedAttn a)
 {
+    __shared__ f4 s_v[4][32];
+    __shared__ float s_sum[4];
     const Paged& c = a.c;
-    const int t = blockIdx.x, lane = threadIdx.x & 63;
-    const int head = 4 * blockIdx.y + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int head = W == 1 ? 4 * blockIdx.y + wave : blockIdx.y;
     if (head >= a.nh) return;
     const int s = find_seq(c, t, lane);
     if (s < 0 || s >= c.n_seqs) return;
@@ -650,17 +903,46 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttn a)
     for (int x = lane; x < nc; x += 64) top = fmaxf(top, a.part_ml[2 * (at + x)]);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const int hd = c.hd, d0 = lane, d1 = lane + 64;
-    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int x = 0; x < nc; ++x) {
-        const float2 ml = *(const float2*)(a.part_ml + 2 * (at + x));
-        const float b = __builtin_amdgcn_exp2f(__fsub_rn(ml.x, top));
-        sum = __fmaf_rn(b, ml.y, sum);
-        if (d0 < hd) o0 = __fmaf_rn(b, a.part_o[(at + x) * hd + d0], o0);
-        if (d1 < hd) o1 = __fmaf_rn(b, a.part_o[(at + x) * hd + d1], o1);
+    const int hd = c.hd, d = 4 * (lane & 31), set = lane >> 5;
+    float sum = 0.0f;
+    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int STEP = 2 * W, U = 4;
+    for (int x0 = 2 * (W == 1 ? 0 : wave) + set; x0 < nc; x0 += STEP * U) {
+        f4 o[U];
+        float2 ml[U];
+#pragma unroll
+        for (int y = 0; y < U; ++y) {
+            const int64_t x = at + min(x0 + STEP * y, nc - 1);
+            ml[y] = *(const float2*)(a.part_ml + 2 * x);
+            o[y] = d < hd ? *(const f4*)(a.part_o + x * hd + d) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+            if (x0 + STEP * y < nc) {
+                const float b = __builtin_amdgcn_exp2f(__fsub_rn(ml[y].x, top));
+                sum = __fmaf_rn(b, ml[y].y, sum);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, o[y][e], v[e]);
+            }
     }
-    if (d0 < hd) store1<BF>(a.out, r * hd + d0, __fdiv_rn(o0, sum));
-    if (d1 < hd) store1<BF>(a.out, r * hd + d1, __fdiv_rn(o1, sum));
+    sum = __fadd_rn(sum, __shfl_xor(sum, 32, 64));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __fadd_rn(v[e], __shfl_xor(v[e], 32, 64));
+    if (W > 1) {
+        if (lane < 32) s_v[wave][lane] = v;
+        if (lane == 0) s_sum[wave] = sum;
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < 4; ++w) {
+            sum = __fadd_rn(sum, s_sum[w]);
+            v += s_v[w][lane & 31];
+        }
+    }
+    if (lane < 32 && d < hd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
+        store4<BF>(a.out, r * hd + d, v);
+    }
 }
 
 AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c)
@@ -689,24 +971,29 @@ bool paged_attention_fits(const Paged& c, const AttnPlan& p)
     return (int64_t)c.nkv * p.tok_n * c.n_seqs <= most && (int64_t)c.nkv * p.tile_n * p.tiles <= most;
 }
 
-template <int NJ, bool BF>
+template <int DT, bool BF>
 static hipError_t launch_attn(const PagedAttn& a, hipStream_t st)
 {
     if (a.p.tok_n)
-        hipLaunchKernelGGL((k_paged_attn<NJ, 1, true, BF>), dim3((unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs)), dim3(256),
-                           0, st, a);
+        hipLaunchKernelGGL((k_paged_tok<DT, BF>), dim3((unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs)), dim3(256), 0, st, a);
     if (a.p.tile_n)
-        hipLaunchKernelGGL((k_paged_attn<NJ, kTileRows / 64, false, BF>),
-                           dim3((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles)), dim3(256), 0, st, a);
-    if (a.parts > 1)
-        hipLaunchKernelGGL(k_paged_merge<BF>, dim3((unsigned)a.c.rows, (unsigned)((a.nh + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_paged_tile<DT, kTileRows / 64, BF>), dim3((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles)),
+                           dim3(256), 0, st, a);
+    if (a.parts > 8)
+        hipLaunchKernelGGL((k_paged_merge<4, BF>), dim3((unsigned)a.c.rows, (unsigned)a.nh), dim3(256), 0, st, a);
+    else if (a.parts > 1)
+        hipLaunchKernelGGL((k_paged_merge<1, BF>), dim3((unsigned)a.c.rows, (unsigned)((a.nh + 3) / 4)), dim3(256), 0, st,
+                           a);
     return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(const PagedAttn& a, hipStream_t st)
 {
-    if (a.c.hd <= 64) return a.bf ? launch_attn<1, true>(a, st) : launch_attn<1, false>(a, st);
-    return a.bf ? launch_attn<2, true>(a, st) : launch_attn<2, false>(a, st);
+    // tiles of 16 values, in twos
+    if (a.c.hd <= 32) return a.bf ? launch_attn<2, true>(a, st) : launch_attn<2, false>(a, st);
+    if (a.c.hd <= 64) return a.bf ? launch_attn<4, true>(a, st) : launch_attn<4, false>(a, st);
+    if (a.c.hd <= 96) return a.bf ? launch_attn<6, true>(a, st) : launch_attn<6, false>(a, st);
+    return a.bf ? launch_attn<8, true>(a, st) : launch_attn<8, false>(a, st);
 }
 
 }  // namespace btl

@@ -18,9 +18,10 @@ struct Paged {
     const int32_t* pos;
     const int32_t* pages;
     int n_pages, nkv, ps, hd;
-    int ppg, ppg_shift;  // groups of 16 slots a page, and its log2 (-1: no power of two)
+    int ppg;             // groups of 16 slots a page
+    uint32_t ppg_mul;    // ceil(2^31 / ppg): g / ppg = (2 g * ppg_mul) >> 32 for g < 2^19, ppg <= 2^12
     int n_seqs, max_pages, rows, max_rows;
-    int cap;             // tokens a sequence may have: min(max_len, max_pages * ps)
+    int cap;             // tokens a sequence may have: min(max_len, max_pages * ps, 2^23)
 };
 
 struct PagedAppend {
@@ -69,6 +70,7 @@ struct PagedAttn {
     AttnPlan p;
     int parts;
     int nh, group;
+    uint32_t group_mul;  // ceil(2^31 / group): m / group = (2 m * group_mul) >> 32 for m < 2^27, group <= 16
     float scale_log2;  // log2(e) / sqrt(hd)
     int bf;
 };

@@ -60,14 +60,12 @@ int check_sizes(const btl_kv_paged_t* k, const btl_paged_batch_t* b, btl::Paged*
     c->ps = (int)k->page_size;
     c->hd = (int)k->head_dim;
     c->ppg = c->ps / 16;
-    c->ppg_shift = -1;
-    for (int s = 0; s < 16; ++s)
-        if (c->ppg == 1 << s) c->ppg_shift = s;
+    c->ppg_mul = (uint32_t)((((int64_t)1 << 31) + c->ppg - 1) / c->ppg);
     c->n_seqs = (int)b->n_seqs;
     c->max_pages = (int)b->max_pages;
     c->rows = (int)b->rows;
     c->max_rows = (int)std::min(b->max_rows, b->rows);
-    c->cap = (int)std::min<int64_t>(std::min(b->max_len, b->max_pages * k->page_size), 1 << 30);
+    c->cap = (int)std::min<int64_t>(std::min(b->max_len, b->max_pages * k->page_size), 1 << 23);
     return BTL_OK;
 }
 
@@ -211,6 +209,7 @@ int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_
     a.out = out;
     a.nh = (int)n_heads;
     a.group = (int)n_heads / a.c.nkv;
+    a.group_mul = (uint32_t)((((int64_t)1 << 31) + a.group - 1) / a.group);
     a.scale_log2 = (float)(1.4426950408889634074 / std::sqrt((double)a.c.hd));
     a.bf = dtype == BTL_BF16;
     const hipError_t e = btl::launch_paged_attention(a, (hipStream_t)stream);

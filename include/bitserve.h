@@ -66,8 +66,8 @@ typedef struct btl_kv_paged {
  * max_rows, max_len: the host's bounds on any sequence's rows and on its tokens
  *   with them (pos + rows); they choose launches and split the work.
  * What the device finds wrong is answered there: a sequence with pos < 0, more
- * than max_rows rows or more than min(max_len, max_pages * page_size) tokens has
- * NaN in all its output rows and nothing is appended for it; a row that needs a
+ * than max_rows rows or more than min(max_len, max_pages * page_size, 2^23) tokens
+ * has NaN in all its output rows and nothing is appended for it; a row that needs a
  * page outside [0, n_pages) has NaN (attention, read) or is not stored (append).
  */
 typedef struct btl_paged_batch {
