@@ -492,12 +492,25 @@ __device__ __forceinline__ int64_t group_slot(const Paged& c, const int32_t* tab
     return page < 0 ? -1 : ((int64_t)page * c.nkv + h) * c.ps + 16 * in;
 }
 
-__device__ __forceinline__ int64_t pick(int x, int64_t s0, int64_t s1, int64_t s2, int64_t s3)
-{
-    s0 = x == 1 ? s1 : s0;
-    s0 = x == 2 ? s2 : s0;
-    return x == 3 ? s3 : s0;
-}
+// The slots of 64 neighbouring groups, one a lane: looked up together, so a step
+// takes its four from registers instead of waiting for the page table.
+struct Slots {
+    int64_t mine;
+    int base;
+
+    __device__ __forceinline__ void find(const Paged& c, const int32_t* table, int grp, int last_grp, int h, int lane)
+    {
+        base = grp;
+        mine = group_slot(c, table, grp + lane, last_grp, h);
+    }
+    // of group `grp`, base <= grp < base + 64
+    __device__ __forceinline__ int64_t of(int grp) const
+    {
+        const int lo = __builtin_amdgcn_ds_bpermute(4 * (grp - base), (int)(uint32_t)mine);
+        const int hi = __builtin_amdgcn_ds_bpermute(4 * (grp - base), (int)(mine >> 32));
+        return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+    }
+};
 
 // Where a workgroup works: its KV head, chunk of keys and sequence.
 struct Place {
@@ -534,7 +547,7 @@ __device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h
 // from memory into the operands' registers, and are merged in LDS.  DT: 16-value
 // tiles of a head, hd / 16 or one more.
 template <int DT, bool BF>
-__global__ __launch_bounds__(256) void k_paged_tok(PagedAttn a)
+__global__ __launch_bounds__(256, 2) void k_paged_tok(PagedAttn a)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;
@@ -561,14 +574,16 @@ __global__ __launch_bounds__(256) void k_paged_tok(PagedAttn a)
 
     Queries<NJ, 1, BF> qs;
     qs.load(a, q, row0, 0, (int)M - 1, lane);
+    Slots slots;
+    slots.find(c, table, (key0 + 64 * wave) >> 4, last_grp, at.h, lane);
     Running<DT> r;
     r.clear();
-    auto step = [&](int kb, auto masked) {
+    for (int kb = key0 + 64 * wave; kb < key1; kb += 256) {
         // a lane loads a key row of group n / 4, and takes the scales and values of group g
-        const int64_t s0 = group_slot(c, table, kb >> 4, last_grp, at.h), s1 = group_slot(c, table, (kb >> 4) + 1, last_grp, at.h),
-                      s2 = group_slot(c, table, (kb >> 4) + 2, last_grp, at.h), s3 = group_slot(c, table, (kb >> 4) + 3, last_grp, at.h);
-        const uint8_t* kp = c.k + (max(pick(n >> 2, s0, s1, s2, s3), (int64_t)0) + (n & 3)) * hd;
-        const int64_t own = pick(g, s0, s1, s2, s3), sv = max(own, (int64_t)0);
+        const int grp = kb >> 4;
+        if (grp + 4 > slots.base + 64) slots.find(c, table, grp, last_grp, at.h, lane);
+        const uint8_t* kp = c.k + (max(slots.of(grp + (n >> 2)), (int64_t)0) + (n & 3)) * hd;
+        const int64_t own = slots.of(grp + g), sv = max(own, (int64_t)0);
         const uint8_t* vp = c.v + sv * hd + 16 * n;
         uint4 kw[4][NJ];
 #pragma unroll
@@ -602,16 +617,16 @@ __global__ __launch_bounds__(256) void k_paged_tok(PagedAttn a)
             sc[t] *= ks[t];
         }
         h8 pw[PARTS][2];
-        if (masked) {
-            const int vis = q.p0 + row_of(a, min(n, (int)M - 1)) + 1;  // keys that this lane's row sees
-            r.template weigh_masked<PARTS>(sc, vs, kb + 16 * g, vis, qs.cq[0], pw);
-        } else {
+        if (kb + 64 <= q.p0 + 1) {  // every row sees every key
             const int e = max(r.ve, expo(r.largest(vs)));
             if (__any(e != r.ve)) r.raise(e);
             const float up = exp2i(kVUp - r.ve);
 #pragma unroll
             for (int t = 0; t < 4; ++t) vs[t] *= up;
             r.template weigh<PARTS>(sc, vs, qs.cq[0], pw);
+        } else {
+            const int vis = q.p0 + row_of(a, min(n, (int)M - 1)) + 1;  // keys that this lane's row sees
+            r.template weigh_masked<PARTS>(sc, vs, kb + 16 * g, vis, qs.cq[0], pw);
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -622,10 +637,7 @@ __global__ __launch_bounds__(256) void k_paged_tok(PagedAttn a)
                 r.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pw[p][1], r.o[d], 0, 0, 0);
             }
         }
-    };
-    int kb = key0 + 64 * wave;
-    for (; kb + 64 <= min(key1, q.p0 + 1); kb += 256) step(kb, False{});  // every row sees every key
-    for (; kb < key1; kb += 256) step(kb, True{});
+    }
 
     const float l = xor16_sum(r.l), unit = r.unit();
     if (g == 0) {
@@ -732,17 +744,19 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
     // the scales (waves 0 and 1)
     uint4 kw[NJ], vw[NJ];
     float scale = 0.0f;
+    Slots slots;
+    slots.find(c, table, key0 >> 4, last_grp, at.h, lane);
     auto fetch = [&](int kb) {
-        const int64_t s0 = group_slot(c, table, kb >> 4, last_grp, at.h), s1 = group_slot(c, table, (kb >> 4) + 1, last_grp, at.h),
-                      s2 = group_slot(c, table, (kb >> 4) + 2, last_grp, at.h), s3 = group_slot(c, table, (kb >> 4) + 3, last_grp, at.h);
+        const int grp = kb >> 4;
+        if (grp + 4 > slots.base + 64) slots.find(c, table, grp, last_grp, at.h, lane);
         // offsets made anew from the lane each time: the compiler kept them across the
         // loop as 64-bit addresses, and spilled
         int ln = lane;
         asm("" : "+v"(ln));
         const int n = ln & 15, g = ln >> 4, g16 = 16 * g;
         const int koff = ((n & 3) + 4 * wave) * hd, voff = 16 * n;
-        const int64_t kat = max(pick(n >> 2, s0, s1, s2, s3), (int64_t)0) * hd;
-        const int64_t own = pick(g, s0, s1, s2, s3), sv = max(own, (int64_t)0);
+        const int64_t kat = max(slots.of(grp + (n >> 2)), (int64_t)0) * hd;
+        const int64_t own = slots.of(grp + g), sv = max(own, (int64_t)0);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int ko = 64 * j + g16;
