@@ -483,33 +483,22 @@ struct False {
     constexpr operator bool() const { return false; }
 };
 
-// First slot, counted over all pages, of the group of 16 keys `grp` (past the last
-// one: of that) for KV head h; -1: its page is outside the pool.
-__device__ __forceinline__ int64_t group_slot(const Paged& c, const int32_t* table, int grp, int last_grp, int h)
-{
-    int in;
-    const int page = page_of(c, table, min(grp, last_grp), &in);
-    return page < 0 ? -1 : ((int64_t)page * c.nkv + h) * c.ps + 16 * in;
-}
-
-// The slots of 64 neighbouring groups, one a lane: looked up together, so a step
-// takes its four from registers instead of waiting for the page table.
+// The groups of 16 slots, counted over all pages and heads, that hold 64 neighbouring
+// groups of a sequence's keys, one a lane (past its last group: that one; -1: the
+// page is outside the pool).  Looked up together, so a step takes its four from
+// registers instead of waiting for the page table.
 struct Slots {
-    int64_t mine;
-    int base;
+    int mine, base;
 
     __device__ __forceinline__ void find(const Paged& c, const int32_t* table, int grp, int last_grp, int h, int lane)
     {
+        int in;
+        const int page = page_of(c, table, min(grp + lane, last_grp), &in);
+        mine = page < 0 ? -1 : (page * c.nkv + h) * c.ppg + in;  // below 2^31: the host checks it
         base = grp;
-        mine = group_slot(c, table, grp + lane, last_grp, h);
     }
     // of group `grp`, base <= grp < base + 64
-    __device__ __forceinline__ int64_t of(int grp) const
-    {
-        const int lo = __builtin_amdgcn_ds_bpermute(4 * (grp - base), (int)(uint32_t)mine);
-        const int hi = __builtin_amdgcn_ds_bpermute(4 * (grp - base), (int)(mine >> 32));
-        return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
-    }
+    __device__ __forceinline__ int of(int grp) const { return __builtin_amdgcn_ds_bpermute(4 * (grp - base), mine); }
 };
 
 // Where a workgroup works: its KV head, chunk of keys and sequence.
@@ -582,9 +571,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_tok(PagedAttn a)
         // a lane loads a key row of group n / 4, and takes the scales and values of group g
         const int grp = kb >> 4;
         if (grp + 4 > slots.base + 64) slots.find(c, table, grp, last_grp, at.h, lane);
-        const uint8_t* kp = c.k + (max(slots.of(grp + (n >> 2)), (int64_t)0) + (n & 3)) * hd;
-        const int64_t own = slots.of(grp + g), sv = max(own, (int64_t)0);
-        const uint8_t* vp = c.v + sv * hd + 16 * n;
+        const int own = slots.of(grp + g), at_v = max(own, 0);
+        const uint8_t* kp = c.k + (uint64_t)(uint32_t)max(slots.of(grp + (n >> 2)), 0) * (uint32_t)(16 * hd) + (n & 3) * hd;
+        const uint8_t* vp = c.v + (uint64_t)(uint32_t)at_v * (uint32_t)(16 * hd) + 16 * n;
+        const float* kscale = c.ks + 16 * (int64_t)at_v;
+        const float* vscale = c.vs + 16 * (int64_t)at_v;
         uint4 kw[4][NJ];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -593,8 +584,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_tok(PagedAttn a)
         f4 ks[4], vs[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            ks[t] = *(const f4*)(c.ks + sv + 4 * t);
-            vs[t] = *(const f4*)(c.vs + sv + 4 * t);
+            ks[t] = *(const f4*)(kscale + 4 * t);
+            vs[t] = *(const f4*)(vscale + 4 * t);
         }
         uint4 vw[DT];
 #pragma unroll
@@ -744,6 +735,7 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
     // the scales (waves 0 and 1)
     uint4 kw[NJ], vw[NJ];
     float scale = 0.0f;
+    bool lost = false;  // its page is outside the pool
     Slots slots;
     slots.find(c, table, key0 >> 4, last_grp, at.h, lane);
     auto fetch = [&](int kb) {
@@ -755,16 +747,17 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
         asm("" : "+v"(ln));
         const int n = ln & 15, g = ln >> 4, g16 = 16 * g;
         const int koff = ((n & 3) + 4 * wave) * hd, voff = 16 * n;
-        const int64_t kat = max(slots.of(grp + (n >> 2)), (int64_t)0) * hd;
-        const int64_t own = slots.of(grp + g), sv = max(own, (int64_t)0);
+        const int own = slots.of(grp + g), at_v = max(own, 0);
+        const uint8_t* kp = c.k + (uint64_t)(uint32_t)max(slots.of(grp + (n >> 2)), 0) * (uint32_t)(16 * hd);
+        const uint8_t* vp = c.v + (uint64_t)(uint32_t)at_v * (uint32_t)(16 * hd);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int ko = 64 * j + g16;
-            kw[j] = *(const uint4*)(c.k + (kat + (koff + (ko < hd ? ko : 0))));
-            vw[j] = *(const uint4*)(c.v + (sv * hd + (voff + 256 * min(wave + 4 * j, ndt - 1))));
+            kw[j] = *(const uint4*)(kp + (koff + (ko < hd ? ko : 0)));
+            vw[j] = *(const uint4*)(vp + (voff + 256 * min(wave + 4 * j, ndt - 1)));
         }
-        const float v = (wave & 1 ? c.vs : c.ks)[sv + n];
-        scale = own < 0 ? __builtin_nanf("") : v;
+        scale = (wave & 1 ? c.vs : c.ks)[16 * (int64_t)at_v + n];
+        lost = own < 0;
     };
     auto put = [&](int b) {
 #pragma unroll
@@ -776,7 +769,7 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
                 s_v[b][wave + 4 * j][1][lane] = widen8(vw[j].z, vw[j].w);
             }
         }
-        if (wave == 0) s_ks[b][lane] = scale;
+        if (wave == 0) s_ks[b][lane] = lost ? __builtin_nanf("") : scale;
         if (wave == 1) {
             s_vs[b][lane] = scale;
             const uint32_t m = __float_as_uint(scale) & 0x7FFFFFFFu;
@@ -806,6 +799,13 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
             }
 #pragma unroll
             for (int u = 0; u < NT; ++u) sc[u][t] *= ks;
+        }
+        // operands are read some products ahead: LDS answers after some 130 cycles, two products take 32
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+        for (int x = 0; x < 4 * 2 * NJ; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PARTS * NT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         f4 vs[4];
@@ -847,6 +847,12 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
                     for (int u = 0; u < NT; ++u)
                         r[u].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[u][p][x], r[u].o[d], 0, 0, 0);
             }
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+        for (int x = 0; x < 2 * DT; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PARTS * NT, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        }
         if (kb + 64 < key1) put(b ^ 1);
         __syncthreads();
     };

@@ -52,6 +52,8 @@ int check_sizes(const btl_kv_paged_t* k, const btl_paged_batch_t* b, btl::Paged*
         return failf(BTL_ERR_SHAPE, "page_size %lld: need a multiple of 16 up to 65536", (long long)k->page_size);
     if (k->head_dim < 16 || k->head_dim % 16 || k->head_dim > 128)
         return failf(BTL_ERR_SHAPE, "head_dim %lld: need a multiple of 16 up to 128", (long long)k->head_dim);
+    if (k->n_pages * k->n_kv_heads * (k->page_size / 16) >= ((int64_t)1 << 31))
+        return fail_msg(BTL_ERR_SHAPE, "paged cache too large: n_pages * n_kv_heads * page_size / 16 must be below 2^31");
     if (b->n_seqs < 0 || b->n_seqs > (1 << 20) || b->rows < 0 || b->rows > (1 << 23) || b->max_pages < 0 ||
         b->max_pages > (1 << 24) || b->max_rows < 0 || b->max_len < 0)
         return fail_msg(BTL_ERR_SHAPE, "batch size out of range");

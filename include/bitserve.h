@@ -40,8 +40,8 @@ extern "C" {
  *    the tokens innermost (the order in which the attention's second product
  *    takes them: 16 tokens of one value are one load)
  * k_scale, v_scale: [n_pages, n_kv_heads, page_size] f32
- * page_size a multiple of 16, head_dim a multiple of 16 up to 128; k, v 16-byte
- * and the scales 16-byte aligned.
+ * page_size a multiple of 16 up to 65536, head_dim a multiple of 16 up to 128,
+ * n_pages * n_kv_heads * page_size < 2^35; every array 16-byte aligned.
  */
 typedef struct btl_kv_paged {
     uint8_t* k;
