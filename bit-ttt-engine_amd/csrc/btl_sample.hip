@@ -9,7 +9,8 @@
 // complement of the index; "larger word" is "comes first".  top-k, top-p and the
 // draw each ask for one place in that order, by count or by running weight.  No row
 // is sorted: a histogram over bins of (max - l) / T -- in the order's direction --
-// says which bin holds the place, and only that bin's tokens are brought together.
+// says which bin holds the place, and only the tokens of that bin, or of the bins
+// up to it where they are few, are brought together and ordered.
 //
 // Kernels:
 //   k_sample_max   per slice of a row the first token in the order; clears the
@@ -19,6 +20,8 @@
 //   k_sample_pick  per row: the places in turn.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "btl_device.hpp"
 #include "btl_serve.hpp"
 
@@ -27,7 +30,7 @@ namespace btl {
 namespace {
 
 constexpr int kBins = kSampleBins;
-constexpr int kSlice = kSampleSlice;
+constexpr int kFewK = 1024;
 constexpr float kSpan = 28.5f;  // weights are 0 past (max - l) / T = 41 ln 2 = 28.42
 constexpr double kOne = 1099511627776.0;  // 2^40
 constexpr float kMaxF = 3.40282346638528859812e38f;
@@ -55,7 +58,7 @@ __device__ __forceinline__ uint64_t word_of(uint32_t key, uint32_t idx)
 
 // A row's weights: its maximum and temperature (T > 0).
 struct Weigh {
-    double top, t;
+    double top, per_t;
     float topf, per_bin;
     bool inf;  // the maximum is +inf: those tokens alone, alike
 };
@@ -66,19 +69,43 @@ __device__ __forceinline__ Weigh weigh_at(uint32_t top_key, float t)
     w.topf = value_of(top_key);
     w.inf = top_key >= kPlusInf;
     w.top = w.inf ? 0.0 : (double)w.topf;
-    w.t = (double)t;
+    w.per_t = __ddiv_rn(1.0, (double)t);
     w.per_bin = fminf(__fdiv_rn((float)kBins / kSpan, t), kMaxF);  // finite: 0 times it is 0
     return w;
+}
+
+// e^x for -30 < x <= 0 in f64: x = n ln 2 + r with ln 2 in two parts, n * hi exact;
+// e^r, |r| <= ln 2 / 2, by its Taylor polynomial to r^13 / 13! (what is left out is
+// 4e-18 of it) in Horner form; times 2^n.
+__device__ __forceinline__ double exp_f64(double x)
+{
+    const double n = __builtin_rint(__dmul_rn(x, 1.4426950408889634074));
+    const double r = __fma_rn(n, -0x1.ef35793c7673p-45, __fma_rn(n, -0x1.62e42fefa38p-1, x));
+    double p = 1.0 / 6227020800.0;
+    p = __fma_rn(p, r, 1.0 / 479001600.0);
+    p = __fma_rn(p, r, 1.0 / 39916800.0);
+    p = __fma_rn(p, r, 1.0 / 3628800.0);
+    p = __fma_rn(p, r, 1.0 / 362880.0);
+    p = __fma_rn(p, r, 1.0 / 40320.0);
+    p = __fma_rn(p, r, 1.0 / 5040.0);
+    p = __fma_rn(p, r, 1.0 / 720.0);
+    p = __fma_rn(p, r, 1.0 / 120.0);
+    p = __fma_rn(p, r, 1.0 / 24.0);
+    p = __fma_rn(p, r, 1.0 / 6.0);
+    p = __fma_rn(p, r, 0.5);
+    p = __fma_rn(p, r, 1.0);
+    p = __fma_rn(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
 }
 
 // the weight of a logit (2^40 for the largest); 0 for -inf and NaN
 __device__ __forceinline__ uint64_t weight(const Weigh& w, float l)
 {
     if (w.inf) return l == w.topf ? (uint64_t)1 << 40 : 0;
-    if (!(l > -__builtin_inff())) return 0;
-    const double x = ((double)l - w.top) / w.t;
+    const double x = __dmul_rn((double)l - w.top, w.per_t);
+    if (!(x > -30.0)) return 0;
     // adding 2^52 rounds to a whole number, halves to even, and leaves it in the low bits
-    const double y = __dadd_rn(__dmul_rn(exp(x), kOne), 4503599627370496.0);
+    const double y = __dadd_rn(__dmul_rn(exp_f64(x), kOne), 4503599627370496.0);
     return (uint64_t)__double_as_longlong(y) & (((uint64_t)1 << 52) - 1);
 }
 
@@ -86,10 +113,9 @@ __device__ __forceinline__ uint64_t weight(const Weigh& w, float l)
 // order); from kBins on the weight is 0
 __device__ __forceinline__ float place_of(const Weigh& w, float l)
 {
-    return w.inf ? 0.0f : __fmul_rn(fminf(__fsub_rn(w.topf, l), kMaxF), w.per_bin);
+    if (w.inf) return l == w.topf ? 0.0f : (float)kBins;
+    return __fmul_rn(fminf(__fsub_rn(w.topf, l), kMaxF), w.per_bin);
 }
-
-__device__ __forceinline__ int bin_of(const Weigh& w, float l) { return (int)fminf(place_of(w, l), (float)(kBins - 1)); }
 
 struct RowFilters {
     float t;
@@ -113,20 +139,24 @@ __device__ __forceinline__ RowFilters filters_at(const SampleArgs& a, int row)
     return f;
 }
 
+// Whether the bins' weights are asked for: where top-k leaves few tokens they are all
+// brought together, and only counted before.
+__device__ __forceinline__ bool weighed(const RowFilters& f) { return !(f.k > 0 && f.k <= kFewK); }
+
 // Every logit of [i0, i1) of a row to f(value, index), spread over the workgroup's
-// threads, four at a time where the row is 16-byte aligned.
-template <int NTHR, typename F>
+// threads, U loads ahead; four logits a load where the row is 16-byte aligned (i0 is
+// a multiple of 4).
+template <int NTHR, int U, typename F>
 __device__ __forceinline__ void each(const float* x, int i0, int i1, int tid, F f)
 {
-    if (((uintptr_t)x & 15u) == 0) {  // i0 is a multiple of 4
+    if (((uintptr_t)x & 15u) == 0) {
         const int n4 = i1 >> 2;
-        for (int i = (i0 >> 2) + tid; i < n4; i += NTHR * 4) {
-            float4 v[4];
+        for (int i = (i0 >> 2) + tid; i < n4; i += NTHR * U) {
+            float4 v[U];
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (i + NTHR * b < n4) v[b] = ((const float4*)x)[i + NTHR * b];
+            for (int b = 0; b < U; ++b) v[b] = ((const float4*)x)[min(i + NTHR * b, n4 - 1)];
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < U; ++b)
                 if (i + NTHR * b < n4) {
                     const int at = 4 * (i + NTHR * b);
                     f(v[b].x, at);
@@ -135,9 +165,17 @@ __device__ __forceinline__ void each(const float* x, int i0, int i1, int tid, F 
                     f(v[b].w, at + 3);
                 }
         }
-        for (int i = max(4 * n4, i0) + tid; i < i1; i += NTHR) f(x[i], i);
+        const int i = max(4 * n4, i0) + tid;
+        if (i < i1) f(x[i], i);
     } else {
-        for (int i = i0 + tid; i < i1; i += NTHR) f(x[i], i);
+        for (int i = i0 + tid; i < i1; i += NTHR * U) {
+            float v[U];
+#pragma unroll
+            for (int b = 0; b < U; ++b) v[b] = x[min(i + NTHR * b, i1 - 1)];
+#pragma unroll
+            for (int b = 0; b < U; ++b)
+                if (i + NTHR * b < i1) f(v[b], i + NTHR * b);
+        }
     }
 }
 
@@ -171,8 +209,8 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleArgs a)
     const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const float* x = a.logits + (int64_t)row * a.ld;
     uint64_t best = 0;
-    each<256>(x, slice * kSlice, min(a.n, (slice + 1) * kSlice), tid,
-              [&](float v, int i) { best = max(best, word_of(key_of(v), (uint32_t)i)); });
+    each<256, 4>(x, slice * a.slice, min(a.n, (slice + 1) * a.slice), tid,
+                 [&](float v, int i) { best = max(best, word_of(key_of(v), (uint32_t)i)); });
     best = wave_max64(best);
     if ((tid & 63) == 0) s_best[tid >> 6] = best;
     for (int b = slice * 256 + tid; b < kBins; b += a.slices * 256) {
@@ -199,7 +237,8 @@ __device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int row, int t
     return best;
 }
 
-// grid (slices, rows), block 256
+// grid (slices, rows), block 256.  Every token up to the last bin is counted; its
+// weight goes in where min-p keeps it.
 __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a)
 {
     __shared__ uint64_t s_best[4];
@@ -215,19 +254,22 @@ __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a)
     const uint32_t top = (uint32_t)(row_best<4>(a, row, tid, s_best) >> 32);  // holds a barrier
     if (top <= kMinusInf) return;
     const Weigh w = weigh_at(top, f.t);
-    each<256>(a.logits + (int64_t)row * a.ld, slice * kSlice, min(a.n, (slice + 1) * kSlice), tid, [&](float v, int) {
-        if (place_of(w, v) >= (float)kBins) return;
-        const uint64_t m = weight(w, v);
-        if (m < f.least) return;
-        const int b = bin_of(w, v);
-        atomicAdd((unsigned long long*)&s_mass[b], (unsigned long long)m);
-        atomicAdd(&s_count[b], 1u);
-    });
+    const bool weigh = weighed(f);
+    each<256, 1>(a.logits + (int64_t)row * a.ld, slice * a.slice, min(a.n, (slice + 1) * a.slice), tid,
+                 [&](float v, int) {
+                     const float p = place_of(w, v);
+                     if (p >= (float)kBins) return;
+                     atomicAdd(&s_count[(int)p], 1u);
+                     if (!weigh) return;
+                     const uint64_t m = weight(w, v);
+                     if (m >= f.least) atomicAdd((unsigned long long*)&s_mass[(int)p], (unsigned long long)m);
+                 });
     __syncthreads();
     for (int b = tid; b < kBins; b += 256)
         if (s_count[b]) {
-            __hip_atomic_fetch_add(&a.mass[(int64_t)row * kBins + b], s_mass[b], __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
+            if (s_mass[b])
+                __hip_atomic_fetch_add(&a.mass[(int64_t)row * kBins + b], s_mass[b], __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_fetch_add(&a.count[(int64_t)row * kBins + b], s_count[b], __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -236,8 +278,9 @@ __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a)
 namespace {
 
 constexpr int kThr = 512;
+constexpr int kU = 16;       // loads ahead over a whole row
 constexpr int kList = 2048;  // tokens that are ordered at once
-constexpr int kSub = kThr;  // parts that a fuller bin is split into
+constexpr int kSub = kThr;   // parts that a fuller bin is split into
 
 struct PickLds {
     uint64_t mass[kBins];    // running weight up to and with a bin
@@ -278,49 +321,161 @@ __device__ __forceinline__ void scan_pairs(PickLds& s, int tid, uint64_t& m, uin
     }
 }
 
-// Words of the list in order (largest first), then their running weights.
-__device__ __forceinline__ void order_list(PickLds& s, int tid, int c, const Weigh& w)
+// the bins' weights and counts into running ones, two bins a thread
+__device__ __forceinline__ void run_bins(PickLds& s, int tid)
+{
+    static_assert(kBins == 2 * kThr, "two bins a thread");
+    __syncthreads();
+    const uint64_t m1 = s.mass[2 * tid + 1];
+    const uint32_t c1 = s.count[2 * tid + 1];
+    uint64_t m = s.mass[2 * tid] + m1;
+    uint32_t c = s.count[2 * tid] + c1;
+    scan_pairs(s, tid, m, c);  // holds barriers
+    s.mass[2 * tid] = m - m1;
+    s.mass[2 * tid + 1] = m;
+    s.count[2 * tid] = c - c1;
+    s.count[2 * tid + 1] = c;
+    __syncthreads();
+}
+
+// The row, and what is asked of it.
+struct Row {
+    const float* x;
+    int n;
+    Weigh w;
+    uint64_t least;
+};
+
+__device__ __forceinline__ uint64_t kept(const Row& r, uint64_t word)
+{
+    const uint64_t m = weight(r.w, value_of((uint32_t)(word >> 32)));
+    return m >= r.least ? m : 0;
+}
+
+// The smallest logit whose place is before p (place_of falls as the logit rises, so
+// bins are intervals of logits): 32 halvings over the ordered keys.
+__device__ __forceinline__ float first_before(const Weigh& w, float p)
+{
+    uint32_t lo = kMinusInf, hi = kPlusInf;  // place_of(value_of(hi)) < p <= place_of(value_of(lo)), or lo is it
+    if (place_of(w, value_of(lo)) < p) return value_of(lo);
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (place_of(w, value_of(mid)) < p) hi = mid;
+        else lo = mid;
+    }
+    return value_of(hi);
+}
+
+// Every token of bins b0 .. b1 to f(value, index).  The loads run kU ahead and leave
+// a bit a token; f's code is there once, behind them (unrolled with the loads it was
+// fetched slower than it ran).  Two comparisons a token: one workgroup reads the
+// whole row, and three rounded operations a token were more than its loads.
+template <typename F>
+__device__ __forceinline__ void each_in(const Row& r, int tid, int b0, int b1, F f)
+{
+    const float v0 = first_before(r.w, (float)(b1 + 1));
+    const float v1 = b0 > 0 ? first_before(r.w, (float)b0) : __builtin_inff();
+    const bool any = b0 <= 0;  // no upper end
+    auto in = [&](float v) { return v >= v0 && (any || v < v1); };
+    const bool wide = ((uintptr_t)r.x & 15u) == 0;
+    const int per = wide ? 4 : 1;
+    const int m = wide ? r.n >> 2 : r.n;  // loads
+    for (int i0 = tid; i0 < m; i0 += kThr * kU) {
+        uint64_t hit = 0;
+        if (wide) {
+            float4 v[kU];
+#pragma unroll
+            for (int b = 0; b < kU; ++b) v[b] = ((const float4*)r.x)[min(i0 + kThr * b, m - 1)];
+#pragma unroll
+            for (int b = 0; b < kU; ++b) {
+                const float most = fmaxf(fmaxf(v[b].x, v[b].y), fmaxf(v[b].z, v[b].w));
+                if (!__any(most >= v0)) continue;
+                const uint32_t bits = (in(v[b].x) ? 1u : 0u) | (in(v[b].y) ? 2u : 0u) | (in(v[b].z) ? 4u : 0u) |
+                                      (in(v[b].w) ? 8u : 0u);
+                hit |= (uint64_t)(i0 + kThr * b < m ? bits : 0u) << (4 * b);
+            }
+        } else {
+            float v[kU];
+#pragma unroll
+            for (int b = 0; b < kU; ++b) v[b] = r.x[min(i0 + kThr * b, m - 1)];
+#pragma unroll
+            for (int b = 0; b < kU; ++b) hit |= (uint64_t)(i0 + kThr * b < m && in(v[b]) ? 1u : 0u) << b;
+        }
+        while (hit) {
+            const int bit = __ffsll((unsigned long long)hit) - 1;
+            hit &= hit - 1;
+            const int i = wide ? 4 * (i0 + kThr * (bit >> 2)) + (bit & 3) : i0 + kThr * bit;
+            f(r.x[i], i);
+        }
+    }
+    const int i = per * m + tid;
+    if (i < r.n && in(r.x[i])) f(r.x[i], i);
+}
+
+// The words of bins b0 .. b1 from lo to hi into the list, in order, with their running
+// weights; returns how many (at most kList of them are there).
+__device__ __forceinline__ int gather(PickLds& s, const Row& r, int tid, int b0, int b1, uint64_t lo, uint64_t hi)
 {
     __syncthreads();
-    int size = 2;
-    while (size < c) size <<= 1;
-    for (int i = c + tid; i < size; i += kThr) s.list[i] = 0;  // behind every word
+    if (tid == 0) s.fill = 0;
     __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = tid; i < size / 2; i += kThr) {
-                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                const uint64_t x = s.list[lo], y = s.list[hi];
-                if ((x < y) == ((lo & k) == 0)) {
-                    s.list[lo] = y;
-                    s.list[hi] = x;
+    each_in(r, tid, b0, b1, [&](float v, int i) {
+        const uint64_t o = word_of(key_of(v), (uint32_t)i);
+        if (o < lo || o > hi) return;
+        const uint32_t at = atomicAdd(&s.fill, 1u);
+        if (at < kList) s.list[at] = o;
+    });
+    __syncthreads();
+    const int c = (int)min(s.fill, (uint32_t)kList);
+    if (c <= 64) {
+        // one wave, in registers
+        if (tid < 64) {
+            uint64_t v = tid < c ? s.list[tid] : 0;  // 0: behind every word
+#pragma unroll
+            for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+                for (int j = k >> 1; j > 0; j >>= 1) {
+                    const uint64_t o = shfl_xor64(v, j);
+                    v = ((tid & k) == 0) == ((tid & j) == 0) ? max(v, o) : min(v, o);
                 }
-            }
-            __syncthreads();
+            if (tid < c) s.list[tid] = v;
         }
+        __syncthreads();
+    } else {
+        int size = 128;
+        while (size < c) size <<= 1;
+        for (int i = c + tid; i < size; i += kThr) s.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int i = tid; i < size / 2; i += kThr) {
+                    const int at = 2 * i - (i & (j - 1));
+                    const uint64_t x = s.list[at], y = s.list[at + j];
+                    if ((x < y) == ((at & k) == 0)) {
+                        s.list[at] = y;
+                        s.list[at + j] = x;
+                    }
+                }
+                __syncthreads();
+            }
+    }
     uint64_t carry = 0;
     for (int i0 = 0; i0 < c; i0 += kThr) {
         const int i = i0 + tid;
-        uint64_t m = i < c ? weight(w, value_of((uint32_t)(s.list[i] >> 32))) : 0;
+        uint64_t m = i < c ? kept(r, s.list[i]) : 0;
         uint32_t one = 0;
         scan_pairs(s, tid, m, one);
         if (i < c) s.cum[i] = carry + m;
         __syncthreads();
         carry = s.cum[min(i0 + kThr, c) - 1];
     }
+    return c;
 }
 
-// A place in the order: the word there, the running weight up to and with it.
-struct Place {
-    uint64_t word, upto;
-};
-
-// The first token at which the running count reaches `goal` (by_count) or the
-// running weight does.  1 <= goal <= the row's.  `x`, `n`: the row.
-__device__ __forceinline__ Place locate(PickLds& s, const SampleArgs& a, const float* x, const Weigh& w, uint64_t least, int tid,
-                        bool by_count, uint64_t goal)
+// The bin at which the running count reaches `goal` (by_count) or the running weight does.
+__device__ __forceinline__ int bin_at(PickLds& s, int tid, bool by_count, uint64_t goal)
 {
-    // the bin
+    __syncthreads();
     if (tid == 0) s.found = 0;
     __syncthreads();
     for (int b = tid; b < kBins; b += kThr) {
@@ -329,16 +484,44 @@ __device__ __forceinline__ Place locate(PickLds& s, const SampleArgs& a, const f
         if (before < goal && with >= goal) s.found = b;
     }
     __syncthreads();
-    const int bin = s.found;
-    uint64_t mass0 = bin ? s.mass[bin - 1] : 0;                      // weight ahead of what is looked at
+    return s.found;
+}
+
+// The token of the list at which the running count, mass0 and count0 ahead of it,
+// reaches `goal`, or the running weight does.
+__device__ __forceinline__ int list_at(PickLds& s, int tid, int c, uint64_t mass0, uint64_t count0, bool by_count,
+                                       uint64_t goal)
+{
+    __syncthreads();
+    if (tid == 0) s.found = c - 1;
+    __syncthreads();
+    for (int i = tid; i < c; i += kThr) {
+        const uint64_t before = by_count ? count0 + i : mass0 + (i ? s.cum[i - 1] : 0);
+        const uint64_t with = by_count ? count0 + i + 1 : mass0 + s.cum[i];
+        if (before < goal && with >= goal) s.found = i;
+    }
+    __syncthreads();
+    return s.found;
+}
+
+// A place in the order: the word there, the running weight up to and with it.
+struct Place {
+    uint64_t word, upto;
+};
+
+// The first token at which the running count reaches `goal` (by_count) or the
+// running weight does.  1 <= goal <= the row's.
+__device__ __forceinline__ Place locate(PickLds& s, const Row& r, int tid, bool by_count, uint64_t goal)
+{
+    const int bin = bin_at(s, tid, by_count, goal);
+    uint64_t mass0 = bin ? s.mass[bin - 1] : 0;  // weight ahead of what is looked at
     uint64_t count0 = bin ? s.count[bin - 1] : 0;
     uint32_t held = s.count[bin] - (uint32_t)count0;
     uint64_t lo = 0, hi = ~(uint64_t)0;  // words that are looked at
     if (held > kList) {
         // too many to order: their words' range first
         uint64_t wl = ~(uint64_t)0, wh = 0;
-        each<kThr>(x, 0, a.n, tid, [&](float v, int i) {
-            if (bin_of(w, v) != bin || weight(w, v) < least) return;
+        each_in(r, tid, bin, bin, [&](float v, int i) {
             const uint64_t o = word_of(key_of(v), (uint32_t)i);
             wl = min(wl, o);
             wh = max(wh, o);
@@ -367,14 +550,11 @@ __device__ __forceinline__ Place locate(PickLds& s, const SampleArgs& a, const f
             s.sub_count[i] = 0;
         }
         __syncthreads();
-        each<kThr>(x, 0, a.n, tid, [&](float v, int i) {
-            if (bin_of(w, v) != bin) return;
+        each_in(r, tid, bin, bin, [&](float v, int i) {
             const uint64_t o = word_of(key_of(v), (uint32_t)i);
             if (o < lo || o > hi) return;
-            const uint64_t m = weight(w, v);
-            if (m < least) return;
             const int part = kSub - 1 - (int)((o - lo) >> shift);  // larger words first
-            atomicAdd((unsigned long long*)&s.sub_mass[part], (unsigned long long)m);
+            atomicAdd((unsigned long long*)&s.sub_mass[part], (unsigned long long)kept(r, o));
             atomicAdd(&s.sub_count[part], 1u);
         });
         __syncthreads();
@@ -399,29 +579,24 @@ __device__ __forceinline__ Place locate(PickLds& s, const SampleArgs& a, const f
         hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
         __syncthreads();
     }
-    if (tid == 0) s.fill = 0;
-    __syncthreads();
-    each<kThr>(x, 0, a.n, tid, [&](float v, int i) {
-        if (bin_of(w, v) != bin) return;
-        const uint64_t o = word_of(key_of(v), (uint32_t)i);
-        if (o < lo || o > hi || weight(w, v) < least) return;
-        const uint32_t at = atomicAdd(&s.fill, 1u);
-        if (at < kList) s.list[at] = o;
-    });
-    __syncthreads();
-    const int c = (int)min(s.fill, (uint32_t)kList);
-    order_list(s, tid, c, w);
-    __syncthreads();
-    for (int i = tid; i < c; i += kThr) {
-        const uint64_t before = by_count ? count0 + i : mass0 + (i ? s.cum[i - 1] : 0);
-        const uint64_t with = by_count ? count0 + i + 1 : mass0 + s.cum[i];
-        if (before < goal && with >= goal) s.found = i;
-    }
-    __syncthreads();
-    const int at = min(s.found, c - 1);
+    const int c = gather(s, r, tid, bin, bin, lo, hi);
+    const int at = list_at(s, tid, c, mass0, count0, by_count, goal);
     const Place p = {s.list[at], mass0 + s.cum[at]};
     __syncthreads();
     return p;
+}
+
+// top-p's running weight
+__device__ __forceinline__ uint64_t goal_of(double p, uint64_t W)
+{
+    return min(max((uint64_t)__builtin_ceil(__dmul_rn(p, (double)W)), (uint64_t)1), W);
+}
+
+// the draw's
+__device__ __forceinline__ uint64_t draw_of(float u, uint64_t W)
+{
+    const double r = __dmul_rn(u > 0.0f ? (double)u : 0.0, (double)W);
+    return (r < (double)W ? min((uint64_t)r, W - 1) : W - 1) + 1;
 }
 
 }  // namespace
@@ -433,7 +608,6 @@ __global__ __launch_bounds__(kThr) void k_sample_pick(SampleArgs a)
     const int row = blockIdx.x, tid = threadIdx.x;
     const RowFilters f = filters_at(a, row);
     const uint64_t best = row_best<kThr / 64>(a, row, tid, s.best);
-    __syncthreads();
     const uint32_t top = (uint32_t)(best >> 32);
     if (top <= kMinusInf || !(f.t > 0.0f)) {
         if (tid == 0) {
@@ -442,39 +616,65 @@ __global__ __launch_bounds__(kThr) void k_sample_pick(SampleArgs a)
         }
         return;
     }
-    const Weigh w = weigh_at(top, f.t);
-    const float* x = a.logits + (int64_t)row * a.ld;
-    uint64_t m0 = 0;
-    uint32_t c0 = 0;
-    for (int b0 = 0; b0 < kBins; b0 += kThr) {
-        uint64_t m = a.mass[(int64_t)row * kBins + b0 + tid];
-        uint32_t c = a.count[(int64_t)row * kBins + b0 + tid];
-        scan_pairs(s, tid, m, c);
-        s.mass[b0 + tid] = m0 + m;
-        s.count[b0 + tid] = c0 + c;
-        __syncthreads();
-        m0 = s.mass[b0 + kThr - 1];
-        c0 = s.count[b0 + kThr - 1];
+    const Row r = {a.logits + (int64_t)row * a.ld, a.n, weigh_at(top, f.t), f.least};
+    for (int b = tid; b < kBins; b += kThr) {
+        s.mass[b] = a.mass[(int64_t)row * kBins + b];
+        s.count[b] = a.count[(int64_t)row * kBins + b];
     }
+    run_bins(s, tid);
+    const uint32_t c0 = s.count[kBins - 1];
+    const uint64_t m0 = s.mass[kBins - 1];
+    const bool by_k = f.k > 0 && (uint32_t)f.k < c0, by_p = f.p < 1.0;
+    const bool few = !weighed(f);
     uint64_t W = m0;  // the weight of what stays
     Place p{};
-    // in turn: where top-k cuts, where top-p cuts, the draw
-    for (int step = 0; step < 3; ++step) {
-        if (step == 0 && !(f.k > 0 && (uint32_t)f.k < c0)) continue;
-        if (step == 1 && !(f.p < 1.0)) continue;
-        uint64_t goal = (uint64_t)f.k;
-        if (step == 1) goal = min(max((uint64_t)__builtin_ceil(__dmul_rn(f.p, (double)W)), (uint64_t)1), W);
-        if (step == 2) {
-            const double r = __dmul_rn(f.u > 0.0f ? (double)f.u : 0.0, (double)W);
-            goal = (r < (double)W ? min((uint64_t)r, W - 1) : W - 1) + 1;
+    int last = kBins;  // the bin that the first filter cuts in
+    if (by_k) last = bin_at(s, tid, true, (uint64_t)f.k);
+    else if (few) last = kBins - 1;
+    else if (by_p) last = bin_at(s, tid, false, goal_of(f.p, W));
+    if (last < kBins && s.count[last] <= kList) {
+        // the tokens up to there in one list: every place is in it
+        const int c = gather(s, r, tid, 0, last, 0, ~(uint64_t)0);
+        if (by_k || few) W = s.cum[by_k ? min(f.k, c) - 1 : c - 1];
+        if (by_p) W = s.cum[list_at(s, tid, c, 0, 0, false, goal_of(f.p, W))];
+        const int at = list_at(s, tid, c, 0, 0, false, draw_of(f.u, W));
+        p = {s.list[at], s.cum[at]};
+    } else {
+        if (few) {
+            // few are asked for, but the bin that top-k cuts in is full of tokens: its weights after all
+            __syncthreads();
+            for (int b = tid; b < kBins; b += kThr) s.mass[b] = 0;
+            __syncthreads();
+            each_in(r, tid, 0, kBins - 1, [&](float v, int) {
+                const uint64_t m = weight(r.w, v);
+                if (m >= r.least) atomicAdd((unsigned long long*)&s.mass[(int)place_of(r.w, v)], (unsigned long long)m);
+            });
+            __syncthreads();
+            for (int b = tid; b < kBins; b += kThr) s.count[b] = a.count[(int64_t)row * kBins + b];
+            run_bins(s, tid);
+            W = s.mass[kBins - 1];
         }
-        p = locate(s, a, x, w, f.least, tid, step == 0, goal);
-        if (step < 2) W = p.upto;
+        // in turn: where top-k cuts, where top-p cuts, the draw
+        for (int step = 0; step < 3; ++step) {
+            if ((step == 0 && !by_k) || (step == 1 && !by_p)) continue;
+            const uint64_t goal = step == 0 ? (uint64_t)f.k : (step == 1 ? goal_of(f.p, W) : draw_of(f.u, W));
+            p = locate(s, r, tid, step == 0, goal);
+            if (step < 2) W = p.upto;
+        }
     }
     if (tid == 0) {
         a.ids[row] = (int32_t)~(uint32_t)p.word;
-        if (a.probs) a.probs[row] = (float)__ddiv_rn((double)weight(w, value_of((uint32_t)(p.word >> 32))), (double)W);
+        if (a.probs) a.probs[row] = (float)__ddiv_rn((double)kept(r, p.word), (double)W);
     }
+}
+
+// logits of one workgroup of the first two launches: some 512 workgroups, so that few
+// rows spread over the chip and many rows add few histograms together
+int sample_slice(int64_t rows, int64_t n)
+{
+    int slice = 2048;
+    while (slice < 32768 && rows * n > (int64_t)512 * slice) slice *= 2;
+    return slice;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st)

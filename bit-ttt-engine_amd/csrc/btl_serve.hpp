@@ -77,8 +77,8 @@ struct PagedAttn {
 hipError_t launch_paged_attention(const PagedAttn& a, hipStream_t st);
 
 // sampling
-constexpr int kSampleBins = 2048;
-constexpr int kSampleSlice = 4096;  // logits of one workgroup of the first two launches
+constexpr int kSampleBins = 1024;
+int sample_slice(int64_t rows, int64_t n);  // logits of one workgroup of the first two launches
 struct SampleArgs {
     const float* logits;
     int64_t ld;
@@ -92,7 +92,7 @@ struct SampleArgs {
     uint64_t* best;   // [rows][slices] largest (key, index) word of a slice
     uint64_t* mass;   // [rows][kSampleBins]
     uint32_t* count;  // [rows][kSampleBins]
-    int rows, n, slices;
+    int rows, n, slice, slices;
 };
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
 

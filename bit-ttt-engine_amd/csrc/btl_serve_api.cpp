@@ -109,7 +109,8 @@ struct SampleWs {
 };
 SampleWs sample_ws(int64_t rows, int64_t n)
 {
-    const size_t slices = (size_t)((n + btl::kSampleSlice - 1) / btl::kSampleSlice);
+    // of the smallest slice: a workspace for some rows serves fewer
+    const size_t slices = (size_t)((n + 2047) / 2048);
     SampleWs w;
     w.mass = up256((size_t)rows * slices * 8);
     w.count = w.mass + up256((size_t)rows * btl::kSampleBins * 8);
@@ -256,7 +257,8 @@ int btl_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, const f
     a.count = (uint32_t*)((uint8_t*)p + w.count);
     a.rows = (int)rows;
     a.n = (int)n;
-    a.slices = (int)((n + btl::kSampleSlice - 1) / btl::kSampleSlice);
+    a.slice = btl::sample_slice(rows, n);
+    a.slices = (int)((n + a.slice - 1) / a.slice);
     const hipError_t e = btl::launch_sample(a, (hipStream_t)stream);
     return e == hipSuccess ? BTL_OK : hip_error(e, "sampling kernel launch");
 }
