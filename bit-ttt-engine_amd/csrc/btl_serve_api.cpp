@@ -134,9 +134,8 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
     if ((rc = check_pointers(cache, batch, &a.c))) return rc;
     if (!q || !k || !v || !q_out || (rope_len && (!rope_cos || !rope_sin))) return fail_msg(BTL_ERR_LAYOUT, "null pointer");
     const size_t size = dtype == BTL_F32 ? 4 : 2;
-    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & (size - 1))
-        return fail_msg(BTL_ERR_LAYOUT, "q, k, v and q_out must be aligned to their elements");
-    if (!aligned4(rope_cos) || !aligned4(rope_sin)) return fail_msg(BTL_ERR_LAYOUT, "rope tables must be 4-byte aligned");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(rope_cos) || !aligned16(rope_sin))
+        return fail_msg(BTL_ERR_LAYOUT, "q, k, v, q_out and the rope tables must be 16-byte aligned");
     const size_t qn = (size_t)a.c.rows * n_heads * a.c.hd * size, kn = (size_t)a.c.rows * a.c.nkv * a.c.hd * size;
     if ((q_out != q && overlap(q_out, qn, q, qn)) || overlap(q_out, qn, k, kn) || overlap(q_out, qn, v, kn))
         return fail_msg(BTL_ERR_LAYOUT, "q_out must be q itself or not overlap q, k and v");
@@ -164,8 +163,7 @@ int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, 
     if (a.c.rows == 0 || a.c.n_seqs == 0 || (!k_out && !v_out)) return BTL_OK;
     if ((rc = check_pointers(cache, batch, &a.c))) return rc;
     const size_t size = dtype == BTL_F32 ? 4 : 2, n = (size_t)a.c.rows * a.c.nkv * a.c.hd * size;
-    if (((uintptr_t)k_out | (uintptr_t)v_out) & (size - 1))
-        return fail_msg(BTL_ERR_LAYOUT, "k_out and v_out must be aligned to their elements");
+    if (!aligned16(k_out) || !aligned16(v_out)) return fail_msg(BTL_ERR_LAYOUT, "k_out and v_out must be 16-byte aligned");
     if (overlap(k_out, n, v_out, n)) return fail_msg(BTL_ERR_LAYOUT, "k_out and v_out overlap");
     int dev;
     if ((rc = btl::host::device(&dev))) return rc;

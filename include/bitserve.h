@@ -89,7 +89,8 @@ typedef struct btl_paged_batch {
  * widened exactly, computed in f32, q_out rounded to nearest even; k is quantised
  * from its f32 rotation).  rope_cos / rope_sin: device [rope_len, head_dim / 2]
  * (btl_rope_table); a row at a position >= rope_len is not stored and its q_out
- * is NaN.  q, k, v and q_out share no memory but q_out == q.
+ * is NaN.  Every array is 16-byte aligned; q, k, v and q_out share no memory but
+ * q_out == q.
  */
 int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t n_heads,
                           const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const float* rope_cos,
@@ -98,7 +99,8 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
 /*
  * The cache read back: for every row, its position's key and value (code - 128) *
  * scale into k_out and v_out [rows, n_kv * head_dim] of dtype (either may be
- * NULL).  Whole contexts are rows at pos = 0.  Keys are as stored, rotated.
+ * NULL), 16-byte aligned.  Whole contexts are rows at pos = 0.  Keys are as stored,
+ * rotated.
  */
 int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, void* k_out, void* v_out, int dtype,
                    void* stream);
