@@ -22,7 +22,18 @@ from ._lib import (
     BTL_ERR_ARG, BTL_ERR_DEVICE, BTL_ERR_DTYPE, BTL_ERR_LAYOUT, BTL_ERR_SHAPE, BitLinearError, BtlKvPaged, BtlPagedBatch,
     check, lib,
 )
-from .layer import _dtype_code, _on_gpu, _stream
+from .layer import _DT, _dtype_code, _on_gpu
+
+# A decoded token's calls take microseconds on the GPU: the checks around them look at
+# what is right first and only then for what is wrong.
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(device):
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _on_its_device(f):
@@ -31,7 +42,7 @@ def _on_its_device(f):
     @functools.wraps(f)
     def call(x, *args, **kw):
         dev = x.device
-        if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        if dev.type == "cuda" and dev.index != _current_device():
             with torch.cuda.device(dev):
                 return f(x, *args, **kw)
         return f(x, *args, **kw)
@@ -41,6 +52,9 @@ def _on_its_device(f):
 
 def _tensor(t, what, dtype, shape, device):
     """A contiguous tensor on `device` of this dtype and shape (None in the shape: any)."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous() \
+            and t.device == device:
+        return t
     if not torch.is_tensor(t):
         raise BitLinearError(BTL_ERR_ARG, "%s must be a tensor" % what)
     _on_gpu(t, what)
@@ -59,7 +73,8 @@ class Scratch:
     def __init__(self, nbytes, device):
         self.nbytes = int(nbytes)
         self.buf = torch.empty(max(self.nbytes, 256), dtype=torch.uint8, device=device)
-        self._args = ctypes.c_void_p(self.buf.data_ptr()), self.nbytes
+        self.device = self.buf.device
+        self._args = self.buf.data_ptr(), self.nbytes
 
     def args(self):
         return self._args
@@ -68,8 +83,8 @@ class Scratch:
 def _ws_args(ws, device):
     if ws is None:
         return None, 0
-    if ws.buf.device != device:
-        raise BitLinearError(BTL_ERR_DEVICE, "the workspace is on %s, not on %s" % (ws.buf.device, device))
+    if ws.device != device:
+        raise BitLinearError(BTL_ERR_DEVICE, "the workspace is on %s, not on %s" % (ws.device, device))
     return ws.args()
 
 
@@ -133,19 +148,17 @@ class PagedBatch:
         self._ref = ctypes.byref(self.c)
 
 
-def _together(x, cache, batch):
-    if cache.device != x.device or batch.device != x.device:
-        raise BitLinearError(BTL_ERR_DEVICE, "rows on %s, cache on %s, batch on %s"
-                             % (x.device, cache.device, batch.device))
-
-
 def _heads(q, cache, batch):
-    _on_gpu(q, "q")
-    if q.dim() != 2 or q.shape[0] != batch.rows or q.shape[1] % cache.head_dim:
+    """q's dtype code, heads and device."""
+    if not q.is_cuda or not q.is_contiguous():
+        _on_gpu(q, "q")
+    shape, device, dt = q.shape, q.device, _DT.get(q.dtype)
+    if len(shape) != 2 or shape[0] != batch.rows or shape[1] % cache.head_dim:
         raise BitLinearError(BTL_ERR_SHAPE, "q must be [%d, n_heads * %d], got %s"
-                             % (batch.rows, cache.head_dim, list(q.shape)))
-    _together(q, cache, batch)
-    return _dtype_code(q, "q"), q.shape[1] // cache.head_dim
+                             % (batch.rows, cache.head_dim, list(shape)))
+    if cache.device != device or batch.device != device:
+        raise BitLinearError(BTL_ERR_DEVICE, "q on %s, cache on %s, batch on %s" % (device, cache.device, batch.device))
+    return _dtype_code(q, "q") if dt is None else dt, shape[1] // cache.head_dim, device
 
 
 @_on_its_device
@@ -153,19 +166,20 @@ def paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, q_out=None):
     """btl_paged_rope_append: RoPE of the rows q [rows, n_heads * head_dim] and k [rows,
     n_kv * head_dim], k and v quantised into the cache.  Returns the rotated q (q_out,
     which may be q).  rope_cos, rope_sin: float32 [positions, head_dim / 2]."""
-    dt, nh = _heads(q, cache, batch)
+    dt, nh, dev = _heads(q, cache, batch)
     kv = (batch.rows, cache.n_kv_heads * cache.head_dim)
-    _tensor(k, "k", q.dtype, kv, q.device)
-    _tensor(v, "v", q.dtype, kv, q.device)
-    _tensor(rope_cos, "rope_cos", torch.float32, (None, cache.head_dim // 2), q.device)
-    _tensor(rope_sin, "rope_sin", torch.float32, tuple(rope_cos.shape), q.device)
+    _tensor(k, "k", q.dtype, kv, dev)
+    _tensor(v, "v", q.dtype, kv, dev)
+    length = rope_cos.shape[0] if rope_cos.dim() == 2 else -1
+    _tensor(rope_cos, "rope_cos", torch.float32, (length, cache.head_dim // 2), dev)
+    _tensor(rope_sin, "rope_sin", torch.float32, (length, cache.head_dim // 2), dev)
     if q_out is None:
         q_out = torch.empty_like(q)
     else:
-        _tensor(q_out, "q_out", q.dtype, tuple(q.shape), q.device)
+        _tensor(q_out, "q_out", q.dtype, q.shape, dev)
     check(lib.btl_paged_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, nh, cache._ref, batch._ref,
-                                    rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], q_out.data_ptr(),
-                                    _stream(q.device)))
+                                    rope_cos.data_ptr(), rope_sin.data_ptr(), length, q_out.data_ptr(),
+                                    _stream(dev)))
     return q_out
 
 
@@ -174,17 +188,17 @@ def paged_read(cache, batch, dtype=torch.float32, k_out=None, v_out=None):
     """btl_paged_read: the rows' keys and values out of the cache, each [rows, n_kv *
     head_dim] of `dtype` (or of k_out's and v_out's).  Whole contexts are a batch at
     pos = 0 with as many rows as tokens."""
-    shape = (batch.rows, cache.n_kv_heads * cache.head_dim)
-    if cache.device != batch.device:
-        raise BitLinearError(BTL_ERR_DEVICE, "cache on %s, batch on %s" % (cache.device, batch.device))
+    shape, dev = (batch.rows, cache.n_kv_heads * cache.head_dim), cache.device
+    if dev != batch.device:
+        raise BitLinearError(BTL_ERR_DEVICE, "cache on %s, batch on %s" % (dev, batch.device))
     first = k_out if k_out is not None else v_out
     dtype = dtype if first is None else first.dtype
     k_out = torch.empty(shape, dtype=dtype, device=cache.device) if k_out is None else k_out
     v_out = torch.empty(shape, dtype=dtype, device=cache.device) if v_out is None else v_out
-    _tensor(k_out, "k_out", dtype, shape, cache.device)
-    _tensor(v_out, "v_out", dtype, shape, cache.device)
+    _tensor(k_out, "k_out", dtype, shape, dev)
+    _tensor(v_out, "v_out", dtype, shape, dev)
     check(lib.btl_paged_read(cache._ref, batch._ref, k_out.data_ptr(), v_out.data_ptr(), _dtype_code(k_out, "output"),
-                             _stream(cache.device)))
+                             _stream(dev)))
     return k_out, v_out
 
 
@@ -192,14 +206,14 @@ def paged_read(cache, batch, dtype=torch.float32, k_out=None, v_out=None):
 def paged_attention(q, cache, batch, out=None, workspace=None):
     """btl_paged_attention: causal attention of the rotated rows q [rows, n_heads *
     head_dim] over their sequences' pages.  Returns out, of q's dtype."""
-    dt, nh = _heads(q, cache, batch)
+    dt, nh, dev = _heads(q, cache, batch)
     if out is None:
         out = torch.empty_like(q)
     else:
-        _tensor(out, "out", q.dtype, tuple(q.shape), q.device)
-    wsp, wsn = _ws_args(workspace, q.device)
+        _tensor(out, "out", q.dtype, q.shape, dev)
+    wsp, wsn = _ws_args(workspace, dev)
     check(lib.btl_paged_attention(q.data_ptr(), dt, nh, cache._ref, batch._ref, out.data_ptr(), wsp, wsn,
-                                  _stream(q.device)))
+                                  _stream(dev)))
     return out
 
 
@@ -223,9 +237,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=
     given random numbers u [rows] in [0, 1).  temperature, top_p, min_p (float32) and
     top_k (int32): tensors [rows], numbers, or None.  Returns (ids int32 [rows], probs
     float32 [rows]: each token's probability among those the filters left)."""
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         _on_gpu(logits, "logits")
-    if logits.dtype != torch.float32:
+    if logits.dtype is not torch.float32:
         raise BitLinearError(BTL_ERR_DTYPE, "logits must be float32, got %s" % logits.dtype)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise BitLinearError(BTL_ERR_LAYOUT, "logits must be [rows, n], each row contiguous")
@@ -233,7 +247,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=
     dev = logits.device
     f = torch.float32
     ld = logits.stride(0) if rows > 1 else n
-    u = _tensor(u, "u", f, (rows,), dev)
+    _tensor(u, "u", f, (rows,), dev)
     row = [_per_row(temperature, "temperature", f, rows, dev), _per_row(top_k, "top_k", torch.int32, rows, dev),
            _per_row(top_p, "top_p", f, rows, dev), _per_row(min_p, "min_p", f, rows, dev)]
     ids = torch.empty((rows,), dtype=torch.int32, device=dev) if ids is None \

@@ -815,9 +815,9 @@ __device__ __forceinline__ Place place_of(const Paged& c, int chunks)
 
 // The rows of a refused sequence.
 template <bool BF>
-__device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h, int wave, int lane)
+__device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h, int wave, int waves, int lane)
 {
-    for (int i = wave; i < q.n; i += 4)
+    for (int i = wave; i < q.n; i += waves)
         for (int x = lane; x < a.group * a.c.hd; x += 64)
             store1<BF>(a.out, ((int64_t)(q.a + i) * a.nh + h * a.group) * a.c.hd + x, __builtin_nanf(""));
 }
@@ -825,42 +825,46 @@ __device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h
 }  // namespace
 
 // The token form: at most 16 query rows of a sequence.  grid nkv * chunks * n_seqs,
-// block 256: the four waves take the chunk's keys in turn, 64 at a time, straight
-// from memory into the operands' registers, and are merged in LDS.  DT: 16-value
+// block 64 NW: the waves take the chunk's keys in turn, 64 at a time, straight from
+// memory into the operands' registers, and are merged in LDS.  NW is 4; 8 where the
+// sequences are short enough to be one chunk each, which saves the merge's launch.  DT: 16-value
 // tiles of a head, hd / 16 or one more.
-template <int DT, bool BF>
-__global__ __launch_bounds__(256, 2) void k_paged_tok(PagedAttn a)
+template <int DT, int NW, bool BF>
+__global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedAttn a)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;
-    __shared__ float s_o[4][16][16 * DT + 4];
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ __align__(16) float s_o[NW][16][16 * DT + 4];
+    __shared__ float s_m[NW][16], s_l[NW][16];
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
     const int hd = c.hd, ndt = hd >> 4, C = a.p.tok_c;
     const Place at = place_of(c, a.p.tok_n);
+    const int key0 = at.chunk * C;
+    const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
+    // the pages are looked up beside the sequence's size, not after it: what the table holds
+    // behind its last page is checked like any id, and its keys are masked
+    const int last_grp = (c.cap - 1) >> 4;
+    Slots slots{};
+    if (c.cap > 0) slots.find(c, table, (key0 + 64 * wave) >> 4, last_grp, at.h, lane);
     const Seq q = seq_at(c, at.s);
     const int64_t M = (int64_t)q.n * a.group;
     if (M == 0 || M > a.p.lo) return;
     const int64_t row0 = (int64_t)q.a * a.nh + at.h * a.group;  // output row of m: row0 + (m / group) * nh + m % group
     if (!q.ok) {
-        if (at.chunk == 0) fill_nan<BF>(a, q, at.h, wave, lane);
+        if (at.chunk == 0) fill_nan<BF>(a, q, at.h, wave, NW, lane);
         return;
     }
     const int seen = q.p0 + q.n;  // keys that the last row sees
-    const int key0 = at.chunk * C, key1 = min(key0 + C, seen);
+    const int key1 = min(key0 + C, seen);
     if (key0 >= key1) return;
-    const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
-    const int last_grp = (key1 - 1) >> 4;
 
     Queries<NJ, 1, BF> qs;
     qs.load(a, q, row0, 0, (int)M - 1, lane);
-    Slots slots;
-    slots.find(c, table, (key0 + 64 * wave) >> 4, last_grp, at.h, lane);
     Running<DT> r;
     r.clear();
-    for (int kb = key0 + 64 * wave; kb < key1; kb += 256) {
+    for (int kb = key0 + 64 * wave; kb < key1; kb += 64 * NW) {
         // a lane loads a key row of group n / 4, and takes the scales and values of group g
         const int grp = kb >> 4;
         if (grp + 4 > slots.base + 64) slots.find(c, table, grp, last_grp, at.h, lane);
@@ -932,14 +936,16 @@ __global__ __launch_bounds__(256, 2) void k_paged_tok(PagedAttn a)
     for (int d = 0; d < DT; ++d) *(f4*)&s_o[wave][n][16 * d + 4 * g] = r.o[d] * unit;
     __syncthreads();
     const bool whole = seen <= C;  // the sequence is one chunk
-    for (int x = threadIdx.x; x < (int)M * (hd >> 2); x += 256) {
+    for (int x = threadIdx.x; x < (int)M * (hd >> 2); x += 64 * NW) {
         const int m = x / (hd >> 2), d = 4 * (x - m * (hd >> 2));
-        float top = fmaxf(fmaxf(s_m[0][m], s_m[1][m]), fmaxf(s_m[2][m], s_m[3][m]));
+        float top = s_m[0][m];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, s_m[w][m]);
         top = top == -__builtin_inff() ? 0.0f : top;
         float sum = 0.0f;
         f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float b = __builtin_amdgcn_exp2f(__fsub_rn(s_m[w][m], top));
             sum = __fmaf_rn(b, s_l[w][m], sum);
             const f4 ow = *(const f4*)&s_o[w][m][d];
@@ -992,7 +998,7 @@ __global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
     const int64_t M = (int64_t)q.n * a.group;
     const int64_t row0 = (int64_t)q.a * a.nh + at.h * a.group;
     if (!q.ok) {
-        if (at.chunk == 0 && at.tile == 0) fill_nan<BF>(a, q, at.h, wave, lane);
+        if (at.chunk == 0 && at.tile == 0) fill_nan<BF>(a, q, at.h, wave, 4, lane);
         return;
     }
     const int m_tile = at.tile * MT;
@@ -1245,9 +1251,16 @@ AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c)
     AttnPlan p{};
     // one kind of launch where the bounds leave one kind of sequence
     p.lo = c.max_rows * group <= kTokRows ? INT_MAX : (c.n_seqs == 1 ? 0 : kTokRows);
-    const int64_t want = 2048;
-    const int64_t all = up(longest, 256);
-    p.tok_c = (int)std::min(all, up(longest * c.n_seqs * c.nkv / want + 1, 256));
+    const int64_t all = up(longest, 256), heads = (int64_t)c.n_seqs * c.nkv;
+    // Workgroups aimed at: two a CU where the sequences are few (one token over 100001
+    // positions: 35.8 us and 5.0 for the merge with 512, 43 + 9.3 with 2048), more
+    // where they are many and, as a batch's are, of different lengths (32 of up to
+    // 8192: 70.1 us with 4096, 73.2 with 512).
+    const int64_t want = heads <= 64 ? 512 : 4096;
+    // 512 positions are one step of eight waves: 7.4 us, and 7.2 + 3.2 in chunks; 777 are
+    // two steps: 11, and 7.2 + 3.2
+    p.tok_w = longest <= 512 ? 8 : 4;
+    p.tok_c = (int)(p.tok_w == 8 ? all : std::min(all, up(longest * heads / want + 1, 256)));
     p.tok_n = (int)((longest + p.tok_c - 1) / p.tok_c);
     const int64_t per = ((int64_t)c.max_rows * group + kTileRows - 1) / kTileRows;
     p.tiles = (int)std::min<int64_t>((int64_t)c.n_seqs * per, (int64_t)c.rows * group / kTileRows + c.n_seqs);
@@ -1267,8 +1280,11 @@ bool paged_attention_fits(const Paged& c, const AttnPlan& p)
 template <int DT, bool BF>
 static hipError_t launch_attn(const PagedAttn& a, hipStream_t st)
 {
-    if (a.p.tok_n)
-        hipLaunchKernelGGL((k_paged_tok<DT, BF>), dim3((unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs)), dim3(256), 0, st, a);
+    if (a.p.tok_n) {
+        const dim3 grid((unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs));
+        if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((k_paged_tok<DT, 4, BF>), grid, dim3(256), 0, st, a);
+    }
     if (a.p.tile_n)
         hipLaunchKernelGGL((k_paged_tile<DT, kTileRows / 64, BF>), dim3((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles)),
                            dim3(256), 0, st, a);
