@@ -36,7 +36,9 @@ Deliberate differences from the reference, all on the host side:
     (a GPU test checks this);
   * the first decode step feeds the token chosen from the prompt's last logits
     (the reference feeds the last prompt token a second time, llama.rs:496-499);
-  * the TTT layer variant and sampling with temperature are not built.
+  * a pick at a temperature (llama.rs:516-530) takes its random numbers from the
+    caller and may be filtered (btl_sample);
+  * the TTT layer variant is not built.
 """
 import ctypes
 
@@ -45,6 +47,7 @@ import torch
 
 from ._lib import BTL_ACT_F32_REF, BTL_F32, BTL_BF16, BtlKvQ8, BtlPacked, check, lib
 from .packed import PackedTensor
+from .serve import sample, sample_workspace
 
 RMS_NORM_EPS = 1e-5  # block.rs:10
 
@@ -202,6 +205,7 @@ class BitLlamaHip:
         self.pos = 0
         self.graph = None
         self._expect = 0  # where a captured step will mostly run, if past self.pos
+        self._draw = None  # what the device loop's picks go by; None: greedy
 
     # ------------------------------------------------------------------ steps
     def _stream(self):
@@ -349,6 +353,7 @@ class BitLlamaHip:
         self.pos = 0
         self.graph = None
         self._expect = 0
+        self._draw = None
 
     def forward_one(self, token):
         """BitLlama::forward_one (llama.rs:201-271): one token at the current position;
@@ -381,12 +386,40 @@ class BitLlamaHip:
                                   self._stream()))
         return int(self.next_id.item())
 
+    def sample(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """The pick of the current logits at a temperature (llama.rs:516-530) with the
+        random number u in [0, 1) and the filters of btl_sample, on the device, into
+        self.next_id; returns it as an int (synchronises)."""
+        self._set_draw(temperature, top_k, top_p, min_p)
+        d, self._draw = self._draw, None
+        d["u1"].fill_(float(u))
+        sample(self.logits, d["u1"], d["temperature"], d["top_k"], d["top_p"], d["min_p"], ids=self.next_id,
+               probs=d["probs"], workspace=d["space"])
+        return int(self.next_id.item())
+
+    def _set_draw(self, temperature, top_k, top_p, min_p):
+        one = lambda v, t: torch.full((1,), v, dtype=t, device=self.dev)  # noqa: E731
+        f = torch.float32
+        self._draw = dict(temperature=one(float(temperature), f), top_k=one(int(top_k), torch.int32),
+                          top_p=one(float(top_p), f), min_p=one(float(min_p), f), u1=one(0.0, f), probs=one(0.0, f),
+                          u=torch.zeros((self.cfg.max_seq,), dtype=f, device=self.dev),
+                          space=sample_workspace(1, self.cfg.vocab, self.dev))
+
     # ------------------------------------------------------- device decode loop
     def _step_device(self):
         """One decode step with the position on the device: the token in next_id at
-        position *d_pos through the blocks and the head, then the greedy pick
-        (next_id, log[*d_pos + 1], ++*d_pos)."""
+        position *d_pos through the blocks and the head, then the greedy pick, or the
+        sampled one with the position's random number (next_id, log[*d_pos + 1],
+        ++*d_pos)."""
         self._run(1, max(self.pos, self._expect), self.d_pos, self.next_id)
+        if self._draw is not None:
+            d = self._draw
+            torch.index_select(d["u"], 0, self.d_pos, out=d["u1"])
+            sample(self.logits, d["u1"], d["temperature"], d["top_k"], d["top_p"], d["min_p"], ids=self.next_id,
+                   probs=d["probs"], workspace=d["space"])
+            self.d_pos.add_(1)
+            self.log.index_copy_(0, self.d_pos.long(), self.next_id)
+            return
         check(lib.btl_greedy_next(self.logits.data_ptr(), self.cfg.vocab, self.next_id.data_ptr(),
                                   self.d_pos.data_ptr(), self.log.data_ptr(), self.log.numel(), self._stream()))
 
@@ -423,13 +456,26 @@ class BitLlamaHip:
                 self._step_device()
             self.pos += 1
 
-    def generate(self, prompt_ids, max_tokens, use_graph=True):
-        """Llama::stream_completion at temperature 0 (llama.rs:471-530): prefill, then
-        greedy decode.  Returns the max_tokens generated ids."""
+    def generate(self, prompt_ids, max_tokens, use_graph=True, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
+        """Llama::stream_completion (llama.rs:471-530): prefill, then decode, greedily at
+        temperature 0, else by btl_sample with the filters and the random numbers u in
+        [0, 1), one a token (None: torch's).  Returns the max_tokens generated ids."""
         self.reset()
         self.prefill(prompt_ids)
-        self.greedy()
         start = self.pos
+        if temperature > 0 and max_tokens > 0:
+            u = torch.rand((max_tokens,)) if u is None else torch.as_tensor(u, dtype=torch.float32)
+            if u.dim() != 1 or u.numel() < max_tokens:
+                raise ValueError("%d tokens need as many random numbers" % max_tokens)
+            if start + max_tokens - 1 > self.cfg.max_seq:
+                raise ValueError("%d tokens from position %d overflow the cache of %d rows"
+                                 % (max_tokens, start, self.cfg.max_seq))
+            self.sample(float(u[0]), temperature, top_k, top_p, min_p)
+            self._set_draw(temperature, top_k, top_p, min_p)
+            # the token of position p + 1 is picked with *d_pos = p
+            self._draw["u"][start:start + max_tokens - 1].copy_(u[1:max_tokens])
+        else:
+            self.greedy()
         self.start_decode()
         if max_tokens > 1:
             if use_graph:

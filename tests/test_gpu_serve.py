@@ -551,3 +551,27 @@ def test_on_another_stream():
             outs.append((bl.paged_attention(q, paged, batch, workspace=ws), ws))
     torch.cuda.synchronize()
     assert all(torch.equal(o, exp) for o, _ in outs)
+
+
+def test_the_decoder_samples():
+    """BitLlamaHip.generate at a temperature: every token is the definition's pick of the logits of
+    the tokens before it, captured or not; temperature 0 stays the greedy pick."""
+    from test_gpu_model import gpu_model
+    from test_model_oracle import TinyCfg, tiny_weights
+    cfg = TinyCfg()
+    model = gpu_model(cfg, tiny_weights(cfg, 3), max_rows=8)
+    prompt, n = [3, 9, 27, 5], 20
+    greedy = model.generate(prompt, n)
+    u = np.random.default_rng(2).random(n).astype(np.float32)
+    f = dict(temperature=0.9, top_k=12, top_p=0.9, min_p=0.01)
+    got = model.generate(prompt, n, u=u, **f)
+    assert np.array_equal(got, model.generate(prompt, n, use_graph=False, u=u, **f))
+    model.reset()
+    logits = host(model.prefill(prompt)).copy()
+    for i in range(n):
+        assert got[i] == ref.sample_one(logits, 0.9, 12, 0.9, 0.01, float(u[i]))[0], i
+        assert model.sample(u[i], **f) == got[i]
+        logits = host(model.forward_one(int(got[i]))).copy()
+    assert not np.array_equal(got, greedy) and np.array_equal(model.generate(prompt, n), greedy)
+    with pytest.raises(ValueError):
+        model.generate(prompt, n, u=u[:-1], **f)
