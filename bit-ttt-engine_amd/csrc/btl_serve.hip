@@ -972,7 +972,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedAttn a)
 // operand fragments (64 lanes x 16 bytes, read and written without conflicts), so a
 // code is widened once a workgroup instead of once a wave.
 template <int DT, int NT, bool BF>
-__global__ __launch_bounds__(256, BF ? 2 : 1) void k_paged_tile(PagedAttn a)
+__global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttn a)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;
@@ -1244,7 +1244,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedAttn a)
     }
 }
 
-AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c)
+AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c, bool bf)
 {
     auto up = [](int64_t v, int64_t m) { return (v + m - 1) / m * m; };
     const int64_t group = n_heads / c.nkv, longest = std::max(c.cap, 1);
@@ -1262,9 +1262,16 @@ AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c)
     p.tok_w = longest <= 512 ? 8 : 4;
     p.tok_c = (int)(p.tok_w == 8 ? all : std::min(all, up(longest * heads / want + 1, 256)));
     p.tok_n = (int)((longest + p.tok_c - 1) / p.tok_c);
-    const int64_t per = ((int64_t)c.max_rows * group + kTileRows - 1) / kTileRows;
-    p.tiles = (int)std::min<int64_t>((int64_t)c.n_seqs * per, (int64_t)c.rows * group / kTileRows + c.n_seqs);
-    p.tile_c = (int)std::min(all, up(longest * p.tiles * c.nkv / 512 + 1, 256));
+    // Query rows of a tile.  64 in f32, whose two parts leave no room for 128 beside a
+    // second wave a SIMD (512 rows over 8192: 194 us and 236); in bf16 128 where there
+    // are many (111 us and 144), 64 where they are few (100 rows over 1500: 20 and 26).
+    auto tiles_of = [&](int64_t mt) {
+        const int64_t per = ((int64_t)c.max_rows * group + mt - 1) / mt;
+        return std::min<int64_t>((int64_t)c.n_seqs * per, (int64_t)c.rows * group / mt + c.n_seqs);
+    };
+    p.tile_rows = bf && (int64_t)c.rows * n_heads >= 96 * 128 ? 128 : 64;
+    p.tiles = (int)tiles_of(p.tile_rows);
+    p.tile_c = (int)std::min(all, up(longest * p.tiles * c.nkv / (p.tile_rows == 128 ? 512 : 1024) + 1, 256));
     p.tile_n = (int)((longest + p.tile_c - 1) / p.tile_c);
     if (p.lo == 0) p.tok_n = 0;
     if (p.lo == INT_MAX) p.tile_n = p.tiles = 0;
@@ -1285,9 +1292,13 @@ static hipError_t launch_attn(const PagedAttn& a, hipStream_t st)
         if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF>), grid, dim3(512), 0, st, a);
         else hipLaunchKernelGGL((k_paged_tok<DT, 4, BF>), grid, dim3(256), 0, st, a);
     }
-    if (a.p.tile_n)
-        hipLaunchKernelGGL((k_paged_tile<DT, kTileRows / 64, BF>), dim3((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles)),
-                           dim3(256), 0, st, a);
+    if (a.p.tile_n) {
+        const dim3 grid((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles));
+        if constexpr (BF) {
+            if (a.p.tile_rows == 128) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF>), grid, dim3(256), 0, st, a);
+        }
+        if (a.p.tile_rows == 64) hipLaunchKernelGGL((k_paged_tile<DT, 1, BF>), grid, dim3(256), 0, st, a);
+    }
     if (a.parts > 8)
         hipLaunchKernelGGL((k_paged_merge<4, BF>), dim3((unsigned)a.c.rows, (unsigned)a.nh), dim3(256), 0, st, a);
     else if (a.parts > 1)

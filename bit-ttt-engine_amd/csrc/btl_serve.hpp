@@ -49,16 +49,16 @@ hipError_t launch_paged_read(const PagedRead& a, hipStream_t st);
 // query heads of a group go to the token form, the others to the tile form;
 // each takes its keys in chunks (multiples of 256).
 constexpr int kTokRows = 16;    // rows times heads of one workgroup of the token form, at most
-constexpr int kTileRows = 128;  // of the tile form
 struct AttnPlan {
     int lo;               // 0: no token form, INT_MAX: no tile form
     int tok_w;            // waves of a workgroup of the token form
     int tok_c, tile_c;    // keys a chunk
     int tok_n, tile_n;    // chunks of max_len keys
+    int tile_rows;        // rows times heads of one workgroup of the tile form: 64 or 128
     int tiles;            // workgroups along the rows of the tile form, at most
     int parts() const { return tok_n > tile_n ? tok_n : tile_n; }
 };
-AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c);
+AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c, bool bf);
 // its launches stay within a grid's size
 bool paged_attention_fits(const Paged& c, const AttnPlan& p);
 

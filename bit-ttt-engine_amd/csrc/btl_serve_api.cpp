@@ -179,7 +179,8 @@ size_t btl_paged_attention_workspace_bytes(int64_t n_heads, const btl_kv_paged_t
 {
     btl::Paged c{};
     if (check_sizes(cache, batch, &c) || check_heads(n_heads, c) || c.rows == 0 || c.n_seqs == 0) return 0;
-    return attention_bytes(c, n_heads, btl::plan_paged_attention(n_heads, c));
+    return std::max(attention_bytes(c, n_heads, btl::plan_paged_attention(n_heads, c, false)),
+                    attention_bytes(c, n_heads, btl::plan_paged_attention(n_heads, c, true)));
 }
 
 int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
@@ -189,7 +190,7 @@ int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_
     int rc;
     if ((rc = check_dtype(dtype)) || (rc = check_sizes(cache, batch, &a.c)) || (rc = check_heads(n_heads, a.c))) return rc;
     if (a.c.rows == 0 || a.c.n_seqs == 0) return BTL_OK;
-    a.p = btl::plan_paged_attention(n_heads, a.c);
+    a.p = btl::plan_paged_attention(n_heads, a.c, dtype == BTL_BF16);
     if (!btl::paged_attention_fits(a.c, a.p)) return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
     if ((rc = check_pointers(cache, batch, &a.c))) return rc;
     if (!q || !out) return fail_msg(BTL_ERR_LAYOUT, "null pointer");
