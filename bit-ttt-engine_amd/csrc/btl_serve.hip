@@ -211,6 +211,13 @@ __device__ __forceinline__ float2 load2(const void* p, int64_t i)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
+template <bool BF>
+__device__ __forceinline__ void store2(void* p, int64_t i, float x, float y)
+{
+    if (BF) *(uint32_t*)((uint16_t*)p + i) = (uint32_t)f32_to_bf16(x) | (uint32_t)f32_to_bf16(y) << 16;
+    else *(float2*)((float*)p + i) = make_float2(x, y);
+}
+
 __device__ __forceinline__ float q8_scale(uint32_t amax)
 {
     return __fadd_rn(__fmul_rn(__uint_as_float(amax), (float)(1.0 / 127.0)), 0.0f);
@@ -237,13 +244,18 @@ __global__ __launch_bounds__(256) void k_paged_append_runs(PagedAppend a, int gr
         const unsigned b = blockIdx.x - kvs;
         const int t = b % (unsigned)c.rows, first = N * (4 * (int)(b / (unsigned)c.rows) + wave);
         if (first >= a.nh) return;
-        const bool act = lane < half;
-        float x1[N], x2[N];
+        // two heads at a time, half a wave each, two neighbouring pairs a lane
+        const int m = lane & 31, up = lane >> 5;
+        const bool act = 2 * m < half;
+        float2 x1[N / 2], x2[N / 2];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int64_t row = ((int64_t)t * a.nh + min(first + e, a.nh - 1)) * hd;
-            x1[e] = act ? load1<BF>(a.q, row + lane) : 0.0f;
-            x2[e] = act ? load1<BF>(a.q, row + lane + half) : 0.0f;
+        for (int e = 0; e < N / 2; ++e) {
+            x1[e] = x2[e] = make_float2(0.0f, 0.0f);
+            if (act && first + 2 * e + up < a.nh) {
+                const int64_t row = ((int64_t)t * a.nh + first + 2 * e + up) * hd + 2 * m;
+                x1[e] = load2<BF>(a.q, row);
+                x2[e] = load2<BF>(a.q, row + half);
+            }
         }
         const int s = find_seq(c, t, lane);
         if (s < 0 || s >= c.n_seqs) return;
@@ -251,14 +263,19 @@ __global__ __launch_bounds__(256) void k_paged_append_runs(PagedAppend a, int gr
         const int i = t - q.a;
         if (i < 0 || i >= q.n || !act) return;
         const int pos = q.p0 + i;
-        const bool good = q.ok && pos < a.rope_len;
-        const float co = good ? a.cos_t[(int64_t)pos * half + lane] : nan, si = good ? a.sin_t[(int64_t)pos * half + lane] : nan;
+        float2 co = make_float2(nan, nan), si = co;
+        if (q.ok && pos < a.rope_len) {
+            co = *(const float2*)(a.cos_t + (int64_t)pos * half + 2 * m);
+            si = *(const float2*)(a.sin_t + (int64_t)pos * half + 2 * m);
+        }
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            if (first + e >= a.nh) return;
-            const int64_t row = ((int64_t)t * a.nh + first + e) * hd;
-            store1<BF>(a.q_out, row + lane, __fsub_rn(__fmul_rn(x1[e], co), __fmul_rn(x2[e], si)));
-            store1<BF>(a.q_out, row + lane + half, __fadd_rn(__fmul_rn(x1[e], si), __fmul_rn(x2[e], co)));
+        for (int e = 0; e < N / 2; ++e) {
+            if (first + 2 * e + up >= a.nh) return;
+            const int64_t row = ((int64_t)t * a.nh + first + 2 * e + up) * hd + 2 * m;
+            store2<BF>(a.q_out, row, __fsub_rn(__fmul_rn(x1[e].x, co.x), __fmul_rn(x2[e].x, si.x)),
+                       __fsub_rn(__fmul_rn(x1[e].y, co.y), __fmul_rn(x2[e].y, si.y)));
+            store2<BF>(a.q_out, row + half, __fadd_rn(__fmul_rn(x1[e].x, si.x), __fmul_rn(x2[e].x, co.x)),
+                       __fadd_rn(__fmul_rn(x1[e].y, si.y), __fmul_rn(x2[e].y, co.y)));
         }
         return;
     }
@@ -482,8 +499,7 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedRead a)
             const float f = page < 0 ? nan : ss[b];
             const float v0 = value_at(a0[r4], b, f), v1 = value_at(a1[r4], b, f);
             const int64_t at = out + i * step + 2 * lane;
-            if (BF) *(uint32_t*)((uint16_t*)a.v_out + at) = (uint32_t)f32_to_bf16(v0) | (uint32_t)f32_to_bf16(v1) << 16;
-            else *(float2*)((float*)a.v_out + at) = make_float2(v0, v1);
+            store2<BF>(a.v_out, at, v0, v1);
         }
     }
 }
