@@ -279,14 +279,17 @@ namespace {
 
 constexpr int kThr = 512;
 constexpr int kU = 16;       // loads ahead over a whole row
-constexpr int kList = 2048;  // tokens that are ordered at once
+constexpr int kList = 2048;  // tokens that are brought together at once
+constexpr int kOrdered = 256;  // of them, that are sorted; more are narrowed down first
 constexpr int kSub = kThr;   // parts that a fuller bin is split into
+static_assert(kOrdered <= kThr, "a token a thread");
 
 struct PickLds {
     uint64_t mass[kBins];    // running weight up to and with a bin
     uint32_t count[kBins];   // running count
-    uint64_t list[kList];    // words, ordered
-    uint64_t cum[kList];     // running weights of the list
+    uint64_t list[kList];    // words
+    uint64_t part[64];       // those that a search is down to
+    uint64_t cum[kOrdered];  // running weights of the ordered list
     uint64_t sub_mass[kSub];
     uint32_t sub_count[kSub];
     uint64_t scan[kThr / 64];
@@ -412,8 +415,8 @@ __device__ __forceinline__ void each_in(const Row& r, int tid, int b0, int b1, F
     if (i < r.n && in(r.x[i])) f(r.x[i], i);
 }
 
-// The words of bins b0 .. b1 from lo to hi into the list, in order, with their running
-// weights; returns how many (at most kList of them are there).
+// The words of bins b0 .. b1 from lo to hi into the list, in any order; returns how
+// many (at most kList of them are there).
 __device__ __forceinline__ int gather(PickLds& s, const Row& r, int tid, int b0, int b1, uint64_t lo, uint64_t hi)
 {
     __syncthreads();
@@ -426,7 +429,13 @@ __device__ __forceinline__ int gather(PickLds& s, const Row& r, int tid, int b0,
         if (at < kList) s.list[at] = o;
     });
     __syncthreads();
-    const int c = (int)min(s.fill, (uint32_t)kList);
+    return (int)min(s.fill, (uint32_t)kList);
+}
+
+// The list's c <= kOrdered words in order, with their running weights.
+__device__ __forceinline__ void order_list(PickLds& s, const Row& r, int tid, int c)
+{
+    __syncthreads();
     if (c <= 64) {
         // one wave, in registers
         if (tid < 64) {
@@ -459,17 +468,11 @@ __device__ __forceinline__ int gather(PickLds& s, const Row& r, int tid, int b0,
                 __syncthreads();
             }
     }
-    uint64_t carry = 0;
-    for (int i0 = 0; i0 < c; i0 += kThr) {
-        const int i = i0 + tid;
-        uint64_t m = i < c ? kept(r, s.list[i]) : 0;
-        uint32_t one = 0;
-        scan_pairs(s, tid, m, one);
-        if (i < c) s.cum[i] = carry + m;
-        __syncthreads();
-        carry = s.cum[min(i0 + kThr, c) - 1];
-    }
-    return c;
+    uint64_t m = tid < c ? kept(r, s.list[tid]) : 0;
+    uint32_t one = 0;
+    scan_pairs(s, tid, m, one);
+    if (tid < c) s.cum[tid] = m;
+    __syncthreads();
 }
 
 // The bin at which the running count reaches `goal` (by_count) or the running weight does.
@@ -509,6 +512,128 @@ struct Place {
     uint64_t word, upto;
 };
 
+// kSub parts of the words lo .. hi, larger words first: cleared, a word counted and
+// weighed, and on with the part that holds the place.
+__device__ __forceinline__ int clear_parts(PickLds& s, int tid, uint64_t lo, uint64_t hi)
+{
+    int shift = 0;
+    while (((hi - lo) >> shift) >= kSub) ++shift;
+    __syncthreads();
+    s.sub_mass[tid] = 0;
+    s.sub_count[tid] = 0;
+    if (tid == 0) {
+        // no part holds the place: nothing is left to look at, and the search ends
+        s.best[2] = 0;
+        s.found = 0;
+    }
+    __syncthreads();
+    return shift;
+}
+
+__device__ __forceinline__ void to_part(PickLds& s, const Row& r, uint64_t o, uint64_t lo, int shift)
+{
+    const int part = kSub - 1 - (int)((o - lo) >> shift);
+    atomicAdd((unsigned long long*)&s.sub_mass[part], (unsigned long long)kept(r, o));
+    atomicAdd(&s.sub_count[part], 1u);
+}
+
+__device__ __forceinline__ uint32_t take_part(PickLds& s, int tid, bool by_count, uint64_t goal, int shift, uint64_t& lo,
+                                              uint64_t& hi, uint64_t& mass0, uint64_t& count0)
+{
+    __syncthreads();
+    uint64_t m = s.sub_mass[tid];
+    uint32_t c = s.sub_count[tid];
+    const uint64_t m1 = m;
+    const uint32_t c1 = c;
+    scan_pairs(s, tid, m, c);
+    const uint64_t before = by_count ? count0 + c - c1 : mass0 + m - m1, with = by_count ? count0 + c : mass0 + m;
+    if (c1 && before < goal && with >= goal) {
+        s.found = tid;
+        s.best[0] = mass0 + m - m1;
+        s.best[1] = count0 + c - c1;
+        s.best[2] = c1;
+    }
+    __syncthreads();
+    mass0 = s.best[0];
+    count0 = s.best[1];
+    const uint32_t held = (uint32_t)s.best[2];
+    lo += (uint64_t)(kSub - 1 - s.found) << shift;
+    hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+    __syncthreads();
+    return held;
+}
+
+// The place among the list's c words (kept as they are): narrowed down part by part
+// to one wave's.
+__device__ __forceinline__ Place search_list(PickLds& s, const Row& r, int tid, int c, uint64_t mass0, uint64_t count0,
+                                             bool by_count, uint64_t goal)
+{
+    uint64_t wl = ~(uint64_t)0, wh = 0;
+    for (int i = tid; i < c; i += kThr) {
+        wl = min(wl, s.list[i]);
+        wh = max(wh, s.list[i]);
+    }
+    wl = ~wave_max64(~wl);
+    wh = wave_max64(wh);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+        s.best[tid >> 6] = wh;
+        s.scan[tid >> 6] = wl;
+    }
+    __syncthreads();
+    uint64_t lo = s.scan[0], hi = s.best[0];
+    for (int i = 1; i < kThr / 64; ++i) {
+        lo = min(lo, s.scan[i]);
+        hi = max(hi, s.best[i]);
+    }
+    uint32_t held = (uint32_t)c;
+    while (held > 64) {
+        const int shift = clear_parts(s, tid, lo, hi);
+        for (int i = tid; i < c; i += kThr) {
+            const uint64_t o = s.list[i];
+            if (o >= lo && o <= hi) to_part(s, r, o, lo, shift);
+        }
+        held = take_part(s, tid, by_count, goal, shift, lo, hi, mass0, count0);
+    }
+    if (tid == 0) {
+        s.fill = 0;
+        s.best[0] = s.list[0];
+        s.best[1] = mass0;
+    }
+    __syncthreads();
+    for (int i = tid; i < c; i += kThr) {
+        const uint64_t o = s.list[i];
+        if (o >= lo && o <= hi) s.part[atomicAdd(&s.fill, 1u) & 63] = o;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        uint64_t v = (uint32_t)tid < held ? s.part[tid] : 0;
+#pragma unroll
+        for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                const uint64_t o = shfl_xor64(v, j);
+                v = ((tid & k) == 0) == ((tid & j) == 0) ? max(v, o) : min(v, o);
+            }
+        const uint64_t m1 = (uint32_t)tid < held ? kept(r, v) : 0;
+        uint64_t m = m1;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint64_t o = shfl_up64(m, off);
+            m += tid >= off ? o : 0;
+        }
+        const uint64_t before = by_count ? count0 + tid : mass0 + m - m1, with = by_count ? count0 + tid + 1 : mass0 + m;
+        if ((uint32_t)tid < held && before < goal && with >= goal) {
+            s.best[0] = v;
+            s.best[1] = mass0 + m;
+        }
+    }
+    __syncthreads();
+    const Place p = {s.best[0], s.best[1]};
+    __syncthreads();
+    return p;
+}
+
 // The first token at which the running count reaches `goal` (by_count) or the
 // running weight does.  1 <= goal <= the row's.
 __device__ __forceinline__ Place locate(PickLds& s, const Row& r, int tid, bool by_count, uint64_t goal)
@@ -543,43 +668,16 @@ __device__ __forceinline__ Place locate(PickLds& s, const Row& r, int tid, bool 
     }
     while (held > kList) {
         // kSub parts of the range, counted and weighed, and on with the one that holds the place
-        int shift = 0;
-        while (((hi - lo) >> shift) >= kSub) ++shift;
-        for (int i = tid; i < kSub; i += kThr) {
-            s.sub_mass[i] = 0;
-            s.sub_count[i] = 0;
-        }
-        __syncthreads();
+        const int shift = clear_parts(s, tid, lo, hi);
         each_in(r, tid, bin, bin, [&](float v, int i) {
             const uint64_t o = word_of(key_of(v), (uint32_t)i);
-            if (o < lo || o > hi) return;
-            const int part = kSub - 1 - (int)((o - lo) >> shift);  // larger words first
-            atomicAdd((unsigned long long*)&s.sub_mass[part], (unsigned long long)kept(r, o));
-            atomicAdd(&s.sub_count[part], 1u);
+            if (o >= lo && o <= hi) to_part(s, r, o, lo, shift);
         });
-        __syncthreads();
-        uint64_t m = s.sub_mass[tid];
-        uint32_t c = s.sub_count[tid];
-        const uint64_t m1 = m;
-        const uint32_t c1 = c;
-        scan_pairs(s, tid, m, c);
-        const uint64_t before = by_count ? count0 + c - c1 : mass0 + m - m1, with = by_count ? count0 + c : mass0 + m;
-        if (c1 && before < goal && with >= goal) {
-            s.found = tid;
-            s.best[0] = mass0 + m - m1;
-            s.best[1] = count0 + c - c1;
-            s.best[2] = c1;
-        }
-        __syncthreads();
-        const int part = kSub - 1 - s.found;
-        mass0 = s.best[0];
-        count0 = s.best[1];
-        held = (uint32_t)s.best[2];
-        lo += (uint64_t)part << shift;
-        hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
-        __syncthreads();
+        held = take_part(s, tid, by_count, goal, shift, lo, hi, mass0, count0);
     }
     const int c = gather(s, r, tid, bin, bin, lo, hi);
+    if (c > kOrdered) return search_list(s, r, tid, c, mass0, count0, by_count, goal);
+    order_list(s, r, tid, c);
     const int at = list_at(s, tid, c, mass0, count0, by_count, goal);
     const Place p = {s.list[at], mass0 + s.cum[at]};
     __syncthreads();
@@ -635,10 +733,18 @@ __global__ __launch_bounds__(kThr) void k_sample_pick(SampleArgs a)
     if (last < kBins && s.count[last] <= kList) {
         // the tokens up to there in one list: every place is in it
         const int c = gather(s, r, tid, 0, last, 0, ~(uint64_t)0);
-        if (by_k || few) W = s.cum[by_k ? min(f.k, c) - 1 : c - 1];
-        if (by_p) W = s.cum[list_at(s, tid, c, 0, 0, false, goal_of(f.p, W))];
-        const int at = list_at(s, tid, c, 0, 0, false, draw_of(f.u, W));
-        p = {s.list[at], s.cum[at]};
+        const bool ordered = c <= kOrdered;
+        if (ordered) order_list(s, r, tid, c);
+        auto place = [&](bool by_count, uint64_t goal) {
+            if (!ordered) return search_list(s, r, tid, c, 0, 0, by_count, goal);
+            const int at = list_at(s, tid, c, 0, 0, by_count, goal);
+            return Place{s.list[at], s.cum[at]};
+        };
+        for (int step = 0; step < 3; ++step) {  // where top-k cuts (or all of them), where top-p cuts, the draw
+            if ((step == 0 && !by_k && !few) || (step == 1 && !by_p)) continue;
+            p = place(step == 0, step == 0 ? (uint64_t)(by_k ? f.k : c) : (step == 1 ? goal_of(f.p, W) : draw_of(f.u, W)));
+            if (step < 2) W = p.upto;
+        }
     } else {
         if (few) {
             // few are asked for, but the bin that top-k cuts in is full of tokens: its weights after all
