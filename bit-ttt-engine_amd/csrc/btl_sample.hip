@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256) void k_sample_hist(SampleArgs a)
     each<256, 1>(a.logits + (int64_t)row * a.ld, slice * a.slice, min(a.n, (slice + 1) * a.slice), tid,
                  [&](float v, int) {
                      const float p = place_of(w, v);
-                     if (p >= (float)kBins) return;
+                     if (p >= (float)kBins || v != v) return;
                      atomicAdd(&s_count[(int)p], 1u);
                      if (!weigh) return;
                      const uint64_t m = weight(w, v);

@@ -549,7 +549,10 @@ namespace {
 
 constexpr float kAhead = 6.0f;   // a score may pass the reference by this (log2)
 constexpr int kVUp = 8;          // weights times value scales stay below 2^(kAhead + 1 + kVUp) = 2^15
-constexpr int kLeastExp = -100;  // the least exponent of a value scale that weights are scaled by
+// The least exponent of a query row, and of a value scale, that is scaled up in full:
+// a row's products, as far above their scores as its queries are scaled, stay below
+// 2^128 for scores up to 2^16.
+constexpr int kLeastExp = -96;
 
 // four codes -> four f16 (code - 128)
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t* o)
@@ -713,6 +716,14 @@ struct Running {
         ve = e;
     }
 
+    // 16 scores in log2 units, less the reference: two roundings, not a fused one, so that
+    // the largest score's is the reference exactly however large it is.
+    __device__ __forceinline__ static void score(const f4* sc, float cq, float at, float* y)
+    {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) y[x] = __fsub_rn(__fmul_rn(sc[x >> 2][x & 3], cq), at);
+    }
+
     // sc: the products of 16 keys with their scales (-inf: not seen); vs: value
     // scales times 2^(kVUp - ve).  Leaves the weights, in f16 parts.
     template <int PARTS>
@@ -721,22 +732,22 @@ struct Running {
         float y[16];
         float big = -__builtin_inff();
         float at = ref == -__builtin_inff() ? 0.0f : ref;
+        score(sc, cq, at, y);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-            y[x] = __fmaf_rn(sc[x >> 2][x & 3], cq, -at);
-            big = fmaxf(big, y[x]);
-        }
+        for (int x = 0; x < 16; ++x) big = fmaxf(big, y[x]);
         if (__any(big > kAhead || ref == -__builtin_inff())) {
-            const float mine = xor16_max(big);
-            const bool moves = mine > (ref == -__builtin_inff() ? -__builtin_inff() : kAhead);
-            const float to = moves ? __fadd_rn(at, mine) : ref;
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) top = fmaxf(top, __fmul_rn(sc[x >> 2][x & 3], cq));
+            top = xor16_max(top);
+            const bool moves = ref == -__builtin_inff() ? top > ref : xor16_max(big) > kAhead;
+            const float to = moves ? top : ref;
             const float down = ref == -__builtin_inff() ? 0.0f : (moves ? __builtin_amdgcn_exp2f(__fsub_rn(at, to)) : 1.0f);
             l = __fmul_rn(l, down);
             scale(down);
             ref = to;
             at = ref == -__builtin_inff() ? 0.0f : ref;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) y[x] = __fmaf_rn(sc[x >> 2][x & 3], cq, -at);
+            score(sc, cq, at, y);
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) {

@@ -114,7 +114,8 @@ int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, 
  * Arithmetic: the codes are exact in the matrix instructions' f16; queries and
  * softmax weights are taken in two f16 parts (22 bits) for BTL_F32, in one (11
  * bits; a bf16 query is exact) for BTL_BF16, scaled by powers of two so that they
- * neither overflow nor vanish; products are summed in f32, the softmax's maxima,
+ * neither overflow nor vanish (a row of queries all below 2^-96, and value scales
+ * below 2^-96, lose bits from there on); products are summed in f32, the softmax's maxima,
  * sums and outputs are f32.  What a row's mask hides has no effect on it, whatever
  * it holds; a row that sees a scale or holds a query that is not finite is NaN.
  * ws: btl_paged_attention_workspace_bytes (or NULL: the library's).  q, out 16-byte

@@ -243,8 +243,37 @@ def test_attention_of_large_and_small_numbers(dtype):
         q[2] *= np.float32(2.0 ** -100)
         cache[3][table[0, 0], :, :8] *= np.float32(2.0 ** 20)
         cache[3][table[0, 1], :, 3] = 0
-        cache[3][table[1]] *= np.float32(2.0 ** -90)
+        cache[3][table[1][:6]] *= np.float32(2.0 ** -90)
+        q[3] *= np.float32(2.0 ** -90)
+        cache[2][table[1][:6]] *= np.float32(2.0 ** 120)  # the second sequence's scores: as large as ever
+        cache[2][table[1][:6]] *= np.float32(2.0 ** 30)
     check_attention(8, 2, 64, 16, [(3, 40), (1, 90)], dtype, change=change)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [10, 30, 60])
+def test_attention_of_one_key(dtype, power):
+    """Scores so far apart that each row is its best key's value, of either sign, over several steps
+    and chunks (no rounding of a score changes which is best: they are whole multiples of one)."""
+    nh, nkv, hd, ps, sizes = 8, 2, 64, 16, [(1, 1300), (20, 90), (2, 3)]
+    rng = np.random.default_rng(power)
+    table, n_pages = ref.pages_for(sizes, ps, rng)
+    cache = ref.rand_cache(rng, n_pages, nkv, ps, hd)
+    cache[0][...] = 128
+    cache[0][..., 0] = rng.integers(1, 256, cache[0].shape[:3])
+    cache[2][...] = np.float32(2.0 ** power)
+    rows = sum(r for r, _ in sizes)
+    q = np.zeros((rows, nh, hd), np.float32)
+    q[..., 0] = np.where(rng.random((rows, nh)) < 0.5, 1024, -1024)
+    batch, starts = batch_of(table, sizes)
+    got = host(bl.paged_attention(dev(q.reshape(rows, -1), DT[dtype]), bl.PagedKVCacheQ8.of(*[dev(x) for x in cache]),
+                                  batch)).reshape(rows, nh, hd)
+    exp, _ = ref.attention(q, cache, table, sizes, starts, dtype == "bf16")
+    # equal best keys are averaged: their weights are alike, off by the f16 parts and the sums alone
+    most = 0.032 * 127
+    tol = (2.0 ** -8 if dtype == "bf16" else 2.0 ** -24) * np.abs(exp) + ((2.0 ** -11 if dtype == "bf16" else 2.0 ** -22)
+                                                                       + 1400 * 2.0 ** -24) * most
+    assert np.isfinite(got).all() and (np.abs(got - exp) <= tol).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -404,7 +433,7 @@ def test_sample_ties(n):
     logits[5, ::2] = -0.0
     logits[6] = rng.standard_normal(n) * 1e-4
     logits[7] = rng.integers(0, 3, n) * 50.0
-    for f in (dict(), dict(k=3333), dict(p=0.37), dict(k=4000, p=0.71), dict(m=0.9, k=4999)):
+    for f in (dict(), dict(k=3333), dict(p=0.37), dict(k=4000, p=0.71), dict(m=0.9, k=4999), dict(k=700), dict(k=1024, p=0.4)):
         cols = {c: [x] * rows for c, x in f.items()}
         check_sample(logits, u=rng.random(rows).astype(np.float32).tolist(), **cols)
 
@@ -427,7 +456,9 @@ def test_sample_odd_rows():
     for u in (0.0, 0.3, 0.999, 1.0, 7.0, -1.0, nan):
         print("sample odd", u, flush=True)
         check_sample(a, t=t, u=[u] * 12)
+        check_sample(a, t=t, k=[2] * 12, p=[0.7] * 12, u=[u] * 12)
     check_sample(a, t=t, p=[nan] * 12, m=[nan] * 12, u=[0.6] * 12)
+    check_sample(a, t=[1e38] * 12, k=[40] * 12, u=[0.6] * 12)  # every finite logit weighs the same
     ids, probs = bl.sample(dev(a), dev(np.full(12, 0.4, np.float32)))
     assert int(ids[0]) == -1 and int(ids[1]) == -1 and float(probs[0]) == 0
 
