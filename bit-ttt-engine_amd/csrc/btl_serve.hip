@@ -1033,10 +1033,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttn a)
     Place at = place_of(c, a.p.tile_n);
 
     // the sequence that the tile belongs to: sequences of more than `lo` query rows have
-    // one for every MT of them
+    // one for every MT of them.  A refused one has one for its NaN: the launch has tiles for
+    // max_rows rows of it, and the others come behind.
     at.s = __builtin_amdgcn_readfirstlane(find_piece(c, lane, at.tile, [&](int s) {
-        const int64_t rows = (int64_t)seq_at(c, s).n * a.group;
-        return rows > a.p.lo ? (int)((rows + MT - 1) / MT) : 0;
+        const Seq q = seq_at(c, s);
+        const int64_t rows = (int64_t)q.n * a.group;
+        return rows > a.p.lo ? (q.ok ? (int)((rows + MT - 1) / MT) : 1) : 0;
     }));
     if (at.s < 0) return;
     const Seq q = seq_at(c, at.s);
