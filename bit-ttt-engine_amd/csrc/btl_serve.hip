@@ -928,7 +928,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedAttn a)
         f4 sc[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            sc[t] = f4{lost, lost, lost, lost};
+            sc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const h8 k0 = widen8(kw[t][j].x, kw[t][j].y), k1 = widen8(kw[t][j].z, kw[t][j].w);
@@ -938,7 +938,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedAttn a)
                     sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qs.v[p][0][2 * j + 1], sc[t], 0, 0, 0);
                 }
             }
-            sc[t] *= ks[t];
+            // NaN where the page is outside the pool or a scale is not finite: an infinite one
+            // times a negative product would be -inf, which is a key that no row sees
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sc[t][e] = __fmaf_rn(sc[t][e], ks[t][e], __fmaf_rn(ks[t][e], 0.0f, __fmaf_rn(vs[t][e], 0.0f, lost)));
         }
         h8 pw[PARTS][2];
         if (kb + 64 <= q.p0 + 1) {  // every row sees every key
@@ -1095,9 +1099,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedAttn a)
                 s_v[b][wave + 4 * j][1][lane] = widen8(vw[j].z, vw[j].w);
             }
         }
-        if (wave == 0) s_ks[b][lane] = lost ? __builtin_nanf("") : scale;
+        // a scale that is not finite is NaN for whoever sees its key: an infinite one times a
+        // negative product would be -inf, which is a key that no row sees
+        const bool bad = !(__builtin_fabsf(scale) < __builtin_inff());
+        if (wave == 0) s_ks[b][lane] = lost || bad ? __builtin_nanf("") : scale;
         if (wave == 1) {
-            s_vs[b][lane] = scale;
+            s_vs[b][lane] = bad ? __builtin_nanf("") : scale;
             const uint32_t m = __float_as_uint(scale) & 0x7FFFFFFFu;
             const uint32_t top = wave_max_dpp(m < 0x7F800000u ? m : 0u);  // of finite ones
             if (lane == 0) s_top[b] = __uint_as_float(top);
