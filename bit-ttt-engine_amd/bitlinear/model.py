@@ -205,7 +205,10 @@ class BitLlamaHip:
         self.pos = 0
         self.graph = None
         self._expect = 0  # where a captured step will mostly run, if past self.pos
-        self._draw = None  # what the device loop's picks go by; None: greedy
+        # sample()'s buffers and the sampled device steps': made once and kept as long as the
+        # model, since a captured step holds their addresses
+        self._pick = self._loop = None
+        self._draw = None  # the device loop's picks go by it (self._loop); None: greedy
 
     # ------------------------------------------------------------------ steps
     def _stream(self):
@@ -390,20 +393,29 @@ class BitLlamaHip:
         """The pick of the current logits at a temperature (llama.rs:516-530) with the
         random number u in [0, 1) and the filters of btl_sample, on the device, into
         self.next_id; returns it as an int (synchronises)."""
-        self._set_draw(temperature, top_k, top_p, min_p)
-        d, self._draw = self._draw, None
-        d["u1"].fill_(float(u))
-        sample(self.logits, d["u1"], d["temperature"], d["top_k"], d["top_p"], d["min_p"], ids=self.next_id,
-               probs=d["probs"], workspace=d["space"])
+        if self._pick is None:
+            self._pick = self._draw_buffers()
+        self._set_filters(self._pick, temperature, top_k, top_p, min_p)
+        self._pick["u1"].fill_(float(u))
+        self._sample(self._pick)
         return int(self.next_id.item())
 
-    def _set_draw(self, temperature, top_k, top_p, min_p):
-        one = lambda v, t: torch.full((1,), v, dtype=t, device=self.dev)  # noqa: E731
+    def _draw_buffers(self):
+        one = lambda t: torch.zeros((1,), dtype=t, device=self.dev)  # noqa: E731
         f = torch.float32
-        self._draw = dict(temperature=one(float(temperature), f), top_k=one(int(top_k), torch.int32),
-                          top_p=one(float(top_p), f), min_p=one(float(min_p), f), u1=one(0.0, f), probs=one(0.0, f),
-                          u=torch.zeros((self.cfg.max_seq,), dtype=f, device=self.dev),
-                          space=sample_workspace(1, self.cfg.vocab, self.dev))
+        return dict(temperature=one(f), top_k=one(torch.int32), top_p=one(f), min_p=one(f), u1=one(f), probs=one(f),
+                    space=sample_workspace(1, self.cfg.vocab, self.dev))
+
+    @staticmethod
+    def _set_filters(d, temperature, top_k, top_p, min_p):
+        d["temperature"].fill_(float(temperature))
+        d["top_k"].fill_(int(top_k))
+        d["top_p"].fill_(float(top_p))
+        d["min_p"].fill_(float(min_p))
+
+    def _sample(self, d):
+        sample(self.logits, d["u1"], d["temperature"], d["top_k"], d["top_p"], d["min_p"], ids=self.next_id,
+               probs=d["probs"], workspace=d["space"])
 
     # ------------------------------------------------------- device decode loop
     def _step_device(self):
@@ -415,8 +427,7 @@ class BitLlamaHip:
         if self._draw is not None:
             d = self._draw
             torch.index_select(d["u"], 0, self.d_pos, out=d["u1"])
-            sample(self.logits, d["u1"], d["temperature"], d["top_k"], d["top_p"], d["min_p"], ids=self.next_id,
-                   probs=d["probs"], workspace=d["space"])
+            self._sample(d)
             self.d_pos.add_(1)
             self.log.index_copy_(0, self.d_pos.long(), self.next_id)
             return
@@ -471,8 +482,13 @@ class BitLlamaHip:
                 raise ValueError("%d tokens from position %d overflow the cache of %d rows"
                                  % (max_tokens, start, self.cfg.max_seq))
             self.sample(float(u[0]), temperature, top_k, top_p, min_p)
-            self._set_draw(temperature, top_k, top_p, min_p)
+            if self._loop is None:
+                self._loop = dict(self._draw_buffers(),
+                                  u=torch.zeros((self.cfg.max_seq,), dtype=torch.float32, device=self.dev))
+            self._draw = self._loop
+            self._set_filters(self._draw, temperature, top_k, top_p, min_p)
             # the token of position p + 1 is picked with *d_pos = p
+            self._draw["u"].zero_()
             self._draw["u"][start:start + max_tokens - 1].copy_(u[1:max_tokens])
         else:
             self.greedy()

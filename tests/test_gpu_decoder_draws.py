@@ -1,0 +1,66 @@
+"""GPU tests of BitLlamaHip's sampled picks used together: the host's pick (sample) between
+the device loop's captured steps."""
+import numpy as np
+import pytest
+import torch
+
+import serve_ref as ref
+from test_gpu_model import gpu_model
+from test_gpu_serve import host
+from test_model_oracle import TinyCfg, tiny_weights
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+
+F = dict(temperature=0.9, top_k=12, top_p=0.9, min_p=0.01)
+PROMPT = [3, 9, 27, 5]
+
+
+def model_of(seed=3):
+    cfg = TinyCfg()
+    return cfg, gpu_model(cfg, tiny_weights(cfg, seed), max_rows=8)
+
+
+def picked(logits, u, f=F):
+    return ref.sample_one(logits, f["temperature"], f["top_k"], f["top_p"], f["min_p"], float(u))[0]
+
+
+def definition(cfg, tokens, u, first, n, f=F, seed=3):
+    """The picks after `tokens`, of a model of its own: its first is drawn with u[first]."""
+    _, m = model_of(seed)
+    logits = host(m.prefill(tokens)).copy()
+    got = []
+    for i in range(n):
+        got.append(picked(logits, u[first + i], f))
+        logits = host(m.forward_one(got[-1])).copy()
+    return got
+
+
+def test_a_captured_steps_buffers_stay_where_they_are():
+    """sample() of other filters between replays: the captured step goes on by its own filters and
+    numbers, and writes nothing into memory that was taken meanwhile."""
+    cfg, m = model_of()
+    u = np.random.default_rng(4).random(40).astype(np.float32)
+    n = 10
+    first = m.generate(PROMPT, n, u=u, **F)
+    assert m.graph is not None
+    held = {k: t.data_ptr() for k, t in m._loop.items() if torch.is_tensor(t)}
+    m._loop["u"][m.pos:m.pos + 20].copy_(torch.from_numpy(u[n:n + 20]))
+    got, tokens = [], list(PROMPT) + [int(t) for t in first]
+    for step in range(4):
+        # a pick by other filters: the logits are those of the last token's predecessor
+        for v in (0.1, 0.9):
+            m.sample(v, temperature=1.3, top_k=3)
+        # whatever could have been freed is taken and marked
+        taken = [torch.full((k,), 123.0, device="cuda") for k in (1, 1, 1, 1, 1, cfg.max_seq, 4096, 65536)]
+        m.next_id.fill_(tokens[-1])
+        m.graph.replay()
+        m.pos += 1
+        torch.cuda.synchronize()
+        tokens.append(int(m.next_id))
+        got.append(tokens[-1])
+        assert all(bool((t == 123.0).all()) for t in taken)
+    assert {k: t.data_ptr() for k, t in m._loop.items() if torch.is_tensor(t)} == held
+    assert got == definition(cfg, list(PROMPT) + [int(t) for t in first], u, n, 4)
+    # generate again, captured over the same buffers
+    assert np.array_equal(m.generate(PROMPT, n, u=u, **F), first)
