@@ -209,6 +209,7 @@ class BitLlamaHip:
         # model, since a captured step holds their addresses
         self._pick = self._loop = None
         self._draw = None  # the device loop's picks go by it (self._loop); None: greedy
+        self._draw_end = 0  # the first position that has no random number
 
     # ------------------------------------------------------------------ steps
     def _stream(self):
@@ -449,17 +450,24 @@ class BitLlamaHip:
         return g
 
     def start_decode(self):
-        """Seed the device loop from the host state: *d_pos = pos, log[pos] = next_id."""
+        """Seed the device loop from the host state: *d_pos = pos, log[pos] = next_id.  The
+        steps from here on are greedy (generate's sampled ones end here)."""
+        if self._draw is not None:
+            self._draw = self.graph = None
         self.d_pos.fill_(self.pos)
         if self.pos < self.log.numel():
             self.log[self.pos:self.pos + 1].copy_(self.next_id)
 
     def decode_steps(self, n, use_graph=True):
-        """n greedy steps on the device, no host synchronisation in between; the
-        tokens accumulate in self.log."""
+        """n steps on the device, no host synchronisation in between; the tokens
+        accumulate in self.log.  Greedy, or after a sampled generate() by its filters and
+        the random numbers it was given beyond its tokens."""
         if self.pos + n > self.cfg.max_seq:
             raise ValueError("%d steps from position %d overflow the cache of %d rows"
                              % (n, self.pos, self.cfg.max_seq))
+        if self._draw is not None and n > 0 and self.pos + n > self._draw_end:
+            raise ValueError("%d sampled steps from position %d: random numbers were given for %d"
+                             % (n, self.pos, max(self._draw_end - self.pos, 0)))
         for _ in range(n):
             if use_graph and self.graph is not None:
                 self.graph.replay()
@@ -470,7 +478,8 @@ class BitLlamaHip:
     def generate(self, prompt_ids, max_tokens, use_graph=True, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
         """Llama::stream_completion (llama.rs:471-530): prefill, then decode, greedily at
         temperature 0, else by btl_sample with the filters and the random numbers u in
-        [0, 1), one a token (None: torch's).  Returns the max_tokens generated ids."""
+        [0, 1), one a token (None: torch's; more of them serve decode_steps calls that
+        follow).  Returns the max_tokens generated ids."""
         self.reset()
         self.prefill(prompt_ids)
         start = self.pos
@@ -482,17 +491,19 @@ class BitLlamaHip:
                 raise ValueError("%d tokens from position %d overflow the cache of %d rows"
                                  % (max_tokens, start, self.cfg.max_seq))
             self.sample(float(u[0]), temperature, top_k, top_p, min_p)
+            self.start_decode()
             if self._loop is None:
                 self._loop = dict(self._draw_buffers(),
                                   u=torch.zeros((self.cfg.max_seq,), dtype=torch.float32, device=self.dev))
             self._draw = self._loop
             self._set_filters(self._draw, temperature, top_k, top_p, min_p)
             # the token of position p + 1 is picked with *d_pos = p
+            self._draw_end = min(start + u.numel() - 1, self.cfg.max_seq)
             self._draw["u"].zero_()
-            self._draw["u"][start:start + max_tokens - 1].copy_(u[1:max_tokens])
+            self._draw["u"][start:self._draw_end].copy_(u[1:1 + self._draw_end - start])
         else:
             self.greedy()
-        self.start_decode()
+            self.start_decode()
         if max_tokens > 1:
             if use_graph:
                 # the attention's launches are chosen once for all the steps: by their middle

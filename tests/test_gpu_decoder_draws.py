@@ -64,3 +64,58 @@ def test_a_captured_steps_buffers_stay_where_they_are():
     assert got == definition(cfg, list(PROMPT) + [int(t) for t in first], u, n, 4)
     # generate again, captured over the same buffers
     assert np.array_equal(m.generate(PROMPT, n, u=u, **F), first)
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_steps_past_the_numbers_are_refused(use_graph):
+    """Numbers that generate() was given beyond its tokens serve the steps after it; past them a
+    step is refused and nothing moves; start_decode makes the loop greedy."""
+    cfg, m = model_of()
+    u = np.random.default_rng(5).random(30).astype(np.float32)
+    exp = m.generate(PROMPT, 14, use_graph=use_graph, u=u[:14], **F)
+    n = 9
+    got = m.generate(PROMPT, n, use_graph=use_graph, u=u[:14], **F)
+    assert np.array_equal(got, exp[:n])
+    m.decode_steps(2, use_graph=use_graph)
+    m.decode_steps(3, use_graph=use_graph)
+    start = len(PROMPT)
+    assert np.array_equal(m.log[start:start + 14].cpu().numpy(), exp)
+    for steps in (1, 7):
+        with pytest.raises(ValueError):
+            m.decode_steps(steps, use_graph=use_graph)
+    m.decode_steps(0, use_graph=use_graph)
+    assert m.pos == start + 13 and int(m.d_pos) == m.pos and int(m.next_id) == exp[-1]
+    # from here on greedily
+    logits = host(m.forward_one(int(exp[-1]))).copy()
+    m.greedy()
+    m.start_decode()
+    m.decode_steps(5, use_graph=use_graph)
+    tokens, greedy = list(PROMPT) + [int(t) for t in exp], []
+    for _ in range(6):
+        greedy.append(int(np.flatnonzero(logits == logits.max())[-1]))
+        tokens.append(greedy[-1])
+        fresh = model_of()[1]
+        logits = host(fresh.prefill(tokens)).copy()
+    assert m.log[m.pos - 5:m.pos + 1].cpu().numpy().tolist() == greedy
+    # exactly as many numbers as tokens: none is left for a step after them
+    m.generate(PROMPT, 3, use_graph=use_graph, u=u[:3], **F)
+    with pytest.raises(ValueError):
+        m.decode_steps(1, use_graph=use_graph)
+    # a single token is picked by the host alone; the loop goes on by the numbers behind it
+    one = m.generate(PROMPT, 1, use_graph=use_graph, u=u[:5], **F)
+    assert np.array_equal(one, exp[:1])
+    m.decode_steps(4, use_graph=use_graph)
+    assert np.array_equal(m.log[start:start + 5].cpu().numpy(), exp[:5])
+
+
+def test_numbers_to_the_end_of_the_cache():
+    cfg, m = model_of()
+    u = np.random.default_rng(6).random(cfg.max_seq + 50).astype(np.float32)
+    most = cfg.max_seq - len(PROMPT) + 1  # the last token needs no place
+    got = m.generate(PROMPT, most, u=u, **F)
+    assert got.tolist() == definition(cfg, PROMPT, u, 0, 3) + got.tolist()[3:]
+    assert np.array_equal(m.generate(PROMPT, most, use_graph=False, u=u[:most], **F), got)
+    with pytest.raises(ValueError):
+        m.decode_steps(1)
+    with pytest.raises(ValueError):
+        m.generate(PROMPT, most + 1, u=u, **F)
