@@ -149,7 +149,9 @@ class BitLlamaHip:
         self.ids = torch.zeros((M,), dtype=torch.int32, device=self.dev)
         self.next_id = torch.zeros((1,), dtype=torch.int32, device=self.dev)
         self.d_pos = torch.zeros((1,), dtype=torch.int32, device=self.dev)
-        self.log = torch.zeros((c.max_seq + 1,), dtype=torch.int32, device=self.dev)
+        # one place more than the log has takes the ids of steps past the cache's end
+        self._log = torch.zeros((c.max_seq + 2,), dtype=torch.int32, device=self.dev)
+        self.log = self._log[:c.max_seq + 1]
         cos = np.zeros((c.max_seq, c.head_dim // 2), np.float32)
         sin = np.zeros_like(cos)
         check(lib.btl_rope_table(float(c.rope_theta), c.head_dim, c.max_seq, cos.ctypes.data, sin.ctypes.data))
@@ -427,10 +429,13 @@ class BitLlamaHip:
         self._run(1, max(self.pos, self._expect), self.d_pos, self.next_id)
         if self._draw is not None:
             d = self._draw
-            torch.index_select(d["u"], 0, self.d_pos, out=d["u1"])
+            # *d_pos as an index that stays inside both arrays: a captured step that is replayed
+            # past the cache's end draws with 0 and leaves the log as it is, as btl_greedy_next does
+            torch.minimum(self.d_pos, d["end"], out=d["at"])
+            torch.index_select(d["u"], 0, d["at"], out=d["u1"])
             self._sample(d)
+            self._log[1:].index_copy_(0, d["at"], self.next_id)
             self.d_pos.add_(1)
-            self.log.index_copy_(0, self.d_pos.long(), self.next_id)
             return
         check(lib.btl_greedy_next(self.logits.data_ptr(), self.cfg.vocab, self.next_id.data_ptr(),
                                   self.d_pos.data_ptr(), self.log.data_ptr(), self.log.numel(), self._stream()))
@@ -493,8 +498,10 @@ class BitLlamaHip:
             self.sample(float(u[0]), temperature, top_k, top_p, min_p)
             self.start_decode()
             if self._loop is None:
-                self._loop = dict(self._draw_buffers(),
-                                  u=torch.zeros((self.cfg.max_seq,), dtype=torch.float32, device=self.dev))
+                i64 = dict(dtype=torch.int64, device=self.dev)
+                self._loop = dict(self._draw_buffers(), at=torch.zeros((1,), **i64),
+                                  end=torch.full((1,), self.cfg.max_seq, **i64),
+                                  u=torch.zeros((self.cfg.max_seq + 1,), dtype=torch.float32, device=self.dev))
             self._draw = self._loop
             self._set_filters(self._draw, temperature, top_k, top_p, min_p)
             # the token of position p + 1 is picked with *d_pos = p

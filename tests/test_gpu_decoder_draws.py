@@ -119,3 +119,25 @@ def test_numbers_to_the_end_of_the_cache():
         m.decode_steps(1)
     with pytest.raises(ValueError):
         m.generate(PROMPT, most + 1, u=u, **F)
+
+
+def test_a_captured_step_replayed_past_the_caches_end():
+    """Every index of a sampled step stays inside its array: steps past the last row store nothing
+    and leave the log as it is, as the greedy step's do."""
+    cfg, m = model_of()
+    u = np.random.default_rng(7).random(cfg.max_seq).astype(np.float32)
+    most = cfg.max_seq - len(PROMPT) + 1
+    for sampled in (False, True):
+        m.generate(PROMPT, most, **(dict(u=u, **F) if sampled else {}))
+        assert m.pos == cfg.max_seq == int(m.d_pos)
+        log = m.log.clone()
+        caches = [t.clone() for c in m.caches for t in (c.k, c.v, c.k_scale, c.v_scale)]
+        for i in range(3):
+            m.graph.replay()
+            torch.cuda.synchronize()
+            assert int(m.d_pos) == cfg.max_seq + 1 + i
+        assert torch.equal(m.log, log) and m.log.numel() == cfg.max_seq + 1
+        for a, b in zip(caches, (t for c in m.caches for t in (c.k, c.v, c.k_scale, c.v_scale))):
+            assert torch.equal(a, b)
+    # and the model goes on as ever
+    assert np.array_equal(m.generate(PROMPT, most, u=u, **F), m.generate(PROMPT, most, use_graph=False, u=u, **F))
