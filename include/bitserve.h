@@ -112,8 +112,10 @@ int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, 
  * it): softmax(q . k_deq / sqrt(head_dim)) . v_deq -> out, of dtype.  GQA head h
  * reads KV head h / (n_heads / n_kv), n_heads / n_kv <= 16.
  * Arithmetic: the codes are exact in the matrix instructions' f16; queries and
- * softmax weights are taken in two f16 parts (22 bits) for BTL_F32, in one (11
- * bits; a bf16 query is exact) for BTL_BF16, scaled by powers of two so that they
+ * softmax weights are taken in two f16 parts (22 bits) for BTL_F32; for BTL_BF16
+ * queries in one (exact), weights in two for sequences of at most 16 rows times
+ * heads of a group and in one (11 bits) for longer ones (for a single sequence
+ * max_rows decides it); scaled by powers of two so that they
  * neither overflow nor vanish (a row of queries all below 2^-96, and value scales
  * below 2^-96, lose bits from there on); products are summed in f32, the softmax's maxima,
  * sums and outputs are f32.  What a row's mask hides has no effect on it, whatever
