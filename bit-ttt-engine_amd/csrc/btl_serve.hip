@@ -537,8 +537,10 @@ hipError_t launch_paged_read(const PagedRead& a, hipStream_t st)
 //
 // A code u8 becomes the f16 1024 + u8 by one byte permute, less 1152 (exact).
 // Queries are scaled by a power of two per row to just under 2^15, softmax weights
-// times the value's scale by one per (row, largest value scale so far): what is
-// lost is below 2^-30 of the row's largest term, not below f16's smallest number.
+// times the value's scale by one per (row, largest value scale so far), which is then
+// in [2^8, 2^9): two parts keep 22 bits of a weight at the reference down to 2^-10 of
+// that scale, and what they lose of any is below 2^-33 of it, whatever the weight of
+// the key that has it.
 //
 // The softmax is taken in one pass against a reference that follows the row's
 // largest score, but only when a score passes it by 2^6: then the sums so far are
@@ -553,8 +555,8 @@ namespace {
 constexpr float kAhead = 6.0f;   // a score may pass the reference by this (log2)
 constexpr int kVUp = 8;          // weights times value scales stay below 2^(kAhead + 1 + kVUp) = 2^15
 // The least exponent of a query row, and of a value scale, that is scaled up in full:
-// a row's products, as far above their scores as its queries are scaled, stay below
-// 2^128 for scores up to 2^16.
+// a row's products are scaled as its queries are, by 2^(14 - e), so that q . k reaches
+// 2^128 there from 2^(114 + e) on; e = -96 leaves 2^18.
 constexpr int kLeastExp = -96;
 
 // four codes -> four f16 (code - 128)
@@ -1316,7 +1318,11 @@ AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c, bool bf)
     // Workgroups aimed at: two a CU where the sequences are few (one token over 100001
     // positions: 35.8 us and 5.0 for the merge with 512, 43 + 9.3 with 2048), more
     // where they are many and, as a batch's are, of different lengths (32 of up to
-    // 8192: 70.1 us with 4096, 73.2 with 512).
+    // 8192: 70.1 us with 4096, 73.2 with 512).  Between the two the rule is coarse: 8
+    // sequences of 8192 over 8 heads take 29.7 us with their merge, 9 take 41.1 (their
+    // chunks are the shortest, 256, and the merge the wide one), 16 take 55.8.  Chunks go
+    // by the host's bound: one token at 777 takes 9.2 us bounded by 2048 or less, 9.8 by
+    // 8192 and 14.4 by 131072, in one chunk a head.
     const int64_t want = heads <= 64 ? 512 : 4096;
     // 512 positions are one step of eight waves: 7.4 us, and 7.2 + 3.2 in chunks; 777 are
     // two steps: 11, and 7.2 + 3.2

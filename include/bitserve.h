@@ -115,11 +115,19 @@ int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, 
  * softmax weights are taken in two f16 parts (22 bits) for BTL_F32; for BTL_BF16
  * queries in one (exact), weights in two for sequences of at most 16 rows times
  * heads of a group and in one (11 bits) for longer ones (for a single sequence
- * max_rows decides it); scaled by powers of two so that they
- * neither overflow nor vanish (a row of queries all below 2^-96, and value scales
- * below 2^-96, lose bits from there on); products are summed in f32, the softmax's maxima,
- * sums and outputs are f32.  What a row's mask hides has no effect on it, whatever
- * it holds; a row that sees a scale or holds a query that is not finite is NaN.
+ * max_rows decides it); products are summed in f32, the softmax's maxima, sums and
+ * outputs are f32.  Powers of two keep the parts in f16's range: one a row, by its
+ * largest query, and one by the largest value scale that the row has seen.  Their
+ * limits, with 2^e <= the row's largest query: a row of queries all below 2^-96 loses
+ * bits from there on (e counts as -96); q . k of 2^(114 + e) and more is infinite (a
+ * positive one makes the row NaN, a negative one is not seen); values of scales below
+ * 2^-96, or below 2^-10 of the largest that the row sees, lose bits from there on, of a
+ * weight less than 2^-33 of the likeliest key's at that largest scale.
+ * What a row's mask hides has no effect on it, whatever it holds; a row that sees a
+ * scale or holds a query that is not finite is NaN.
+ * Chunks of keys, which are what few sequences spread over the chip by, are cut for
+ * max_len, not for the lengths that the device finds: a bound far above them leaves
+ * fewer and longer chunks.
  * ws: btl_paged_attention_workspace_bytes (or NULL: the library's).  q, out 16-byte
  * aligned; out overlaps nothing that is read.
  */
