@@ -1347,8 +1347,8 @@ AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c, bool bf)
 
 bool paged_attention_fits(const Paged& c, const AttnPlan& p)
 {
-    const int64_t most = ((int64_t)1 << 24) - 1;  // of 256 threads: under 2^32
-    return (int64_t)c.nkv * p.tok_n * c.n_seqs <= most && (int64_t)c.nkv * p.tile_n * p.tiles <= most;
+    const int64_t threads = ((int64_t)1 << 32) - 1;  // of a grid
+    return (int64_t)c.nkv * p.tok_n * c.n_seqs * 64 * p.tok_w <= threads && (int64_t)c.nkv * p.tile_n * p.tiles * 256 <= threads;
 }
 
 template <int DT, bool BF>

@@ -154,7 +154,8 @@ int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_
  * as -inf; with +inf among the logits only those share the weight; a row without a
  * finite or +inf logit has id -1 and probability 0.  A NaN filter is off; u below
  * 0 or NaN is taken as 0, from 1 on as the last token.
- * 1 <= n <= 2^22.  ws: btl_sample_workspace_bytes (or NULL: the library's).
+ * 1 <= n <= 2^22, at most 65535 rows.  ws: btl_sample_workspace_bytes (or NULL: the
+ * library's).
  */
 size_t btl_sample_workspace_bytes(int64_t rows, int64_t n);
 int btl_sample(const float* logits, int64_t rows, int64_t n, int64_t ld, const float* temperature,
