@@ -161,6 +161,16 @@ def test_attention_of_long_chunks(sizes, dtype):
     check_attention(8, 2, 32, 65536, sizes, dtype, max_len=131072)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_thousands_of_sequences(dtype):
+    """More than 64 * 64 of them: the search for a row's sequence takes a third step."""
+    sizes = [(1 + (i % 97 == 0), 1 + i % 11) if i % 5 else (0, 3) for i in range(4500)] + [(0, 0)] * 3
+    check_append(2, 1, 16, 16, sizes, dtype)
+    check_attention(2, 1, 16, 16, sizes, dtype)
+    sizes[4321] = (30, 50)  # a tile of one among them
+    check_attention(2, 1, 16, 16, sizes, dtype)
+
+
 # ------------------------------------------------------------------ which form runs
 
 def step_of(nh, nkv, hd, ps, sizes, dtype, max_len=None):
