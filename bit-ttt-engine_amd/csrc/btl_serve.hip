@@ -865,8 +865,8 @@ __device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h
 // Bound by the cache's bytes: every code is read once, 16 KB a step and wave in
 // flight, two waves a SIMD (registers: with one, loads prefetched a step ahead, it was
 // 92 us; with three it spills).  32 sequences of up to 8192 positions, 8 heads of 128,
-// bf16: 353 MB in 73 us, 4.8 TB/s; one of 100001, f32: 211 MB in 36 us, 5.9 TB/s (a
-// copy of 4 GiB reaches 4.7 TB/s, read and written).
+// bf16: 353 MB in 75 us, 4.7 TB/s; one of 100001, f32: 211 MB in 35 us, 6.0 TB/s (a
+// sum of 4 GiB reads 6.15 TB/s).
 template <int DT, int NW, bool BF>
 __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedAttn a)
 {
