@@ -171,6 +171,49 @@ def test_thousands_of_sequences(dtype):
     check_attention(2, 1, 16, 16, sizes, dtype)
 
 
+@pytest.mark.parametrize("rows,dtype", [(1, "f32"), (1, "bf16"), (21, "f32"), (21, "bf16")])
+def test_attention_over_the_most_tokens(rows, dtype):
+    """2^23 tokens, the most that a sequence may have, and one more, which is refused.
+
+    Sums of weights: a lane's 16 keys a step over at most 66 steps of a chunk, then lanes, waves and some
+    512 chunks, 64 a set: below 1200 additions in a row, each off by 2^-24, above and below the line; scores
+    off as in serve_ref.attention; weights in bf16 tiles by 2^-11.  Values lie on one side of 0, so every
+    chunk counts: one that is left out moves the result by a five hundredth of itself."""
+    nh = nkv = 1
+    hd, ps, n = 16, 65536, 2 ** 23
+    g = torch.Generator(device=DEV).manual_seed(3)
+    pages = n // ps
+    cache = bl.PagedKVCacheQ8(pages, ps, nkv, hd, DEV)
+    cache.k.random_(1, 256, generator=g)
+    cache.v.random_(160, 256, generator=g)
+    cache.k_scale.uniform_(0.002, 0.032, generator=g)
+    cache.v_scale.uniform_(0.002, 0.032, generator=g)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(4)).to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    q = (torch.randn((rows, hd), generator=g, device=DEV) * 2).to(DT[dtype])
+    batch = bl.PagedBatch(torch.tensor([0, rows], **i32), torch.tensor([n - rows], **i32),
+                          order.to(torch.int32)[None].contiguous(), rows)
+    got = bl.paged_attention(q, cache, batch).double()
+    k = (cache.k[order].view(n, hd).double() - 128) * cache.k_scale[order].view(n, 1).double()
+    v = cache.v[order].view(n // 16, hd, 16).transpose(1, 2).reshape(n, hd).double() - 128
+    v = v * cache.v_scale[order].view(n, 1).double()
+    u = 2.0 ** -24
+    for i in range(rows):
+        seen = n - rows + i + 1
+        x = q[i].double()
+        sc = (k[:seen] * x).sum(1) / hd ** 0.5
+        size = float((k[:seen].abs() * x.abs()).sum(1).max()) / hd ** 0.5
+        w = torch.softmax(sc, 0)
+        e = (w[:, None] * v[:seen]).sum(0)
+        rel = 2 * ((2.0 ** -22 + (hd + 4) * u) * size + 6 * u * size) + 2 * 1200 * u \
+            + (2.0 ** -11 if dtype == "bf16" and rows > 16 else 2.0 ** -22) + (2.0 ** -8 if dtype == "bf16" else u)
+        off = float(((got[i] - e).abs() / e).max())
+        print("most tokens", rows, dtype, i, "off by %.3g of %.3g" % (off, rel), flush=True)
+        assert off <= rel
+    past = bl.PagedBatch(batch.row_start, torch.tensor([n - rows + 1], **i32), batch.pages, rows)
+    assert bool(torch.isnan(bl.paged_attention(q, cache, past)).all())
+
+
 # ------------------------------------------------------------------ which form runs
 
 def step_of(nh, nkv, hd, ps, sizes, dtype, max_len=None):
