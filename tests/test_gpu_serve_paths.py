@@ -7,7 +7,7 @@ import torch
 import bitlinear as bl
 import serve_ref as ref
 from launches import launched
-from test_gpu_serve import (DEV, DT, batch_of, check_attention, dev, host, rope, same,
+from test_gpu_serve import (DEV, DT, batch_of, check_attention, check_sample, dev, host, rope, same,
                             test_append_writes_the_oracles_codes_and_nothing_else as check_append)
 
 pytestmark = [pytest.mark.gpu,
@@ -212,6 +212,20 @@ def test_attention_over_the_most_tokens(rows, dtype):
         assert off <= rel
     past = bl.PagedBatch(batch.row_start, torch.tensor([n - rows + 1], **i32), batch.pages, rows)
     assert bool(torch.isnan(bl.paged_attention(q, cache, past)).all())
+
+
+# ------------------------------------------------------------------ sampling
+
+def test_sample_of_the_longest_rows():
+    """2^22 logits: running weights up to 2^62, every token alike, and rows with a spread."""
+    n = 2 ** 22
+    u = np.array([0.0, 0.25, 0.7, 1 - 2.0 ** -24], np.float32)
+    ids, probs = bl.sample(torch.zeros((4, n), device=DEV), dev(u))
+    # floor(u W) of W = 2^62, over 2^40 a token
+    assert ids.tolist() == [int(float(x) * 2 ** 62) >> 40 for x in u] and probs.tolist() == [2.0 ** -22] * 4
+    rng = np.random.default_rng(5)
+    logits = (rng.standard_normal((2, n)) * 1.5).astype(np.float32)
+    check_sample(logits, t=[0.9, 1.0], p=[0.95, 1.0], k=[0, 3000000], u=[0.93, 0.9999])
 
 
 # ------------------------------------------------------------------ which form runs
