@@ -14,7 +14,7 @@ unsupported device in bit_linear.rs:76-84).
 from ._lib import (  # noqa: F401
     BTL_ACT_F32_REF, BTL_ACT_F32_SEQ, BTL_ACT_I8, BTL_BF16, BTL_ERR_ARG, BTL_ERR_DEVICE, BTL_ERR_DTYPE, BTL_ERR_FAULT,
     BTL_ERR_HIP, BTL_ERR_LAYOUT, BTL_ERR_SHAPE, BTL_ERR_WORKSPACE, BTL_F32, BTL_OK, EXPORTS,
-    LIB_PATH, BitLinearError, BtlKvPaged, BtlKvQ8, BtlPacked, BtlPagedBatch,
+    LIB_PATH, BitLinearError, BtlKvAccount, BtlKvPaged, BtlKvQ8, BtlPacked, BtlPagedBatch,
     BtlStreamLayer, check, check_faults, get_tuning, lib, set_tuning, tuning,
 )
 from .packed import PackedTensor  # noqa: F401
@@ -24,6 +24,7 @@ from .layer import (  # noqa: F401
 )
 from .adaptive import AdaptiveBitLinear, reconstruct_dense, split_bases  # noqa: F401,E402
 from .serve import (  # noqa: F401,E402
-    PagedBatch, PagedKVCacheQ8, paged_attention, paged_attention_workspace, paged_read, paged_rope_append, sample,
-    sample_workspace,
+    KVAccount, PagedBatch, PagedKVCacheQ8, paged_attention, paged_attention_account, paged_attention_account_workspace,
+    paged_attention_prefix, paged_attention_prefix_workspace, paged_attention_workspace, paged_evict,
+    paged_evict_workspace, paged_read, paged_rope_append, sample, sample_workspace,
 )

@@ -46,7 +46,10 @@ EXPORTS = (
     "btl_stream_create", "btl_stream_stage_words", "btl_stream_run", "btl_stream_destroy",
     # include/bitserve.h
     "btl_paged_rope_append", "btl_paged_read", "btl_paged_attention_workspace_bytes", "btl_paged_attention",
-    "btl_sample_workspace_bytes", "btl_sample",
+    "btl_sample_workspace_bytes", "btl_sample", "btl_paged_rope_append_shifted",
+    "btl_paged_attention_prefix_workspace_bytes", "btl_paged_attention_prefix",
+    "btl_paged_attention_account_workspace_bytes", "btl_paged_attention_account",
+    "btl_paged_evict_workspace_bytes", "btl_paged_evict",
 )
 
 
@@ -80,6 +83,12 @@ class BtlPagedBatch(ctypes.Structure):
     _fields_ = [("row_start", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("pages", ctypes.c_void_p),
                 ("n_seqs", ctypes.c_int64), ("max_pages", ctypes.c_int64), ("rows", ctypes.c_int64),
                 ("max_rows", ctypes.c_int64), ("max_len", ctypes.c_int64)]
+
+
+class BtlKvAccount(ctypes.Structure):
+    """btl_kv_account_t: what is known of the positions that the sequences of a batch hold."""
+    _fields_ = [("weight", ctypes.c_void_p), ("token", ctypes.c_void_p), ("filled", ctypes.c_void_p),
+                ("shift", ctypes.c_void_p), ("ld", ctypes.c_int64)]
 
 
 class BitLinearError(RuntimeError):
@@ -152,6 +161,17 @@ def _load():
         "btl_paged_read": (i32, [P(BtlKvPaged), P(BtlPagedBatch), vp, vp, i32, vp]),
         "btl_paged_attention_workspace_bytes": (sz, [i64, P(BtlKvPaged), P(BtlPagedBatch)]),
         "btl_paged_attention": (i32, [vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), vp, vp, sz, vp]),
+        "btl_paged_rope_append_shifted": (i32, [vp, vp, vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), vp, vp, vp, i64,
+                                                vp, vp]),
+        "btl_paged_attention_prefix_workspace_bytes": (sz, [i64, P(BtlKvPaged), P(BtlPagedBatch), P(BtlPagedBatch)]),
+        "btl_paged_attention_prefix": (i32, [vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), P(BtlPagedBatch), vp, vp, sz,
+                                             vp]),
+        "btl_paged_attention_account_workspace_bytes": (sz, [i64, P(BtlKvPaged), P(BtlPagedBatch), P(BtlPagedBatch)]),
+        "btl_paged_attention_account": (i32, [vp, i32, i64, P(BtlKvPaged), P(BtlPagedBatch), P(BtlPagedBatch),
+                                              P(BtlKvAccount), vp, vp, sz, vp]),
+        "btl_paged_evict_workspace_bytes": (sz, [P(BtlKvPaged), P(BtlPagedBatch)]),
+        "btl_paged_evict": (i32, [P(BtlKvPaged), P(BtlPagedBatch), P(BtlKvAccount), vp, vp, vp, i64, P(BtlKvAccount), vp,
+                                  vp, sz, vp]),
         "btl_sample_workspace_bytes": (sz, [i64, i64]),
         "btl_sample": (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     }

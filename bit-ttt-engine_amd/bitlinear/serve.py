@@ -1,6 +1,7 @@
 """Serving a batch of sequences (include/bitserve.h): a Q8 KV cache in pages of a
 shared pool, its append, its reading back, the attention over it, and the choice of
-next tokens.
+next tokens; prefixes that sequences share, the weights that positions are given, and
+sequences cut down to their positions of most weight.
 
 One-sequence counterparts: KVCacheQ8 and BitLlamaHip (bitlinear/model.py) over
 btl_rope_kv_append, btl_attention and btl_greedy_next.  Reference
@@ -12,6 +13,14 @@ layers/attention.rs:149-239, model/llama.rs:496-530 (the pick at a temperature).
     q = paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin)
     o = paged_attention(q, cache, batch)
     ids, probs = sample(logits, u, temperature=0.8, top_k=50, top_p=0.95)
+
+Behind a prompt that all of them share, and within a budget of positions:
+
+    prefix = PagedBatch([0, rows], [prompt], prompt_pages, rows, rows, prompt)   # lists of rows and their pages
+    account = KVAccount(n_seqs, n_kv_heads, max_len, "cuda", shift=prompt)       # one a layer
+    q = paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, rope_shift=account.shift)
+    o = paged_attention_account(q, cache, batch, account, prefix=prefix)
+    held = paged_evict(cache, batch, account, keep=2048, recent=256)             # pos of the next rows
 """
 import ctypes
 import functools
@@ -19,8 +28,8 @@ import functools
 import torch
 
 from ._lib import (
-    BTL_ERR_ARG, BTL_ERR_DEVICE, BTL_ERR_DTYPE, BTL_ERR_LAYOUT, BTL_ERR_SHAPE, BitLinearError, BtlKvPaged, BtlPagedBatch,
-    check, lib,
+    BTL_ERR_ARG, BTL_ERR_DEVICE, BTL_ERR_DTYPE, BTL_ERR_LAYOUT, BTL_ERR_SHAPE, BitLinearError, BtlKvAccount, BtlKvPaged,
+    BtlPagedBatch, check, lib,
 )
 from .layer import _DT, _dtype_code, _on_gpu
 
@@ -162,10 +171,11 @@ def _heads(q, cache, batch):
 
 
 @_on_its_device
-def paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, q_out=None):
+def paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, q_out=None, rope_shift=None):
     """btl_paged_rope_append: RoPE of the rows q [rows, n_heads * head_dim] and k [rows,
     n_kv * head_dim], k and v quantised into the cache.  Returns the rotated q (q_out,
-    which may be q).  rope_cos, rope_sin: float32 [positions, head_dim / 2]."""
+    which may be q).  rope_cos, rope_sin: float32 [positions, head_dim / 2].  rope_shift
+    (int32 [n_seqs]): what a sequence's RoPE positions have over its positions."""
     dt, nh, dev = _heads(q, cache, batch)
     kv = (batch.rows, cache.n_kv_heads * cache.head_dim)
     _tensor(k, "k", q.dtype, kv, dev)
@@ -177,9 +187,15 @@ def paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, q_out=None):
         q_out = torch.empty_like(q)
     else:
         _tensor(q_out, "q_out", q.dtype, q.shape, dev)
-    check(lib.btl_paged_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, nh, cache._ref, batch._ref,
-                                    rope_cos.data_ptr(), rope_sin.data_ptr(), length, q_out.data_ptr(),
-                                    _stream(dev)))
+    if rope_shift is None:
+        check(lib.btl_paged_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, nh, cache._ref, batch._ref,
+                                        rope_cos.data_ptr(), rope_sin.data_ptr(), length, q_out.data_ptr(),
+                                        _stream(dev)))
+        return q_out
+    _tensor(rope_shift, "rope_shift", torch.int32, (batch.c.n_seqs,), dev)
+    check(lib.btl_paged_rope_append_shifted(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, nh, cache._ref, batch._ref,
+                                            rope_shift.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), length,
+                                            q_out.data_ptr(), _stream(dev)))
     return q_out
 
 
@@ -220,6 +236,134 @@ def paged_attention(q, cache, batch, out=None, workspace=None):
 def paged_attention_workspace(cache, batch, n_heads):
     """A workspace for paged_attention calls of this cache's and batch's sizes."""
     return Scratch(lib.btl_paged_attention_workspace_bytes(n_heads, cache._ref, batch._ref), cache.device)
+
+
+def _prefix(prefix, batch, device):
+    if prefix.device != device:
+        raise BitLinearError(BTL_ERR_DEVICE, "the prefix is on %s, not on %s" % (prefix.device, device))
+    return prefix._ref
+
+
+@_on_its_device
+def paged_attention_prefix(q, cache, batch, prefix, out=None, workspace=None):
+    """btl_paged_attention_prefix: paged_attention of rows that also see a prefix, gone
+    through once for all rows of a list.  prefix: a PagedBatch over the same rows; list g's
+    rows row_start[g] .. row_start[g + 1] - 1 see all pos[g] positions of pages[g], ahead of
+    their sequence's own.  Returns out, of q's dtype."""
+    dt, nh, dev = _heads(q, cache, batch)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _tensor(out, "out", q.dtype, q.shape, dev)
+    wsp, wsn = _ws_args(workspace, dev)
+    check(lib.btl_paged_attention_prefix(q.data_ptr(), dt, nh, cache._ref, batch._ref, _prefix(prefix, batch, dev),
+                                         out.data_ptr(), wsp, wsn, _stream(dev)))
+    return out
+
+
+def paged_attention_prefix_workspace(cache, batch, prefix, n_heads):
+    """A workspace for paged_attention_prefix calls of these sizes."""
+    return Scratch(lib.btl_paged_attention_prefix_workspace_bytes(n_heads, cache._ref, batch._ref, prefix._ref),
+                   cache.device)
+
+
+class KVAccount:
+    """btl_kv_account_t: what is known of the positions that each sequence of a batch holds,
+    one a layer.  weight [n_seqs, n_kv_heads, positions] float32: the softmax weights that a
+    position was given; token (int32, the same shape), filled and shift (int32 [n_seqs]):
+    position j holds token[s, h, j] for j < filled[s], else j + shift[s].  A sequence begins
+    with filled 0 and shift 0, or its prefix's length."""
+
+    def __init__(self, n_seqs, n_kv_heads, positions, device="cuda", shift=0):
+        i32 = dict(dtype=torch.int32, device=device)
+        self._hold(torch.zeros((n_seqs, n_kv_heads, positions), dtype=torch.float32, device=device),
+                   torch.zeros((n_seqs, n_kv_heads, positions), **i32), torch.zeros((n_seqs,), **i32),
+                   torch.full((n_seqs,), shift, **i32))
+
+    @staticmethod
+    def of(weight, token=None, filled=None, shift=None):
+        """The account that lies in these tensors (the attention asks for the weights alone)."""
+        a = KVAccount.__new__(KVAccount)
+        a._hold(weight, token, filled, shift)
+        return a
+
+    def _hold(self, weight, token, filled, shift):
+        if not torch.is_tensor(weight) or weight.dim() != 3:
+            raise BitLinearError(BTL_ERR_SHAPE, "weight must be [n_seqs, n_kv_heads, positions]")
+        n, h, ld = weight.shape
+        dev = weight.device
+        self.weight = _tensor(weight, "weight", torch.float32, (n, h, ld), dev)
+        self.token = None if token is None else _tensor(token, "token", torch.int32, (n, h, ld), dev)
+        self.filled = None if filled is None else _tensor(filled, "filled", torch.int32, (n,), dev)
+        self.shift = None if shift is None else _tensor(shift, "shift", torch.int32, (n,), dev)
+        self.device, self.heads = dev, (n, h)
+        self.c = BtlKvAccount(*[None if t is None else t.data_ptr() for t in (self.weight, self.token, self.filled, self.shift)],
+                              ld)
+        self._ref = ctypes.byref(self.c)
+
+
+def _account(account, cache, batch, what="the account"):
+    if account.device != cache.device or batch.device != cache.device:
+        raise BitLinearError(BTL_ERR_DEVICE, "cache on %s, batch on %s, %s on %s"
+                             % (cache.device, batch.device, what, account.device))
+    if account.heads != (batch.c.n_seqs, cache.n_kv_heads):
+        raise BitLinearError(BTL_ERR_SHAPE, "%s is of %d sequences of %d KV heads, not of %d of %d"
+                             % (what, *account.heads, batch.c.n_seqs, cache.n_kv_heads))
+    return account._ref
+
+
+@_on_its_device
+def paged_attention_account(q, cache, batch, account, prefix=None, out=None, workspace=None):
+    """btl_paged_attention_account: paged_attention (with a prefix: paged_attention_prefix),
+    and account.weight of each sequence's own positions becomes the softmax weights that its
+    rows and the heads of a group gave them, added to what positions before this call's rows
+    had.  Returns out, of q's dtype."""
+    dt, nh, dev = _heads(q, cache, batch)
+    acc = _account(account, cache, batch)
+    pre = None if prefix is None else _prefix(prefix, batch, dev)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _tensor(out, "out", q.dtype, q.shape, dev)
+    wsp, wsn = _ws_args(workspace, dev)
+    check(lib.btl_paged_attention_account(q.data_ptr(), dt, nh, cache._ref, batch._ref, pre, acc, out.data_ptr(), wsp, wsn,
+                                          _stream(dev)))
+    return out
+
+
+def paged_attention_account_workspace(cache, batch, n_heads, prefix=None):
+    """A workspace for paged_attention_account calls of these sizes."""
+    return Scratch(lib.btl_paged_attention_account_workspace_bytes(n_heads, cache._ref, batch._ref,
+                                                                   None if prefix is None else prefix._ref), cache.device)
+
+
+@_on_its_device
+def paged_evict(cache, batch, account, keep, sink=None, recent=None, max_keep=None, out=None, held=None, workspace=None):
+    """btl_paged_evict: every sequence cut down to its keep[s] positions of most weight, each
+    KV head to its own; the first tokens (below sink[s]) and the last recent[s] are taken
+    first.  Those that stay below keep[s] are not touched, the others fill its holes.  keep,
+    sink, recent: int32 tensors [n_seqs], numbers, or None (sink, recent: 0); max_keep: a
+    bound on what sequences are cut down to (default: the number, or the account's positions).  out: the account that
+    is put out (default: account itself).  Returns held, int32 [n_seqs]: the positions each
+    sequence has now, the pos of its next rows (-1: refused)."""
+    dev, n = cache.device, batch.c.n_seqs
+    acc = _account(account, cache, batch)
+    acc_out = None if out is None else _account(out, cache, batch, "the account put out")
+    if max_keep is None:
+        max_keep = account.c.ld if torch.is_tensor(keep) else max(int(keep), 0)
+    row = [_per_row(keep, "keep", torch.int32, n, dev), _per_row(sink, "sink", torch.int32, n, dev),
+           _per_row(recent, "recent", torch.int32, n, dev)]
+    held = torch.empty((n,), dtype=torch.int32, device=dev) if held is None \
+        else _tensor(held, "held", torch.int32, (n,), dev)
+    wsp, wsn = _ws_args(workspace, dev)
+    check(lib.btl_paged_evict(cache._ref, batch._ref, acc, *[None if t is None else t.data_ptr() for t in row], max_keep,
+                              acc_out, held.data_ptr(), wsp, wsn, _stream(dev)))
+    return held
+
+
+def paged_evict_workspace(cache, batch):
+    """A workspace for paged_evict calls of these sizes."""
+    return Scratch(lib.btl_paged_evict_workspace_bytes(cache._ref, batch._ref), cache.device)
 
 
 def _per_row(v, what, dtype, rows, device):

@@ -229,6 +229,18 @@ pub struct btl_paged_batch_t {
     pub max_len: i64,
 }
 
+/// `btl_kv_account_t`: what is known of the positions that the sequences of a batch hold
+/// (device arrays; weight and token [n_seqs, n_kv_heads, ld], filled and shift [n_seqs]).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct btl_kv_account_t {
+    pub weight: *mut f32,
+    pub token: *mut i32,
+    pub filled: *mut i32,
+    pub shift: *mut i32,
+    pub ld: i64,
+}
+
 extern "C" {
     pub fn btl_paged_rope_append(q: *const c_void, k: *const c_void, v: *const c_void, dtype: c_int, n_heads: i64,
                                  cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t,
@@ -241,6 +253,28 @@ extern "C" {
     pub fn btl_paged_attention(q: *const c_void, dtype: c_int, n_heads: i64, cache: *const btl_kv_paged_t,
                                batch: *const btl_paged_batch_t, out: *mut c_void, ws: *mut c_void,
                                ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn btl_paged_rope_append_shifted(q: *const c_void, k: *const c_void, v: *const c_void, dtype: c_int,
+                                         n_heads: i64, cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t,
+                                         rope_shift: *const i32, rope_cos: *const f32, rope_sin: *const f32,
+                                         rope_len: i64, q_out: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn btl_paged_attention_prefix_workspace_bytes(n_heads: i64, cache: *const btl_kv_paged_t,
+                                                      batch: *const btl_paged_batch_t,
+                                                      prefix: *const btl_paged_batch_t) -> usize;
+    pub fn btl_paged_attention_prefix(q: *const c_void, dtype: c_int, n_heads: i64, cache: *const btl_kv_paged_t,
+                                      batch: *const btl_paged_batch_t, prefix: *const btl_paged_batch_t,
+                                      out: *mut c_void, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn btl_paged_attention_account_workspace_bytes(n_heads: i64, cache: *const btl_kv_paged_t,
+                                                       batch: *const btl_paged_batch_t,
+                                                       prefix: *const btl_paged_batch_t) -> usize;
+    pub fn btl_paged_attention_account(q: *const c_void, dtype: c_int, n_heads: i64, cache: *const btl_kv_paged_t,
+                                       batch: *const btl_paged_batch_t, prefix: *const btl_paged_batch_t,
+                                       account: *const btl_kv_account_t, out: *mut c_void, ws: *mut c_void,
+                                       ws_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn btl_paged_evict_workspace_bytes(cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t) -> usize;
+    pub fn btl_paged_evict(cache: *const btl_kv_paged_t, batch: *const btl_paged_batch_t,
+                           account: *const btl_kv_account_t, keep: *const i32, sink: *const i32, recent: *const i32,
+                           max_keep: i64, account_out: *const btl_kv_account_t, held: *mut i32, ws: *mut c_void,
+                           ws_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn btl_sample_workspace_bytes(rows: i64, n: i64) -> usize;
     pub fn btl_sample(logits: *const f32, rows: i64, n: i64, ld: i64, temperature: *const f32, top_k: *const i32,
                       top_p: *const f32, min_p: *const f32, u: *const f32, ids: *mut i32, probs: *mut f32,

@@ -1,5 +1,5 @@
 // btl_serve.hpp -- kernel arguments and launchers of the batched serving ops
-// (btl_serve.hip, btl_sample.hip), checked and filled by btl_serve_api.cpp.
+// (btl_serve.hip, btl_share.hip, btl_evict.hip, btl_sample.hip), checked and filled by btl_serve_api.cpp.
 // Not part of the public ABI.
 #pragma once
 
@@ -34,6 +34,7 @@ struct PagedAppend {
     const float* sin_t;
     int rope_len, nh;
     int bf;  // rows are bf16
+    const int32_t* shift;  // RoPE positions less positions, a sequence, or NULL
 };
 hipError_t launch_paged_append(const PagedAppend& a, hipStream_t st);
 
@@ -76,6 +77,57 @@ struct PagedAttn {
     int bf;
 };
 hipError_t launch_paged_attention(const PagedAttn& a, hipStream_t st);
+
+// Attention beside a prefix that row lists share, and with the rows' weights added up.
+struct PagedShare : PagedAttn {
+    Paged g;       // the prefix: its lists of rows and pages (n_seqs 0: none)
+    AttnPlan gp;
+    int own0;      // a row's parts: the prefix's chunks, and from here on its sequence's
+    int split;     // a sequence of one chunk is merged as well
+    float* ml;     // [rows * nh][2]: a row's maximum and sum (log2 domain), or NULL
+    // the token form's scores, log2 domain, -inf where a row does not see: [n_seqs][nkv][score_rows][score_ld]
+    float* scores;
+    int score_rows;
+    int score_ld;
+    // accounted weights
+    float* weight;  // [n_seqs][nkv][ld]
+    int64_t ld;
+    float* sums;    // [splits][n_seqs][nkv][score_ld]: a position's weight from a share of the rows
+    int splits;     // shares of the rows of a sequence that is too long for the token form's scores
+    int scored;     // sequences of the token form have scores
+};
+AttnPlan plan_paged_prefix(int64_t n_heads, const Paged& g, bool bf);
+// fills a's split of the accounting; false: too large for one launch
+bool plan_paged_account(int64_t n_heads, PagedShare& a);
+hipError_t launch_paged_share(const PagedShare& a, hipStream_t st);
+
+struct PagedEvict {
+    Paged c;
+    // a head's weights and tokens lie ld apart
+    const float* weight;
+    const int32_t* token;
+    const int32_t* filled;
+    const int32_t* shift;
+    float* weight_out;
+    int32_t* token_out;
+    int32_t* filled_out;
+    int32_t* shift_out;
+    int64_t ld, ld_out;
+    const int32_t* keep;
+    const int32_t* sink;    // or NULL
+    const int32_t* recent;  // or NULL
+    int32_t* held;
+    int max_keep, from_ld;
+    int32_t* from;    // [n_seqs][nkv][from_ld]
+    int32_t* movers;  // [n_seqs][nkv][cap]
+};
+// workgroups along the slots that may be written to
+inline int evict_blocks(const PagedEvict& a)
+{
+    const int most = a.max_keep < a.c.cap ? a.max_keep : a.c.cap;
+    return most > 64 ? (most + 63) / 64 : 1;
+}
+hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st);
 
 // sampling
 constexpr int kSampleBins = 1024;

@@ -1,5 +1,6 @@
 // btl_serve_api.cpp -- C ABI of the batched serving ops (include/bitserve.h):
-// validation and dispatch to the kernels of btl_serve.hip and btl_sample.hip.
+// validation and dispatch to the kernels of btl_serve.hip, btl_share.hip, btl_evict.hip
+// and btl_sample.hip.
 #include "bitserve.h"
 
 #include <hip/hip_runtime_api.h>
@@ -89,6 +90,16 @@ int check_pointers(const btl_kv_paged_t* k, const btl_paged_batch_t* b, btl::Pag
     return BTL_OK;
 }
 
+// The prefix of a call: a batch over the same rows.
+int check_prefix(const btl_kv_paged_t* k, const btl_paged_batch_t* b, const btl_paged_batch_t* prefix, btl::Paged* g)
+{
+    int rc;
+    if ((rc = check_sizes(k, prefix, g))) return rc;
+    if (prefix->rows != b->rows)
+        return failf(BTL_ERR_SHAPE, "the prefix has %lld rows, the batch %lld", (long long)prefix->rows, (long long)b->rows);
+    return BTL_OK;
+}
+
 int check_heads(int64_t n_heads, const btl::Paged& c)
 {
     if (n_heads < 1 || n_heads % c.nkv || n_heads / c.nkv > 16)
@@ -102,6 +113,50 @@ size_t attention_bytes(const btl::Paged& c, int64_t n_heads, const btl::AttnPlan
     if (p.parts() <= 1) return 0;
     const size_t n = (size_t)c.rows * n_heads * p.parts();
     return up256(n * c.hd * 4) + up256(n * 8);
+}
+
+// Where the parts of a call beside a prefix or with weights lie in its workspace.
+struct ShareWs {
+    size_t part_ml, ml, scores, sums, total;
+};
+ShareWs share_ws(const btl::PagedShare& a, int64_t n_heads, bool account)
+{
+    const size_t heads = (size_t)a.c.rows * n_heads, parts = a.parts > 1 || a.split ? a.parts : 0;
+    ShareWs w{};
+    w.part_ml = up256(heads * parts * a.c.hd * 4);
+    w.ml = w.part_ml + up256(heads * parts * 8);
+    w.scores = w.ml + (account ? up256(heads * 8) : 0);
+    const size_t keys = (size_t)a.c.n_seqs * a.c.nkv * a.score_ld;
+    w.sums = w.scores + (account && a.scored ? up256(keys * a.score_rows * 4) : 0);
+    w.total = w.sums + (account && a.splits > 1 ? up256(keys * a.splits * 4) : 0);
+    return w;
+}
+
+// The plan of such a call; false: too large for its launches.
+bool plan_share(btl::PagedShare& a, int64_t n_heads, bool bf, bool account)
+{
+    a.p = btl::plan_paged_attention(n_heads, a.c, bf);
+    a.split = a.g.n_seqs > 0;
+    if (a.split) a.gp = btl::plan_paged_prefix(n_heads, a.g, bf);
+    a.own0 = a.split ? a.gp.parts() : 0;
+    a.parts = a.own0 + a.p.parts();
+    a.splits = 1;
+    const bool fits = btl::paged_attention_fits(a.c, a.p) && (!a.split || btl::paged_attention_fits(a.g, a.gp));
+    return (!account || btl::plan_paged_account(n_heads, a)) && fits;
+}
+
+size_t share_bytes(int64_t n_heads, const btl_kv_paged_t* cache, const btl_paged_batch_t* batch,
+                   const btl_paged_batch_t* prefix, bool account)
+{
+    btl::PagedShare a{};
+    if (check_sizes(cache, batch, &a.c) || check_heads(n_heads, a.c) || a.c.rows == 0 || a.c.n_seqs == 0) return 0;
+    if (prefix && check_prefix(cache, batch, prefix, &a.g)) return 0;
+    size_t most = 0;
+    for (int bf = 0; bf < 2; ++bf) {
+        if (!plan_share(a, n_heads, bf, account)) return 0;
+        most = std::max(most, share_ws(a, n_heads, account).total);
+    }
+    return most;
 }
 
 struct SampleWs {
@@ -126,6 +181,15 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
                           const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const float* rope_cos,
                           const float* rope_sin, int64_t rope_len, void* q_out, void* stream)
 {
+    return btl_paged_rope_append_shifted(q, k, v, dtype, n_heads, cache, batch, nullptr, rope_cos, rope_sin, rope_len,
+                                         q_out, stream);
+}
+
+int btl_paged_rope_append_shifted(const void* q, const void* k, const void* v, int dtype, int64_t n_heads,
+                                  const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const int32_t* rope_shift,
+                                  const float* rope_cos, const float* rope_sin, int64_t rope_len, void* q_out,
+                                  void* stream)
+{
     btl::PagedAppend a{};
     int rc;
     if ((rc = check_dtype(dtype)) || (rc = check_sizes(cache, batch, &a.c)) || (rc = check_heads(n_heads, a.c))) return rc;
@@ -139,6 +203,7 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
     const size_t qn = (size_t)a.c.rows * n_heads * a.c.hd * size, kn = (size_t)a.c.rows * a.c.nkv * a.c.hd * size;
     if ((q_out != q && overlap(q_out, qn, q, qn)) || overlap(q_out, qn, k, kn) || overlap(q_out, qn, v, kn))
         return fail_msg(BTL_ERR_LAYOUT, "q_out must be q itself or not overlap q, k and v");
+    if (!aligned4(rope_shift)) return fail_msg(BTL_ERR_LAYOUT, "rope_shift must be 4-byte aligned");
     int dev;
     if ((rc = btl::host::device(&dev))) return rc;
     a.q = q;
@@ -148,6 +213,7 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
     a.cos_t = rope_cos;
     a.sin_t = rope_sin;
     a.rope_len = (int)rope_len;
+    a.shift = rope_shift;
     a.nh = (int)n_heads;
     a.bf = dtype == BTL_BF16;
     const hipError_t e = btl::launch_paged_append(a, (hipStream_t)stream);
@@ -216,6 +282,175 @@ int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_
     a.bf = dtype == BTL_BF16;
     const hipError_t e = btl::launch_paged_attention(a, (hipStream_t)stream);
     return e == hipSuccess ? BTL_OK : hip_error(e, "paged attention kernel launch");
+}
+
+// btl_paged_attention_prefix (no account) and btl_paged_attention_account.
+static int attention_share(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
+                           const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix, const btl_kv_account_t* account,
+                           void* out, void* ws, size_t ws_bytes, void* stream)
+{
+    btl::PagedShare a{};
+    int rc;
+    if ((rc = check_dtype(dtype)) || (rc = check_sizes(cache, batch, &a.c)) || (rc = check_heads(n_heads, a.c))) return rc;
+    if (prefix && (rc = check_prefix(cache, batch, prefix, &a.g))) return rc;
+    if (account && (account->ld < a.c.cap || account->ld > ((int64_t)1 << 32)))
+        return failf(BTL_ERR_SHAPE, "an account of %lld positions a head, for sequences of up to %d", (long long)account->ld, a.c.cap);
+    if (a.c.rows == 0 || a.c.n_seqs == 0) return BTL_OK;
+    if (!plan_share(a, n_heads, dtype == BTL_BF16, account)) return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
+    if ((rc = check_pointers(cache, batch, &a.c)) || (a.split && (rc = check_pointers(cache, prefix, &a.g)))) return rc;
+    if (!q || !out || (account && !account->weight)) return fail_msg(BTL_ERR_LAYOUT, "null pointer");
+    if (!aligned16(q) || !aligned16(out)) return fail_msg(BTL_ERR_LAYOUT, "q and out must be 16-byte aligned");
+    if (account && !aligned4(account->weight)) return fail_msg(BTL_ERR_LAYOUT, "weights must be 4-byte aligned");
+    const size_t qn = (size_t)a.c.rows * n_heads * a.c.hd * (dtype == BTL_F32 ? 4 : 2);
+    if (overlap(out, qn, q, qn)) return fail_msg(BTL_ERR_LAYOUT, "out overlaps q");
+    if (account) {
+        const size_t wn = (size_t)a.c.n_seqs * a.c.nkv * account->ld * 4;
+        if (overlap(account->weight, wn, q, qn) || overlap(account->weight, wn, out, qn))
+            return fail_msg(BTL_ERR_LAYOUT, "the weights overlap q or out");
+    }
+    int dev;
+    if ((rc = btl::host::device(&dev))) return rc;
+    const ShareWs w = share_ws(a, n_heads, account);
+    if (w.total) {
+        void* p = nullptr;
+        if ((rc = btl::host::workspace(dev, ws, ws_bytes, w.total, &p, (hipStream_t)stream))) return rc;
+        a.part_o = (float*)p;
+        a.part_ml = (float*)((uint8_t*)p + w.part_ml);
+        a.scores = (float*)((uint8_t*)p + w.scores);
+        a.sums = (float*)((uint8_t*)p + w.sums);
+        if (account) a.ml = (float*)((uint8_t*)p + w.ml);
+    }
+    if (account) {
+        a.weight = account->weight;
+        a.ld = account->ld;
+    }
+    a.q = q;
+    a.out = out;
+    a.nh = (int)n_heads;
+    a.group = (int)n_heads / a.c.nkv;
+    a.group_mul = (uint32_t)((((int64_t)1 << 31) + a.group - 1) / a.group);
+    a.scale_log2 = (float)(1.4426950408889634074 / std::sqrt((double)a.c.hd));
+    a.bf = dtype == BTL_BF16;
+    const hipError_t e = btl::launch_paged_share(a, (hipStream_t)stream);
+    return e == hipSuccess ? BTL_OK : hip_error(e, "paged attention kernel launch");
+}
+
+size_t btl_paged_attention_prefix_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,
+                                                  const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix)
+{
+    return prefix ? share_bytes(n_heads, cache, batch, prefix, false) : 0;
+}
+
+int btl_paged_attention_prefix(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
+                               const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix, void* out, void* ws,
+                               size_t ws_bytes, void* stream)
+{
+    if (!prefix) return fail_msg(BTL_ERR_ARG, "null prefix");
+    return attention_share(q, dtype, n_heads, cache, batch, prefix, nullptr, out, ws, ws_bytes, stream);
+}
+
+size_t btl_paged_attention_account_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,
+                                                   const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix)
+{
+    return share_bytes(n_heads, cache, batch, prefix, true);
+}
+
+int btl_paged_attention_account(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
+                                const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix,
+                                const btl_kv_account_t* account, void* out, void* ws, size_t ws_bytes, void* stream)
+{
+    if (!account) return fail_msg(BTL_ERR_ARG, "null account");
+    return attention_share(q, dtype, n_heads, cache, batch, prefix, account, out, ws, ws_bytes, stream);
+}
+
+static size_t evict_bytes(const btl::Paged& c, size_t* movers)
+{
+    const size_t n = (size_t)c.n_seqs * c.nkv * c.cap * 4;
+    *movers = up256(n);
+    return 2 * up256(n);
+}
+
+size_t btl_paged_evict_workspace_bytes(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch)
+{
+    btl::Paged c{};
+    size_t movers;
+    return check_sizes(cache, batch, &c) ? 0 : evict_bytes(c, &movers);
+}
+
+int btl_paged_evict(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const btl_kv_account_t* account,
+                    const int32_t* keep, const int32_t* sink, const int32_t* recent, int64_t max_keep,
+                    const btl_kv_account_t* account_out, int32_t* held, void* ws, size_t ws_bytes, void* stream)
+{
+    btl::PagedEvict a{};
+    int rc;
+    if ((rc = check_sizes(cache, batch, &a.c))) return rc;
+    if (!account) return fail_msg(BTL_ERR_ARG, "null account");
+    const btl_kv_account_t* to = account_out ? account_out : account;
+    if (max_keep < 0) return failf(BTL_ERR_SHAPE, "max_keep %lld is negative", (long long)max_keep);
+    const int64_t ld = std::min(account->ld, to->ld);
+    if (ld < a.c.cap || std::max(account->ld, to->ld) > ((int64_t)1 << 32))
+        return failf(BTL_ERR_SHAPE, "an account of %lld positions a head, for sequences of up to %d", (long long)ld, a.c.cap);
+    if (a.c.n_seqs == 0) return BTL_OK;
+    a.max_keep = (int)std::min<int64_t>(max_keep, INT_MAX);
+    const int64_t threads = ((int64_t)1 << 32) - 1;
+    if ((int64_t)a.c.nkv * a.c.n_seqs * 1024 > threads ||
+        (int64_t)a.c.nkv * a.c.n_seqs * btl::evict_blocks(a) * 256 > threads)
+        return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
+    if ((rc = check_pointers(cache, batch, &a.c))) return rc;
+    for (const btl_kv_account_t* x : {account, to}) {
+        if (!x->weight || !x->token || !x->filled || !x->shift) return fail_msg(BTL_ERR_LAYOUT, "null account array");
+        if (!aligned4(x->weight) || !aligned4(x->token) || !aligned4(x->filled) || !aligned4(x->shift))
+            return fail_msg(BTL_ERR_LAYOUT, "account arrays must be 4-byte aligned");
+    }
+    if (!keep || !held) return fail_msg(BTL_ERR_LAYOUT, "null pointer");
+    if (!aligned4(keep) || !aligned4(sink) || !aligned4(recent) || !aligned4(held))
+        return fail_msg(BTL_ERR_LAYOUT, "keep, sink, recent and held must be 4-byte aligned");
+    // what is written is read by nobody else: an array put out is the one that came in, or apart from all
+    struct Span {
+        const void* p;
+        size_t n;
+    };
+    const size_t n4 = (size_t)a.c.n_seqs * 4, heads = (size_t)a.c.n_seqs * a.c.nkv * 4;
+    const Span in[] = {{account->weight, heads * account->ld}, {account->token, heads * account->ld}, {account->filled, n4},
+                       {account->shift, n4}, {keep, n4}, {sink, n4}, {recent, n4}, {batch->pos, n4},
+                       {batch->row_start, n4 + 4}, {batch->pages, n4 * a.c.max_pages}};
+    const Span out[] = {{to->weight, heads * to->ld}, {to->token, heads * to->ld}, {to->filled, n4}, {to->shift, n4},
+                        {held, n4}};
+    for (int i = 0; i < 5; ++i) {
+        for (int j = 0; j < 10; ++j) {
+            const bool itself = i == j && i < 4 && out[i].p == in[j].p && out[i].n == in[j].n;
+            if (!itself && overlap(out[i].p, out[i].n, in[j].p, in[j].n))
+                return fail_msg(BTL_ERR_LAYOUT, "an array that is put out must be the account's own or overlap none that is read");
+        }
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i].p, out[i].n, out[j].p, out[j].n))
+                return fail_msg(BTL_ERR_LAYOUT, "arrays that are put out overlap");
+    }
+    int dev;
+    if ((rc = btl::host::device(&dev))) return rc;
+    size_t movers;
+    void* p = nullptr;
+    const size_t need = evict_bytes(a.c, &movers);
+    if (need && (rc = btl::host::workspace(dev, ws, ws_bytes, need, &p, (hipStream_t)stream))) return rc;
+    a.from = (int32_t*)p;
+    a.movers = (int32_t*)((uint8_t*)p + movers);
+    a.from_ld = a.c.cap;
+    a.weight = account->weight;
+    a.token = account->token;
+    a.filled = account->filled;
+    a.shift = account->shift;
+    a.ld = account->ld;
+    a.weight_out = to->weight;
+    a.token_out = to->token;
+    a.filled_out = to->filled;
+    a.shift_out = to->shift;
+    a.ld_out = to->ld;
+    a.keep = keep;
+    a.sink = sink;
+    a.recent = recent;
+    a.held = held;
+    const hipError_t e = btl::launch_paged_evict(a, (hipStream_t)stream);
+    return e == hipSuccess ? BTL_OK : hip_error(e, "eviction kernel launch");
 }
 
 size_t btl_sample_workspace_bytes(int64_t rows, int64_t n)

@@ -2,7 +2,9 @@
  * bitserve.h -- C ABI of the operators that serve a batch of sequences together
  * (MI355X / gfx950): a Q8 KV cache in pages of a shared pool, its append, its
  * reading back, the attention of every sequence's new rows over it, and the
- * choice of next tokens from logits.
+ * choice of next tokens from logits; and what long contexts ask for besides: a prefix
+ * that many sequences share, the weight that each position has been given, and
+ * sequences cut down to their positions of most weight.
  *
  * They stand beside their one-sequence counterparts of bitllama.h
  * (btl_rope_kv_append, btl_attention, btl_greedy_next); the reference
@@ -97,6 +99,18 @@ int btl_paged_rope_append(const void* q, const void* k, const void* v, int dtype
                           const float* rope_sin, int64_t rope_len, void* q_out, void* stream);
 
 /*
+ * The same with RoPE positions that are not the positions in the cache: row i of
+ * sequence s turns at pos + i + rope_shift[s] (device int32 [n_seqs], or NULL: 0) and
+ * lies at pos + i as before.  That is a sequence behind a shared prefix, or one that
+ * positions were evicted from.  A row whose RoPE position is outside [0, rope_len) is
+ * not stored and its q_out is NaN.
+ */
+int btl_paged_rope_append_shifted(const void* q, const void* k, const void* v, int dtype, int64_t n_heads,
+                                  const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const int32_t* rope_shift,
+                                  const float* rope_cos, const float* rope_sin, int64_t rope_len, void* q_out,
+                                  void* stream);
+
+/*
  * The cache read back: for every row, its position's key and value (code - 128) *
  * scale into k_out and v_out [rows, n_kv * head_dim] of dtype (either may be
  * NULL), 16-byte aligned.  Whole contexts are rows at pos = 0.  Keys are as stored,
@@ -135,6 +149,90 @@ size_t btl_paged_attention_workspace_bytes(int64_t n_heads, const btl_kv_paged_t
                                            const btl_paged_batch_t* batch);
 int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
                         const btl_paged_batch_t* batch, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * btl_paged_attention of rows that also see a prefix, whose pages are gone through once
+ * for all the rows that share it.  `prefix` is a batch over the same rows: list g of it
+ * has the rows row_start[g] .. row_start[g+1]-1, and each of them sees all pos[g]
+ * positions of the pages pages[g], ahead of its sequence's own (`batch`: positions
+ * 0 .. pos + i).  One softmax runs over both.  Rows of no list see their own positions
+ * only; a list of pos 0 is no prefix.  rows are the batch's; max_rows bounds a list's
+ * rows and max_len its positions.  A list with pos < 0 or above
+ * min(max_len, max_pages * page_size, 2^23), or with more than max_rows rows, has NaN in
+ * all its rows; so has a row that needs a page outside the pool.
+ * Lists end where the caller says, between sequences or inside one; prefix pages are
+ * only read.
+ * The arithmetic is btl_paged_attention's; which of its forms takes a prefix goes by the
+ * rows times heads of its list.  ws: btl_paged_attention_prefix_workspace_bytes (or
+ * NULL: the library's).
+ */
+size_t btl_paged_attention_prefix_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,
+                                                  const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix);
+int btl_paged_attention_prefix(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
+                               const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix, void* out, void* ws,
+                               size_t ws_bytes, void* stream);
+
+/*
+ * What is known of the positions that the sequences of a batch hold (device arrays,
+ * 4-byte aligned; sequence s of the batch has row s of each):
+ * weight [n_seqs, n_kv_heads, ld] f32: the softmax weights that position j has been
+ *   given, over all rows and the query heads of the KV head's group.
+ * token [n_seqs, n_kv_heads, ld], filled [n_seqs], shift [n_seqs] int32: which token
+ *   (its RoPE position) lies at position j: token[s][h][j] for j < filled[s], else
+ *   j + shift[s].  A sequence begins with filled = 0 and shift = 0 (the prefix's length
+ *   where it has one); btl_paged_evict keeps them.  shift is the rope_shift of its rows.
+ * ld: positions of a head, at least min(max_len, max_pages * page_size, 2^23).
+ */
+typedef struct btl_kv_account {
+    float* weight;
+    int32_t* token;
+    int32_t* filled;
+    int32_t* shift;
+    int64_t ld;
+} btl_kv_account_t;
+
+/*
+ * btl_paged_attention (prefix NULL) or btl_paged_attention_prefix, and the weights that
+ * the rows give their sequence's own positions: with p the row's softmax weights, over
+ * the prefix too, weight[s][h][j] becomes the sum of p_j over the sequence's rows and
+ * the query heads of h's group, plus, for j < pos[s], what it was (a position of this
+ * call's rows begins with it).  Only account->weight is used.  Nothing is done for
+ * positions that no row sees, for sequences without rows and for refused ones; a row
+ * that comes back as NaN adds nothing.  Sums are f32, in an order that the sizes fix.
+ * ws: btl_paged_attention_account_workspace_bytes (or NULL: the library's).
+ */
+size_t btl_paged_attention_account_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,
+                                                   const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix);
+int btl_paged_attention_account(const void* q, int dtype, int64_t n_heads, const btl_kv_paged_t* cache,
+                                const btl_paged_batch_t* batch, const btl_paged_batch_t* prefix,
+                                const btl_kv_account_t* account, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Sequences cut down to keep[s] positions, each KV head to its own.  Sequence s holds
+ * len = pos + rows positions (after a step's append and attention; without rows pos).
+ * If len > keep[s], the first keep[s] in this order stay: those of the first tokens
+ * (token < sink[s]) and of the last (token >= len + shift - recent[s]), then the others
+ * by weight descending (NaN below everything, -0 as 0); equals by position ascending.
+ * A position below keep that stays is not touched; of the others below it the n-th takes
+ * the codes, scales, weight and token of the n-th that stays from keep on, both counted
+ * upwards.  (The attention asks for no order of past positions.)
+ * keep, sink, recent: device int32 [n_seqs]; keep < 0: the sequence stays whole; sink and
+ * recent may be NULL (0).  max_keep: the host's bound on what a sequence is cut down to.
+ * account_out (NULL: account itself): weight and token of the positions that are held,
+ * filled = held, shift = shift + len - held; its arrays are account's, or overlap
+ * nothing.  held [n_seqs] int32: min(keep, len), the pos of the sequence's next rows; -1
+ * for a refused sequence (its pos, rows or len out of the batch's bounds, or to be cut down
+ * to more than max_keep), whose pages and account stay as they are.  A moved position whose page is
+ * outside the pool gets NaN scales; one that would go to such a page is lost.
+ * Pages that two sequences share, and in which one has a position below keep that goes,
+ * would be written for both: share prefixes by btl_paged_attention_prefix, or keep
+ * shared first tokens by sink.
+ * ws: btl_paged_evict_workspace_bytes (or NULL: the library's).
+ */
+size_t btl_paged_evict_workspace_bytes(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch);
+int btl_paged_evict(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const btl_kv_account_t* account,
+                    const int32_t* keep, const int32_t* sink, const int32_t* recent, int64_t max_keep,
+                    const btl_kv_account_t* account_out, int32_t* held, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * Next tokens from logits [rows, n] f32, `ld` apart (ld >= n), and given random
