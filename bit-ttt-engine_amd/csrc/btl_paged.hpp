@@ -99,6 +99,13 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v)
     store_y<BF ? YK_BF16 : YK_F32>(p, i, v);
 }
 
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// four neighbours, 4-byte aligned
+struct __attribute__((packed, aligned(4))) Four {
+    uint32_t v[4];
+};
+
 // Rust `f32 as u8`: saturating, NaN -> 0
 __device__ __forceinline__ uint8_t to_u8(float r)
 {

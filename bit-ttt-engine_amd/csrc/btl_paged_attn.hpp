@@ -83,6 +83,14 @@ __device__ __forceinline__ float xor16_max(float v)
     return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
 }
 
+__device__ __forceinline__ uint32_t xor16_max(uint32_t v)
+{
+    u2 p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p.x, p.y);
+    p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(p.x, p.y);
+}
+
 __device__ __forceinline__ float xor16_sum(float v)
 {
     u2 p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -124,6 +132,33 @@ __device__ __forceinline__ void store4(void* p, int64_t i, f4 v)
 // row of a sequence that query row m belongs to: m / group
 __device__ __forceinline__ int row_of(const PagedAttn& a, int m) { return (int)__umulhi(2u * (uint32_t)m, a.group_mul); }
 
+// A row's values, 16 NJ a lane over the four lanes of the row, scaled by a power of two to
+// just under 2^15 and put out in f16 parts: set(part, step, element, value).  Returns the
+// log2 units of one unit of a product with them; NaN if one is not finite.
+template <int NJ, int PARTS, typename F>
+__device__ __forceinline__ float in_parts(const float (*f)[16], float scale_log2, F set)
+{
+    uint32_t am = 0;  // the largest magnitude's bits: what is not finite is above all that is
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) am = max(am, __float_as_uint(f[j][x]) & 0x7FFFFFFFu);
+    am = xor16_max(am);
+    const bool fin = am < 0x7F800000u;
+    const int sh = fin ? 14 - expo(__uint_as_float(am)) : 0;
+    const float up = exp2i(sh);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float y = fin ? __fmul_rn(f[j][x], up) : 0.0f;  // exact
+            const _Float16 hi = (_Float16)y;
+            set(0, 2 * j + (x >> 3), x & 7, hi);
+            if (PARTS == 2) set(1, 2 * j + (x >> 3), x & 7, (_Float16)__fsub_rn(y, (float)hi));
+        }
+    return fin ? __fmul_rn(scale_log2, exp2i(-sh)) : __builtin_nanf("");
+}
+
 // The query rows of a wave: NT tiles of 16, in PARTS f16 parts.
 template <int NJ, int NT, bool BF>
 struct Queries {
@@ -132,7 +167,8 @@ struct Queries {
     h8 v[PARTS][NT][2 * NJ];
 
     // rows m0 .. of a sequence, none past m_last (those repeat it); row0: the output row of m = 0
-    __device__ __forceinline__ void load(const PagedAttn& a, const Seq& q, int64_t row0, int m0, int m_last, int lane)
+    __device__ __forceinline__ void load(const PagedAttn& a, const Seq& q, int64_t row0, int m0, int m_last, int lane,
+                                         float scale)
     {
         const int g = lane >> 4, n = lane & 15, hd = a.c.hd;
 #pragma unroll
@@ -142,8 +178,6 @@ struct Queries {
             const int i = row_of(a, mm);
             const int64_t r = row0 + (int64_t)i * a.nh + (mm - i * a.group);
             float f[NJ][16];
-            float am = 0.0f;
-            bool bad = false;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int d = 16 * (4 * j + g);
@@ -161,32 +195,16 @@ struct Queries {
                         for (int x = 0; x < 4; ++x) w[x] = *(const uint4*)((const float*)a.q + r * hd + d + 4 * x);
                     widen16<XK_F32>(w, f[j]);
                 }
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    am = fmaxf(am, __builtin_fabsf(f[j][x]));
-                    bad |= !(__builtin_fabsf(f[j][x]) < __builtin_inff());
-                }
             }
-            am = xor16_max(bad ? __builtin_inff() : am);
-            const bool fin = am < __builtin_inff();
-            const int sh = fin ? 14 - expo(am) : 0;
-            const float up = exp2i(sh);
-            cq[u] = fin ? __fmul_rn(a.scale_log2, exp2i(-sh)) : __builtin_nanf("");
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const float y = fin ? __fmul_rn(f[j][x], up) : 0.0f;  // exact
-                    const _Float16 hi = (_Float16)y;
-                    v[0][u][2 * j + (x >> 3)][x & 7] = hi;
-                    if (PARTS == 2) v[PARTS - 1][u][2 * j + (x >> 3)][x & 7] = (_Float16)__fsub_rn(y, (float)hi);
-                }
+            cq[u] = in_parts<NJ, PARTS>(f, scale, [&](int p, int x, int e, _Float16 y) { v[p][u][x][e] = y; });
         }
     }
 };
 
 // One column tile's running softmax and output.
-template <int DT>
+// EXACT: the products come with scale_log2 in them and cq is a power of two, so that one
+// fused operation takes a score and the reference apart as exactly as two do.
+template <int DT, bool EXACT = false>
 struct Running {
     float ref, l;  // reference (log2; -inf before the first key), this lane's part of the sum
     int ve;        // exponent of the value scales that the weights are scaled by
@@ -219,7 +237,8 @@ struct Running {
     __device__ __forceinline__ static void score(const f4* sc, float cq, float at, float* y)
     {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) y[x] = __fsub_rn(__fmul_rn(sc[x >> 2][x & 3], cq), at);
+        for (int x = 0; x < 16; ++x)
+            y[x] = EXACT ? __fmaf_rn(sc[x >> 2][x & 3], cq, -at) : __fsub_rn(__fmul_rn(sc[x >> 2][x & 3], cq), at);
     }
 
     // sc: the products of 16 keys with their scales (-inf: not seen); vs: value
@@ -324,14 +343,14 @@ struct Place {
     int h, chunk, tile, s;
 };
 
-// blockIdx.x = h + nkv (chunk + chunks * tile): the head varies fastest.  Workgroups
+// block = h + nkv (chunk + chunks * tile): the head varies fastest.  Workgroups
 // go to the XCDs in turn, so with 8 KV heads the tiles and chunks of one head share
 // an XCD's L2.
-__device__ __forceinline__ Place place_of(const Paged& c, int chunks)
+__device__ __forceinline__ Place place_of(const Paged& c, int chunks, unsigned block)
 {
     Place p;
-    p.h = (int)(blockIdx.x % (unsigned)c.nkv);
-    const unsigned b = blockIdx.x / (unsigned)c.nkv;
+    p.h = (int)(block % (unsigned)c.nkv);
+    const unsigned b = block / (unsigned)c.nkv;
     p.chunk = (int)(b % (unsigned)chunks);
     p.tile = (int)(b / (unsigned)chunks);
     p.s = p.tile;
@@ -344,7 +363,7 @@ constexpr int kPrefix = 1;  // row lists over a prefix: every row sees the `pos`
 constexpr int kOwn = 2;     // as kPlain, beside a prefix or with the rows' maxima and sums put out
 constexpr int kScored = 3;  // as kOwn, with the scores put out too (the token form)
 template <int MODE>
-using PagedArgs = std::conditional_t<MODE == kPlain, PagedAttn, PagedShare>;
+using PagedArgs = std::conditional_t<MODE == kPlain || MODE == kPrefix, PagedAttn, PagedShare>;
 
 template <int MODE>
 __device__ __forceinline__ Seq seq_of(const Paged& c, int s)
@@ -378,6 +397,45 @@ __device__ __forceinline__ bool whole_of(const PagedArgs<MODE>& a, int seen, int
     else return !a.split && seen <= C;
 }
 
+// The kernel's arguments, or some that are one of its arguments' parts, to be read from here
+// on.  All that a kernel asks for is read at its top otherwise: of several forms in one
+// kernel, and of what only its end needs, that is more than the scalar registers hold.
+template <typename T>
+__device__ __forceinline__ const T& from_here(const __attribute__((address_space(4))) T* p)
+{
+    asm volatile("" : "+s"(p));
+    return *(const T*)p;
+}
+template <typename T>
+__device__ __forceinline__ const T& kernel_args()
+{
+    return from_here((const __attribute__((address_space(4))) T*)__builtin_amdgcn_kernarg_segment_ptr());
+}
+template <int MODE>
+__device__ __forceinline__ const PagedArgs<MODE>& at_the_end(const PagedArgs<MODE>& a)
+{
+    if constexpr (MODE == kOwn || MODE == kScored)
+        return from_here((const __attribute__((address_space(4))) PagedArgs<MODE>*)&a);
+    else
+        return a;
+}
+
+// What row t has in the prefix: its chunks, or that its list is refused.
+struct Behind {
+    int parts;
+    bool lost;
+};
+
+__device__ __forceinline__ Behind behind(const PagedShare& a, int t, int lane)
+{
+    const int list = a.g.n_seqs ? find_seq(a.g, t, lane) : -1;
+    if (list < 0 || list >= a.g.n_seqs) return {0, false};
+    const Seq p = seq_of<kPrefix>(a.g, list);
+    if (t < p.a || t >= p.a + p.n) return {0, false};
+    const int C = (int64_t)p.n * a.group > a.gp.lo ? a.gp.tile_c : a.gp.tok_c;
+    return {p.ok ? (p.p0 + C - 1) / C : 0, !p.ok};
+}
+
 // The rows of a refused sequence.
 template <bool BF>
 __device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h, int wave, int waves, int lane)
@@ -400,21 +458,28 @@ __device__ __forceinline__ void fill_nan(const PagedAttn& a, const Seq& q, int h
 // 92 us; with three it spills).  32 sequences of up to 8192 positions, 8 heads of 128,
 // bf16: 353 MB in 75 us, 4.7 TB/s; one of 100001, f32: 211 MB in 35 us, 6.0 TB/s (a
 // sum of 4 GiB reads 6.15 TB/s).
-template <int DT, int NW, bool BF, int MODE = kPlain>
-__global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
+template <int DT, int NW>
+struct TokLds {
+    float (*o)[16][16 * DT + 4];  // [NW]
+    float (*m)[16];               // [NW]
+    float (*l)[16];               // [NW]
+};
+
+template <int DT, int NW, bool BF, int MODE>
+__device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned block, TokLds<DT, NW> lds)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;  // of the queries (bf16 ones are exact in one)
     // Of the weights.  One part in bf16 would save 1.7 us of the batch's 81.4, and one output in
     // twelve would round the other way; in two it is one in 3000.
     constexpr int WP = 2;
-    __shared__ __align__(16) float s_o[NW][16][16 * DT + 4];
-    __shared__ float s_m[NW][16], s_l[NW][16];
+    const auto s_o = lds.o;
+    const auto s_m = lds.m, s_l = lds.l;
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
     const int hd = c.hd, ndt = hd >> 4, C = a.p.tok_c;
-    const Place at = place_of(c, a.p.tok_n);
+    const Place at = place_of(c, a.p.tok_n, block);
     const int key0 = at.chunk * C;
     const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
     // the pages are looked up beside the sequence's size, not after it: what the table holds
@@ -435,9 +500,19 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
     if (key0 >= key1) return;
 
     Queries<NJ, 1, BF> qs;
-    qs.load(a, q, row0, 0, (int)M - 1, lane);
-    Running<DT> r;
+    qs.load(a, q, row0, 0, (int)M - 1, lane, MODE == kPlain ? a.scale_log2 : 1.0f);
+    Running<DT, MODE != kPlain> r;
     r.clear();
+    f4 kept[4];  // the last step's scores
+    int kept_at = -1;
+    auto keep = [&] {
+        if constexpr (MODE == kScored) {
+            if (kept_at < 0 || n >= M) return;
+            float* to = a.scores + (((int64_t)at.s * c.nkv + at.h) * a.score_rows + n) * a.score_ld + kept_at + 16 * g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *(f4*)(to + 4 * t) = kept[t];
+        }
+    };
     for (int kb = key0 + 64 * wave; kb < key1; kb += 64 * NW) {
         // a lane loads a key row of group n / 4, and takes the scales and values of group g
         const int grp = kb >> 4;
@@ -456,12 +531,15 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             ks[t] = *(const f4*)(kscale + 4 * t);
+            if (MODE != kPlain) ks[t] *= a.scale_log2;
             vs[t] = *(const f4*)(vscale + 4 * t);
         }
         uint4 vw[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d) vw[d] = *(const uint4*)(vp + 256 * min(d, ndt - 1));
         const float lost = own < 0 ? __builtin_nanf("") : 0.0f;
+        // behind the loads, which would be waited for with what was stored ahead of them
+        if constexpr (MODE == kScored) keep();
 
         f4 sc[4];
 #pragma unroll
@@ -495,10 +573,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
             r.template weigh_masked<WP>(sc, vs, kb + 16 * g, vis, qs.cq[0], pw);
         }
         if constexpr (MODE == kScored) {
-            float* to = a.scores + (((int64_t)at.s * c.nkv + at.h) * a.score_rows + n) * a.score_ld + kb + 16 * g;
-            if (n < M)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) *(f4*)(to + 4 * t) = sc[t] * qs.cq[0];
+            for (int t = 0; t < 4; ++t) kept[t] = sc[t] * qs.cq[0];
+            kept_at = kb;
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -511,6 +588,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
         }
     }
 
+    keep();
     const float l = xor16_sum(r.l), unit = r.unit();
     if (g == 0) {
         s_m[wave][n] = r.ref;
@@ -519,7 +597,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
 #pragma unroll
     for (int d = 0; d < DT; ++d) *(f4*)&s_o[wave][n][16 * d + 4 * g] = r.o[d] * unit;
     __syncthreads();
-    const bool whole = whole_of<MODE>(a, seen, C);
+    const PagedArgs<MODE>& z = at_the_end<MODE>(a);
+    const bool whole = whole_of<MODE>(z, seen, C);
     for (int x = threadIdx.x; x < (int)M * (hd >> 2); x += 64 * NW) {
         const int m = x / (hd >> 2), d = 4 * (x - m * (hd >> 2));
         float top = s_m[0][m];
@@ -541,16 +620,25 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
         if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
-            store4<BF>(a.out, row * hd + d, v);
-            if constexpr (MODE != kPlain) {
-                if (d == 0 && a.ml) *(float2*)(a.ml + 2 * row) = make_float2(top, sum);
+            store4<BF>(z.out, row * hd + d, v);
+            if constexpr (MODE == kOwn || MODE == kScored) {
+                if (d == 0 && z.ml) *(float2*)(z.ml + 2 * row) = make_float2(top, sum);
             }
         } else {
-            const int64_t part = row * a.parts + part_of<MODE>(a, at.chunk);
-            store4<false>(a.part_o, part * hd + d, v);
-            if (d == 0) *(float2*)(a.part_ml + 2 * part) = make_float2(top, sum);
+            const int64_t part = row * z.parts + part_of<MODE>(z, at.chunk);
+            store4<false>(z.part_o, part * hd + d, v);
+            if (d == 0) *(float2*)(z.part_ml + 2 * part) = make_float2(top, sum);
         }
     }
+}
+
+template <int DT, int NW, bool BF, int MODE = kPlain>
+__global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
+{
+    __shared__ __align__(16) float s_o[NW][16][16 * DT + 4];
+    __shared__ float s_m[NW][16], s_l[NW][16];
+    if constexpr (MODE == kPlain) paged_tok<DT, NW, BF, MODE>(a, blockIdx.x, {s_o, s_m, s_l});
+    else paged_tok<DT, NW, BF, MODE>(kernel_args<PagedArgs<MODE>>(), blockIdx.x, {s_o, s_m, s_l});
 }
 
 // The tile form: 64 NT query rows of a sequence, 16 NT a wave, every key to all four
@@ -567,8 +655,16 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
 // Tried: each wave widening for itself 267 us; 48 or 64 rows a wave 280 and 223 (one
 // wave a SIMD); without reading operands ahead 124 to 115; a branch-free step 117; wave
 // priorities 129.
-template <int DT, int NT, bool BF, int MODE = kPlain>
-__global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
+template <int DT>
+struct TileLds {
+    h8 (*k)[4][2 * ((DT + 3) / 4)][64];  // [2]
+    h8 (*v)[DT][2][64];                  // [2]
+    float (*ks)[64], (*vs)[64];          // [2]
+    float* top;                          // [2]
+};
+
+template <int DT, int NT, bool BF, int MODE>
+__device__ __forceinline__ void paged_tile(const PagedArgs<MODE>& a, unsigned block, TileLds<DT> lds)
 {
     constexpr int NJ = (DT + 3) / 4;
     // Of the queries and of the weights.  In bf16 a query is exact in one part, and weights are
@@ -577,15 +673,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
     // is the output's rounding alone, in two parts; it takes 114 us so and 137 in two.
     constexpr int PARTS = BF ? 1 : 2;
     constexpr int MT = 64 * NT;
-    __shared__ __align__(16) h8 s_k[2][4][2 * NJ][64];
-    __shared__ __align__(16) h8 s_v[2][DT][2][64];
-    __shared__ __align__(16) float s_ks[2][64], s_vs[2][64];
-    __shared__ float s_top[2];
+    const auto s_k = lds.k;
+    const auto s_v = lds.v;
+    const auto s_ks = lds.ks, s_vs = lds.vs;
+    const auto s_top = lds.top;
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
     const int hd = c.hd, ndt = hd >> 4, C = a.p.tile_c;
-    Place at = place_of(c, a.p.tile_n);
+    Place at = place_of(c, a.p.tile_n, block);
 
     // the sequence that the tile belongs to: sequences of more than `lo` query rows have
     // one for every MT of them.  A refused one has one for its NaN: the launch has tiles for
@@ -637,7 +733,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
             kw[j] = *(const uint4*)(kp + (koff + (ko < hd ? ko : 0)));
             vw[j] = *(const uint4*)(vp + (voff + 256 * min(wave + 4 * j, ndt - 1)));
         }
-        scale = (wave & 1 ? c.vs : c.ks)[16 * (int64_t)at_v + n];
+        scale = (wave & 1 ? +c.vs : +c.ks)[16 * (int64_t)at_v + n];
         lost = own < 0;
     };
     auto put = [&](int b) {
@@ -653,7 +749,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
         // a scale that is not finite is NaN for whoever sees its key: an infinite one times a
         // negative product would be -inf, which is a key that no row sees
         const bool bad = !(__builtin_fabsf(scale) < __builtin_inff());
-        if (wave == 0) s_ks[b][lane] = lost || bad ? __builtin_nanf("") : scale;
+        if (wave == 0) s_ks[b][lane] = lost || bad ? __builtin_nanf("") : (MODE == kPlain ? scale : __fmul_rn(scale, a.scale_log2));
         if (wave == 1) {
             s_vs[b][lane] = bad ? __builtin_nanf("") : scale;
             const uint32_t m = __float_as_uint(scale) & 0x7FFFFFFFu;
@@ -662,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
         }
     };
 
-    Running<DT> r[NT];
+    Running<DT, MODE != kPlain> r[NT];
     Queries<NJ, NT, BF> qs;
     auto step = [&](int kb, int b, auto masked) {
         if (kb + 64 < key1) fetch(kb + 64);
@@ -742,7 +838,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
     };
 
     fetch(key0);
-    qs.load(a, q, row0, m_wave, m_last, lane);
+    qs.load(a, q, row0, m_wave, m_last, lane, MODE == kPlain ? a.scale_log2 : 1.0f);
 #pragma unroll
     for (int u = 0; u < NT; ++u) r[u].clear();
     put(0);
@@ -752,7 +848,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
     for (; kb + 64 <= min(key1, vis_least); kb += 64, b ^= 1) step(kb, b, False{});
     for (; kb < key1; kb += 64, b ^= 1) step(kb, b, True{});
 
-    const bool whole = whole_of<MODE>(a, sees<MODE>(q, q.n - 1), C);
+    const PagedArgs<MODE>& z = at_the_end<MODE>(a);
+    const bool whole = whole_of<MODE>(z, sees<MODE>(q, q.n - 1), C);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
         const float l = xor16_sum(r[u].l), unit = r[u].unit();
@@ -760,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
         asm("" : "+v"(m));
         const int i = row_of(a, m);
         if (m > m_last) continue;
-        const int64_t row = row0 + (int64_t)i * a.nh + (m - i * a.group), part = row * a.parts + part_of<MODE>(a, at.chunk);
+        const int64_t row = row0 + (int64_t)i * a.nh + (m - i * a.group), part = row * z.parts + part_of<MODE>(z, at.chunk);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (d < ndt) {
@@ -768,18 +865,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
                 if (whole) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], l);
-                    store4<BF>(a.out, row * hd + 16 * d + 4 * g, v);
+                    store4<BF>(z.out, row * hd + 16 * d + 4 * g, v);
                 } else {
-                    store4<false>(a.part_o, part * hd + 16 * d + 4 * g, v);
+                    store4<false>(z.part_o, part * hd + 16 * d + 4 * g, v);
                 }
             }
         if (!whole && g == 0)
-            *(float2*)(a.part_ml + 2 * part) = make_float2(r[u].ref == -__builtin_inff() ? 0.0f : r[u].ref, l);
-        if constexpr (MODE != kPlain) {
-            if (whole && g == 0 && a.ml)
-                *(float2*)(a.ml + 2 * row) = make_float2(r[u].ref == -__builtin_inff() ? 0.0f : r[u].ref, l);
+            *(float2*)(z.part_ml + 2 * part) = make_float2(r[u].ref == -__builtin_inff() ? 0.0f : r[u].ref, l);
+        if constexpr (MODE == kOwn) {
+            if (whole && g == 0 && z.ml)
+                *(float2*)(z.ml + 2 * row) = make_float2(r[u].ref == -__builtin_inff() ? 0.0f : r[u].ref, l);
         }
     }
+}
+
+template <int DT, int NT, bool BF, int MODE = kPlain>
+__global__ __launch_bounds__(256, 2) void k_paged_tile(PagedArgs<MODE> a)
+{
+    __shared__ __align__(16) h8 s_k[2][4][2 * ((DT + 3) / 4)][64];
+    __shared__ __align__(16) h8 s_v[2][DT][2][64];
+    __shared__ __align__(16) float s_ks[2][64], s_vs[2][64];
+    __shared__ float s_top[2];
+    if constexpr (MODE == kPlain) paged_tile<DT, NT, BF, MODE>(a, blockIdx.x, {s_k, s_v, s_ks, s_vs, s_top});
+    else paged_tile<DT, NT, BF, MODE>(kernel_args<PagedArgs<MODE>>(), blockIdx.x, {s_k, s_v, s_ks, s_vs, s_top});
 }
 
 // ---------------------------------------------------------------------------
@@ -811,15 +919,9 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs<MODE> a)
     int np = 0;                   // of them of the prefix
     bool lost = false;
     if constexpr (MODE != kPlain) {
-        const int list = a.g.n_seqs ? find_seq(a.g, t, lane) : -1;
-        if (list >= 0 && list < a.g.n_seqs) {
-            const Seq p = seq_of<kPrefix>(a.g, list);
-            if (t >= p.a && t < p.a + p.n) {
-                const int PC = (int64_t)p.n * a.group > a.gp.lo ? a.gp.tile_c : a.gp.tok_c;
-                lost = !p.ok;
-                np = p.ok ? (p.p0 + PC - 1) / PC : 0;
-            }
-        }
+        const Behind b = behind(a, t, lane);
+        np = b.parts;
+        lost = b.lost;
         nc += np;
     }
     const int64_t r = (int64_t)t * a.nh + head, at = r * a.parts;

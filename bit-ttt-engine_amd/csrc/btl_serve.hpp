@@ -96,9 +96,8 @@ struct PagedShare : PagedAttn {
     int splits;     // shares of the rows of a sequence that is too long for the token form's scores
     int scored;     // sequences of the token form have scores
 };
-AttnPlan plan_paged_prefix(int64_t n_heads, const Paged& g, bool bf);
-// fills a's split of the accounting; false: too large for one launch
-bool plan_paged_account(int64_t n_heads, PagedShare& a);
+// fills in a's split of the work; false: too large for one launch
+bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account);
 hipError_t launch_paged_share(const PagedShare& a, hipStream_t st);
 
 struct PagedEvict {

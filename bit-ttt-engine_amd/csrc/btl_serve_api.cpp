@@ -132,19 +132,6 @@ ShareWs share_ws(const btl::PagedShare& a, int64_t n_heads, bool account)
     return w;
 }
 
-// The plan of such a call; false: too large for its launches.
-bool plan_share(btl::PagedShare& a, int64_t n_heads, bool bf, bool account)
-{
-    a.p = btl::plan_paged_attention(n_heads, a.c, bf);
-    a.split = a.g.n_seqs > 0;
-    if (a.split) a.gp = btl::plan_paged_prefix(n_heads, a.g, bf);
-    a.own0 = a.split ? a.gp.parts() : 0;
-    a.parts = a.own0 + a.p.parts();
-    a.splits = 1;
-    const bool fits = btl::paged_attention_fits(a.c, a.p) && (!a.split || btl::paged_attention_fits(a.g, a.gp));
-    return (!account || btl::plan_paged_account(n_heads, a)) && fits;
-}
-
 size_t share_bytes(int64_t n_heads, const btl_kv_paged_t* cache, const btl_paged_batch_t* batch,
                    const btl_paged_batch_t* prefix, bool account)
 {
@@ -153,7 +140,7 @@ size_t share_bytes(int64_t n_heads, const btl_kv_paged_t* cache, const btl_paged
     if (prefix && check_prefix(cache, batch, prefix, &a.g)) return 0;
     size_t most = 0;
     for (int bf = 0; bf < 2; ++bf) {
-        if (!plan_share(a, n_heads, bf, account)) return 0;
+        if (!btl::plan_paged_share(n_heads, a, bf, account)) return 0;
         most = std::max(most, share_ws(a, n_heads, account).total);
     }
     return most;
@@ -296,7 +283,7 @@ static int attention_share(const void* q, int dtype, int64_t n_heads, const btl_
     if (account && (account->ld < a.c.cap || account->ld > ((int64_t)1 << 32)))
         return failf(BTL_ERR_SHAPE, "an account of %lld positions a head, for sequences of up to %d", (long long)account->ld, a.c.cap);
     if (a.c.rows == 0 || a.c.n_seqs == 0) return BTL_OK;
-    if (!plan_share(a, n_heads, dtype == BTL_BF16, account)) return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
+    if (!btl::plan_paged_share(n_heads, a, dtype == BTL_BF16, account)) return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
     if ((rc = check_pointers(cache, batch, &a.c)) || (a.split && (rc = check_pointers(cache, prefix, &a.g)))) return rc;
     if (!q || !out || (account && !account->weight)) return fail_msg(BTL_ERR_LAYOUT, "null pointer");
     if (!aligned16(q) || !aligned16(out)) return fail_msg(BTL_ERR_LAYOUT, "q and out must be 16-byte aligned");

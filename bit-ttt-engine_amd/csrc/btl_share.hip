@@ -19,6 +19,101 @@
 namespace btl {
 
 // ---------------------------------------------------------------------------
+// k_share
+// ---------------------------------------------------------------------------
+// The attention of a call in one launch, the forms of btl_paged_attn.hpp side by side:
+// lists of rows over the prefix (token form, or tile form), then sequences over their own
+// positions (tile form, token form).  The tiles are bound by the vector unit and the
+// tokens by the cache's bytes, and two workgroups a CU is what either's registers allow.
+// Tiles of 128 rows, which fill all of them, have launches of their own.
+namespace {
+
+struct ShareArgs {
+    PagedAttn p;   // the prefix's
+    PagedShare a;  // the sequences'
+};
+
+}  // namespace
+
+template <int DT, bool BF, bool SCORED>
+__global__ __launch_bounds__(256, 2) void k_share(ShareArgs, unsigned prefix_tok, unsigned prefix_tile,
+                                                      unsigned own_tile)
+{
+    constexpr int NW = 4, kK = 2 * 4 * (2 * ((DT + 3) / 4)) * 64, kV = 2 * DT * 2 * 64;  // fragments of k and v
+    constexpr int kO = NW * 16 * (16 * DT + 4);
+    constexpr int kTile = 16 * (kK + kV) + 4 * (2 * 64 + 2 * 64 + 2), kTok = 4 * (kO + 2 * NW * 16);
+    __shared__ __align__(16) uint8_t s[kTile > kTok ? kTile : kTok];
+    uint8_t* const sf = s + 16 * (kK + kV);
+    const TileLds<DT> tile = {(h8(*)[4][2 * ((DT + 3) / 4)][64])s, (h8(*)[DT][2][64])(s + 16 * kK), (float(*)[64])sf,
+                              (float(*)[64])(sf + 512), (float*)(sf + 1024)};
+    const TokLds<DT, NW> tok = {(float(*)[16][16 * DT + 4])s, (float(*)[16])(s + 4 * kO), (float(*)[16])(s + 4 * kO + 64 * NW)};
+    unsigned block = blockIdx.x;
+    if (block < prefix_tok) return paged_tok<DT, NW, BF, kPrefix>(kernel_args<ShareArgs>().p, block, tok);
+    block -= prefix_tok;
+    if (block < prefix_tile) return paged_tile<DT, 1, BF, kPrefix>(kernel_args<ShareArgs>().p, block, tile);
+    block -= prefix_tile;
+    if (block < own_tile) return paged_tile<DT, 1, BF, kOwn>(kernel_args<ShareArgs>().a, block, tile);
+    paged_tok<DT, NW, BF, SCORED ? kScored : kOwn>(kernel_args<ShareArgs>().a, block - own_tile, tok);
+}
+
+// ---------------------------------------------------------------------------
+// k_share_merge
+// ---------------------------------------------------------------------------
+// k_paged_merge for rows of at most U parts: half a wave a (row, head), four values a
+// lane, every lane holding all the parts' maxima; N heads one after the other, so that
+// what is known of the row serves them all.  grid (rows, ceil(nh / (8 N))), block 256.
+template <int N, int U, bool BF>
+__global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
+{
+    const Paged& c = a.c;
+    const int t = blockIdx.x, lane = threadIdx.x & 63, d = 4 * (lane & 31), hd = c.hd;
+    const int s = find_seq(c, t, lane);
+    if (s < 0 || s >= c.n_seqs) return;
+    const Seq q = seq_at(c, s);
+    const int i = t - q.a;
+    if (i < 0 || i >= q.n || !q.ok) return;
+    const int C = (int64_t)q.n * a.group > a.p.lo ? a.p.tile_c : a.p.tok_c;
+    if (whole_of<kOwn>(a, q.p0 + q.n, C)) return;  // written by its one chunk
+    const Behind p = behind(a, t, lane);
+    const int nc = p.parts + (q.p0 + i) / C + 1;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        const int head = (int)blockIdx.y * 8 * N + 8 * x + (int)(threadIdx.x >> 5);
+        if (head >= a.nh) return;
+        const int64_t r = (int64_t)t * a.nh + head, at = r * a.parts;
+        float2 ml[U];
+        f4 o[U];
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+            if (y < nc) {
+                const int64_t part = at + (y < p.parts ? y : a.own0 - p.parts + y);
+                ml[y] = *(const float2*)(a.part_ml + 2 * part);
+                o[y] = *(const f4*)(a.part_o + part * hd + (d < hd ? d : 0));
+            }
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+            if (y < nc) top = fmaxf(top, ml[y].x);
+        f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+            if (y < nc) {
+                const float b = __builtin_amdgcn_exp2f(__fsub_rn(ml[y].x, top));
+                sum = __fmaf_rn(b, ml[y].y, sum);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, o[y][e], v[e]);
+            }
+        if (p.lost) sum = __builtin_nanf("");
+        if (a.ml && d == 0) *(float2*)(a.ml + 2 * r) = make_float2(top, sum);
+        if (d < hd) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
+            store4<BF>(a.out, r * hd + d, v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
 // k_account_tile
 // ---------------------------------------------------------------------------
 // weight[j] = sum over the rows that see j of 2^(s - m) / l, with the rows' m and l from
@@ -34,7 +129,6 @@ namespace btl {
 namespace {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // Codes times this are what a bf16 query meets: 2^128 of a query times 128 values of
 // 2^7 would pass the largest f32.
@@ -73,12 +167,14 @@ __device__ __forceinline__ void put_weight(const PagedShare& a, const Seq& q, in
 }  // namespace
 
 template <int DT, bool BF>
-__global__ __launch_bounds__(256, 2) void k_account_tile(PagedShare a)
+__global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;
     __shared__ __align__(16) u4 s_q[2][4][PARTS * 2 * NJ][64];
-    __shared__ float4 s_r[2][4][16];  // a row's unit of the product, maximum and 1 / sum
+    __shared__ float2 s_r[2][4][16];           // a row's maximum and 1 / sum
+    __shared__ float s_unit[2][4][BF ? 1 : 16];  // the unit of its products
+    __shared__ int s_bad[2][4];       // a tile has rows that came back as NaN
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15, hd = c.hd, ndt = hd >> 4;
@@ -118,54 +214,70 @@ __global__ __launch_bounds__(256, 2) void k_account_tile(PagedShare a)
         }
     f4 ks[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) ks[t] = *(const f4*)(c.ks + 16 * (int64_t)max(own, 0) + 4 * t);
+    for (int t = 0; t < 4; ++t) ks[t] = *(const f4*)(c.ks + 16 * (int64_t)max(own, 0) + 4 * t) * a.scale_log2;
 
     // the rows from the first that sees the block's first key on, this workgroup's share of them
     const int first = max(0, key0 - q.p0) * a.group & ~15;
     const int steps = ((int)M - first + 63) / 64;
     const int step0 = (int)((int64_t)steps * share / a.splits), step1 = (int)((int64_t)steps * (share + 1) / a.splits);
     const int64_t row0 = (int64_t)q.a * a.nh + h * a.group;
-    auto put = [&](int step, int b) {
-        const int m = first + 64 * step + 16 * wave + n, mm = min(m, (int)M - 1);
-        const int i = row_of(a, mm);
+    // this wave's tile of a step: asked for ahead of the work on the step before it
+    constexpr int PER = BF ? 2 : 4;  // 16-byte pieces of 16 values
+    u4 raw[PER * NJ];
+    float2 ml;
+    auto fetch = [&](int step) {
+        const int mm = min(first + 64 * step + 16 * wave + n, (int)M - 1), i = row_of(a, mm);
         const int64_t row = row0 + (int64_t)i * a.nh + (mm - i * a.group);
-        const float2 ml = *(const float2*)(a.ml + 2 * row);
-        float unit;
+        ml = *(const float2*)(a.ml + 2 * row);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int d = 16 * (4 * j + g);
+            const u4* p = (const u4*)((const uint8_t*)a.q + (row * hd + (d < hd ? d : 0)) * (BF ? 2 : 4));
+#pragma unroll
+            for (int x = 0; x < PER; ++x) raw[PER * j + x] = p[x];
+        }
+    };
+    auto put = [&](int step, int b) {
         if constexpr (BF) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int d = 16 * (4 * j + g);
-                const u4* p = (const u4*)((const uint16_t*)a.q + row * hd + (d < hd ? d : 0));
-                const u4 w0 = p[0], w1 = p[1], none = {0, 0, 0, 0};
-                s_q[b][wave][2 * j][lane] = d < hd ? w0 : none;
-                s_q[b][wave][2 * j + 1][lane] = d < hd ? w1 : none;
-            }
-            unit = a.scale_log2 / kCodeDown;
+            for (int x = 0; x < 2 * NJ; ++x) s_q[b][wave][x][lane] = 16 * (4 * (x >> 1) + g) < hd ? raw[x] : u4{0, 0, 0, 0};
         } else {
-            Queries<NJ, 1, false> qs;
-            qs.load(a, q, row0, first + 64 * step + 16 * wave, (int)M - 1, lane);
+            // in two f16 parts, as the attention takes them
+            float f[NJ][16];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    f[j][x] = 16 * (4 * j + g) < hd ? __uint_as_float(raw[4 * j + (x >> 2)][x & 3]) : 0.0f;
+            h8 parts[2][2 * NJ];
+            const float unit = in_parts<NJ, 2>(f, 1.0f, [&](int p, int x, int e, _Float16 y) { parts[p][x][e] = y; });
+            if (g == 0) s_unit[b][wave][n] = unit;
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int j = 0; j < 2 * NJ; ++j)
-                    s_q[b][wave][2 * NJ * p + j][lane] = __builtin_bit_cast(u4, qs.v[p][0][j]);
-            unit = qs.cq[0];
+                for (int j = 0; j < 2 * NJ; ++j) s_q[b][wave][2 * NJ * p + j][lane] = __builtin_bit_cast(u4, parts[p][j]);
         }
         // a row that came back as NaN adds nothing (-1 says so), nor does one behind the last (0)
-        const bool good = ml.y > 0.0f && ml.y < __builtin_inff();
-        const float part = !good ? -1.0f : (m < M ? __fdiv_rn(1.0f, ml.y) : 0.0f);
-        if (g == 0) s_r[b][wave][n] = make_float4(unit, ml.x, part, 0.0f);
+        const bool good = ml.y > 0.0f && ml.y < __builtin_inff(), real = first + 64 * step + 16 * wave + n < M;
+        const float part = !good ? -1.0f : (real ? __fdiv_rn(1.0f, ml.y) : 0.0f);
+        if (g == 0) s_r[b][wave][n] = make_float2(ml.x, part);
+        const bool some = __any(!good);
+        if (lane == 0) s_bad[b][wave] = some;
     };
 
     float sum[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) sum[x] = 0.0f;
-    if (step0 < step1) put(step0, 0);
+    if (step0 < step1) {
+        fetch(step0);
+        put(step0, 0);
+    }
     __syncthreads();
     for (int step = step0, b = 0; step < step1; ++step, b ^= 1) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            f4 sc[4];
+        if (step + 1 < step1) fetch(step + 1);
+        // the scores of tile u, less the row's largest, in the roundings of the attention
+        auto scores = [&](int u, float top, f4* sc) {
+            const float unit = BF ? 1.0f / kCodeDown : s_unit[b][u][BF ? 0 : n];
 #pragma unroll
             for (int t = 0; t < 4; ++t) sc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -176,25 +288,36 @@ __global__ __launch_bounds__(256, 2) void k_account_tile(PagedShare a)
 #pragma unroll
                     for (int t = 0; t < 4; ++t) sc[t] = product<BF>(k[t][j], x, sc[t]);
                 }
-            const float4 r = s_r[b][u][n];
-            // the score in the roundings of the attention, whose largest is r.y
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    sc[t][e] = __fsub_rn(__fmul_rn(__fmul_rn(sc[t][e], ks[t][e]), r.x), r.y);
-            const int m = first + 64 * step + 16 * u;
-            const bool all = kb + 64 <= q.p0 + row_of(a, m) + 1;  // the tile's first row sees every key
-            if (!all || __any(r.z < 0.0f)) {
-                const int vis = q.p0 + row_of(a, min(m + n, (int)M - 1)) + 1 - kb - 16 * g;
+                for (int e = 0; e < 4; ++e) sc[t][e] = __fmaf_rn(__fmul_rn(sc[t][e], ks[t][e]), unit, -top);
+        };
+        const int bad = __builtin_amdgcn_readfirstlane(s_bad[b][0] | s_bad[b][1] | s_bad[b][2] | s_bad[b][3]);
+        const int m0 = first + 64 * step;
+        const bool all = kb + 64 <= q.p0 + row_of(a, m0) + 1;  // the step's first row sees every key
+        if (all && !bad) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f4 sc[4];
+                const float2 r = s_r[b][u][n];
+                scores(u, r.x, sc);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) sum[x] = __fmaf_rn(__builtin_amdgcn_exp2f(sc[x >> 2][x & 3]), r.y, sum[x]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f4 sc[4];
+                const float2 r = s_r[b][u][n];
+                scores(u, r.x, sc);
+                const int vis = q.p0 + row_of(a, min(m0 + 16 * u + n, (int)M - 1)) + 1 - kb - 16 * g;
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float p = __fmul_rn(__builtin_amdgcn_exp2f(sc[x >> 2][x & 3]), r.z);
-                    sum[x] = __fadd_rn(sum[x], x < vis && r.z > 0.0f ? p : 0.0f);
+                    const float p = __fmul_rn(__builtin_amdgcn_exp2f(sc[x >> 2][x & 3]), r.y);
+                    sum[x] = __fadd_rn(sum[x], x < vis && r.y > 0.0f ? p : 0.0f);
                 }
-            } else {
-#pragma unroll
-                for (int x = 0; x < 16; ++x) sum[x] = __fmaf_rn(__builtin_amdgcn_exp2f(sc[x >> 2][x & 3]), r.z, sum[x]);
+                __builtin_amdgcn_sched_barrier(0);  // one tile's temporaries at a time
             }
         }
         if (step + 1 < step1) put(step + 1, b ^ 1);
@@ -218,103 +341,179 @@ __global__ __launch_bounds__(256, 2) void k_account_tile(PagedShare a)
 // ---------------------------------------------------------------------------
 // k_account_sum
 // ---------------------------------------------------------------------------
-// A position a thread: the weights from the scores of at most 16 rows, or the sum of the
-// shares of k_account_tile, in order.  grid nkv * ceil(cap / 256) * n_seqs, block 256.
+// Four positions a thread: the weights from the scores of at most 16 rows, or the sum of
+// the shares of k_account_tile, in order.  grid nkv * ceil(cap / 1024) * n_seqs, block 256.
 __global__ __launch_bounds__(256) void k_account_sum(PagedShare a)
 {
     const Paged& c = a.c;
     const int h = (int)(blockIdx.x % (unsigned)c.nkv);
-    const unsigned at = blockIdx.x / (unsigned)c.nkv, blocks = (unsigned)(c.cap + 255) / 256;
-    const int key = 256 * (int)(at % blocks) + threadIdx.x, s = (int)(at / blocks);
+    const unsigned at = blockIdx.x / (unsigned)c.nkv, blocks = (unsigned)(c.cap + 1023) / 1024;
+    const int key = 4 * (256 * (int)(at % blocks) + threadIdx.x), s = (int)(at / blocks);
     const Seq q = seq_at(c, s);
-    const int64_t M = (int64_t)q.n * a.group;
-    if (M == 0 || !q.ok || key >= q.p0 + q.n) return;
-    float w = 0.0f;
+    const int64_t M = (int64_t)q.n * a.group, head = (int64_t)s * c.nkv + h;
+    const int seen = q.p0 + q.n;
+    if (M == 0 || !q.ok || key >= seen) return;
+    float* to = a.weight + head * a.ld + key;
+    const bool four = key + 4 <= a.ld;
+    Four old = {};  // asked for beside the scores
+    if (four) old = *(const Four*)to;
+    f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
     if (has_scores(a, M)) {
-        const float* sc = a.scores + ((int64_t)s * c.nkv + h) * a.score_rows * a.score_ld + key;
+        const float* sc = a.scores + head * a.score_rows * a.score_ld + key;
         const int64_t row0 = (int64_t)q.a * a.nh + h * a.group;
-        for (int m = 0; m < (int)M; ++m) {
-            const int i = row_of(a, m);
-            const float2 ml = *(const float2*)(a.ml + 2 * (row0 + (int64_t)i * a.nh + (m - i * a.group)));
-            const bool good = ml.y > 0.0f && ml.y < __builtin_inff();  // else it came back as NaN and adds nothing
-            const float p = __fdiv_rn(__builtin_amdgcn_exp2f(__fsub_rn(sc[(int64_t)m * a.score_ld], ml.x)), ml.y);
-            w = __fadd_rn(w, good ? p : 0.0f);
+        constexpr int U = 4;
+        for (int m0 = 0; m0 < (int)M; m0 += U) {
+            f4 y[U];
+            float2 ml[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int m = min(m0 + u, (int)M - 1), i = row_of(a, m);
+                y[u] = *(const f4*)(sc + (int64_t)m * a.score_ld);
+                ml[u] = *(const float2*)(a.ml + 2 * (row0 + (int64_t)i * a.nh + (m - i * a.group)));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                // a row that came back as NaN adds nothing
+                const bool good = m0 + u < (int)M && ml[u].y > 0.0f && ml[u].y < __builtin_inff();
+                const float part = good ? __fdiv_rn(1.0f, ml[u].y) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__fsub_rn(y[u][e], ml[u].x));
+                    w[e] = good ? __fmaf_rn(p, part, w[e]) : w[e];
+                }
+            }
         }
     } else {
         if (a.splits == 1) return;  // put out where they were summed
-        for (int x = 0; x < a.splits; ++x)
-            w = __fadd_rn(w, a.sums[(((int64_t)x * c.n_seqs + s) * c.nkv + h) * a.score_ld + key]);
+        for (int x = 0; x < a.splits; ++x) {
+            const f4 y = *(const f4*)(a.sums + ((int64_t)x * c.n_seqs * c.nkv + head) * a.score_ld + key);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __fadd_rn(w[e], y[e]);
+        }
     }
-    put_weight(a, q, s, h, key, w);
+    if (four && key + 4 <= seen) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            old.v[e] = key + e < q.p0 ? __float_as_uint(__fadd_rn(__uint_as_float(old.v[e]), w[e])) : __float_as_uint(w[e]);
+        *(Four*)to = old;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (key + e < seen) put_weight(a, q, s, h, key + e, w[e]);
 }
 
-AttnPlan plan_paged_prefix(int64_t n_heads, const Paged& g, bool bf) { return plan_paged_attention(n_heads, g, bf); }
-
-bool plan_paged_account(int64_t n_heads, PagedShare& a)
+bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
 {
-    const Paged& c = a.c;
-    const int64_t group = n_heads / c.nkv, blocks = (c.cap + 255) / 256;
-    a.score_rows = (int)std::min<int64_t>(kTokRows, (int64_t)c.max_rows * group);
-    a.score_ld = (c.cap + 63) / 64 * 64;
+    auto up = [](int64_t v, int64_t m) { return (v + m - 1) / m * m; };
+    const Paged &c = a.c, &g = a.g;
+    const int64_t group = n_heads / c.nkv, heads = (int64_t)c.n_seqs * c.nkv, longest = std::max(c.cap, 1);
+    a.split = g.n_seqs > 0;
+    AttnPlan& p = a.p;
+    p = plan_paged_attention(n_heads, c, bf);
     // scores of a batch whose bounds are far above its lengths would be a large workspace:
     // above 1 GiB the keys are gone through again
-    a.scored = a.p.lo > 0 && (int64_t)c.n_seqs * c.nkv * a.score_rows * a.score_ld <= ((int64_t)1 << 28);
-    const bool tiles = a.p.lo != INT_MAX || !a.scored;
-    // sequences that k_account_tile goes through, at most
+    a.scored = account && p.lo > 0 &&
+               heads * std::min<int64_t>(kTokRows, c.max_rows * group) * up(longest, 64) <= ((int64_t)1 << 28);
+    // Sequences of at most 512 positions, their scores kept and nothing beside them, in one
+    // launch of eight waves.  Else four waves.  Beside a prefix, whose tiles fill the chip as
+    // well, chunks for 512 workgroups: 64 sequences of up to 700 52.5 us where btl_serve.hip's
+    // rule takes 59.8, 32 of up to 4000 75.4 and 83.6 (with 256: 52.8 and 80.2; 1024: 60.3 and 77.3).
+    const bool apart = p.tok_w == 8 && p.tok_n && a.scored && !a.split && !p.tile_n;
+    if (!apart) p.tok_w = 4;
+    if (!apart && p.tok_n) {
+        const int64_t want = a.split || heads <= 64 ? 512 : 4096;
+        p.tok_c = (int)std::min(up(longest, 256), up(longest * heads / want + 1, 256));
+        p.tok_n = (int)((longest + p.tok_c - 1) / p.tok_c);
+    }
+    a.own0 = 0;
+    a.gp = AttnPlan{};
+    if (a.split) {
+        // One form for all lists: tokens where every list is that short.
+        AttnPlan& r = a.gp;
+        const int64_t far = std::max(g.cap, 1), all = up(far, 256);
+        r.tok_w = 4;
+        r.lo = g.max_rows * group <= kTokRows ? INT_MAX : 0;
+        r.tile_rows = p.tile_rows;
+        r.tok_c = r.tile_c = (int)all;
+        if (r.lo) {
+            r.tok_c = (int)std::min(all, up(far * g.n_seqs * g.nkv / 512 + 1, 256));
+            r.tok_n = (int)((far + r.tok_c - 1) / r.tok_c);
+        } else {
+            // Chunks so that there are about 256 workgroups, one a CU beside the sequences' own (64
+            // tokens behind 8192 positions: 42.4 us, 48.5 with 192, 48.9 with 512, 58.9 with 1024);
+            // of many tiles 2048, as long as a chunk has 2048 positions (12 questions behind 16001:
+            // 406 us, 433 with 1024, 626 with one chunk).
+            const int64_t per = ((int64_t)g.max_rows * group + r.tile_rows - 1) / r.tile_rows;
+            r.tiles = (int)std::min<int64_t>((int64_t)g.n_seqs * per, (int64_t)g.rows * group / r.tile_rows + g.n_seqs);
+            const int64_t base = (int64_t)r.tiles * g.nkv;
+            const int64_t n = std::max<int64_t>({1, (256 + base / 2) / base, std::min(far / 2048, (2048 + base - 1) / base)});
+            r.tile_c = (int)std::max<int64_t>(256, up((far + n - 1) / n, 64));
+            r.tile_n = (int)((far + r.tile_c - 1) / r.tile_c);
+        }
+        a.own0 = r.parts();
+    }
+    a.parts = a.own0 + p.parts();
+    a.splits = 1;
+    const int64_t threads = ((int64_t)1 << 32) - 1;  // of a grid
+    const int64_t blocks = (int64_t)c.nkv * p.tok_n * c.n_seqs + (int64_t)c.nkv * p.tile_n * p.tiles +
+                           (int64_t)g.nkv * a.gp.tok_n * g.n_seqs + (int64_t)g.nkv * a.gp.tile_n * a.gp.tiles;
+    if (blocks * 64 * p.tok_w > threads) return false;
+    if (!account) return true;
+
+    a.score_rows = (int)std::min<int64_t>(kTokRows, (int64_t)c.max_rows * group);
+    a.score_ld = (int)up(c.cap, 64);
+    // k_account_tile's rows in shares of at least 256, for some 2048 workgroups: of the sequences
+    // that the bounds allow to be long, few may be (two of 14: 39.8 us, 49.7 for 768).
+    const bool tiles = p.lo != INT_MAX || !a.scored;
     const int64_t seqs = !tiles ? 0 : (a.scored ? std::min<int64_t>(c.n_seqs, (int64_t)c.rows * group / 16 + 1) : c.n_seqs);
-    const int64_t want = 768, have = std::max<int64_t>(1, seqs * c.nkv * blocks);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / have, 16, (int64_t)c.max_rows * group / 64}));
-    const int64_t threads = ((int64_t)1 << 32) - 1;
-    return (int64_t)c.nkv * blocks * c.n_seqs * 256 * (tiles ? a.splits : 1) <= threads;
+    const int64_t keys = (c.cap + 255) / 256, have = std::max<int64_t>(1, seqs * c.nkv * keys);
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2048 / have, 16, (int64_t)c.max_rows * group / 256}));
+    return heads * keys * 256 * (tiles ? a.splits : 1) <= threads;
 }
 
 template <int DT, bool BF>
 static hipError_t launch_share(const PagedShare& a, hipStream_t st)
 {
-    if (a.g.n_seqs && a.g.cap) {
-        PagedShare b = a;
-        b.c = a.g;
-        b.p = a.gp;
-        if (b.p.tok_n) {
-            const dim3 grid((unsigned)(b.c.nkv * b.p.tok_n * b.c.n_seqs));
-            if (b.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF, kPrefix>), grid, dim3(512), 0, st, b);
-            else hipLaunchKernelGGL((k_paged_tok<DT, 4, BF, kPrefix>), grid, dim3(256), 0, st, b);
-        }
-        if (b.p.tile_n) {
-            const dim3 grid((unsigned)(b.c.nkv * b.p.tile_n * b.p.tiles));
-            if constexpr (BF) {
-                if (b.p.tile_rows == 128) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kPrefix>), grid, dim3(256), 0, st, b);
-            }
-            if (b.p.tile_rows == 64) hipLaunchKernelGGL((k_paged_tile<DT, 1, BF, kPrefix>), grid, dim3(256), 0, st, b);
+    const bool prefix = a.g.n_seqs && a.g.cap;
+    const unsigned prefix_tok = prefix ? (unsigned)(a.g.nkv * a.gp.tok_n * a.g.n_seqs) : 0;
+    unsigned prefix_tile = prefix ? (unsigned)(a.g.nkv * a.gp.tile_n * a.gp.tiles) : 0;
+    unsigned own_tile = (unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles);
+    const unsigned own_tok = (unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs);
+    ShareArgs args = {a, a};
+    args.p.c = a.g;
+    args.p.p = a.gp;
+    if constexpr (BF) {
+        if (a.p.tile_rows == 128) {
+            if (prefix_tile) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kPrefix>), dim3(prefix_tile), dim3(256), 0, st, args.p);
+            if (own_tile) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kOwn>), dim3(own_tile), dim3(256), 0, st, a);
+            prefix_tile = own_tile = 0;
         }
     }
-    if (a.p.tok_n) {
-        const dim3 grid((unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs));
-        if (a.weight && a.scored) {
-            if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF, kScored>), grid, dim3(512), 0, st, a);
-            else hipLaunchKernelGGL((k_paged_tok<DT, 4, BF, kScored>), grid, dim3(256), 0, st, a);
-        } else {
-            if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF, kOwn>), grid, dim3(512), 0, st, a);
-            else hipLaunchKernelGGL((k_paged_tok<DT, 4, BF, kOwn>), grid, dim3(256), 0, st, a);
-        }
-    }
-    if (a.p.tile_n) {
-        const dim3 grid((unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles));
-        if constexpr (BF) {
-            if (a.p.tile_rows == 128) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kOwn>), grid, dim3(256), 0, st, a);
-        }
-        if (a.p.tile_rows == 64) hipLaunchKernelGGL((k_paged_tile<DT, 1, BF, kOwn>), grid, dim3(256), 0, st, a);
-    }
-    if (a.parts > 8)
+    auto go = [&](auto k) {
+        const unsigned all = prefix_tok + prefix_tile + own_tile + own_tok;
+        if (all) hipLaunchKernelGGL(k, dim3(all), dim3(256), 0, st, args, prefix_tok, prefix_tile, own_tile);
+    };
+    if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF, kScored>), dim3(own_tok), dim3(512), 0, st, a);
+    else if (a.weight && a.scored) go(k_share<DT, BF, true>);
+    else go(k_share<DT, BF, false>);
+    const bool many = (int64_t)a.c.rows * a.nh > 8192;
+    const dim3 one((unsigned)a.c.rows, (unsigned)((a.nh + 7) / 8)), four((unsigned)a.c.rows, (unsigned)((a.nh + 31) / 32));
+    if (a.parts > 16)
         hipLaunchKernelGGL((k_paged_merge<4, BF, kOwn>), dim3((unsigned)a.c.rows, (unsigned)a.nh), dim3(256), 0, st, a);
-    else if (a.parts > 1 || a.split)
-        hipLaunchKernelGGL((k_paged_merge<1, BF, kOwn>), dim3((unsigned)a.c.rows, (unsigned)((a.nh + 3) / 4)), dim3(256), 0,
-                           st, a);
+    else if (a.parts > 8)
+        hipLaunchKernelGGL((k_share_merge<1, 16, BF>), one, dim3(256), 0, st, a);
+    else if (a.parts > 1 && many)
+        hipLaunchKernelGGL((k_share_merge<4, 8, BF>), four, dim3(256), 0, st, a);
+    else if (a.parts > 1)
+        hipLaunchKernelGGL((k_share_merge<1, 8, BF>), one, dim3(256), 0, st, a);
     if (a.weight && a.c.cap) {
-        const unsigned blocks = (unsigned)a.c.nkv * ((a.c.cap + 255) / 256) * a.c.n_seqs;
+        const unsigned heads = (unsigned)(a.c.nkv * a.c.n_seqs);
         const bool tiles = a.p.lo != INT_MAX || !a.scored;
-        if (tiles) hipLaunchKernelGGL((k_account_tile<DT, BF>), dim3(blocks * a.splits), dim3(256), 0, st, a);
-        if (a.scored || a.splits > 1) hipLaunchKernelGGL(k_account_sum, dim3(blocks), dim3(256), 0, st, a);
+        if (tiles)
+            hipLaunchKernelGGL((k_account_tile<DT, BF>), dim3(heads * ((a.c.cap + 255) / 256) * a.splits), dim3(256), 0, st, a);
+        if (a.scored || a.splits > 1)
+            hipLaunchKernelGGL(k_account_sum, dim3(heads * ((a.c.cap + 1023) / 1024)), dim3(256), 0, st, a);
     }
     return hipGetLastError();
 }
