@@ -2,7 +2,8 @@
 // positions of most weight.
 //
 // Kernels:
-//   k_evict_choose   per (sequence, KV head): which positions stay, where each goes.
+//   k_evict_choose   per (sequence, KV head): which positions stay, where each goes;
+//   k_evict_count, k_evict_collect, k_evict_rank   the same for long sequences.
 //   k_evict_move     the moved positions' codes and scales.
 //
 // Of a head's `len` positions the `keep` first in the order (protected, weight, position)
@@ -19,9 +20,9 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kEach = 8;                 // positions of a thread at a time
-constexpr int kSpan = kThreads * kEach;  // positions of the workgroup at a time
-constexpr int kBins = 4096;              // of the first 12 bits; the next two digits have 10
-constexpr int kHeld = 8192;              // keys that LDS holds
+constexpr int kSpan = kThreads * kEach;  // positions of a workgroup at a time
+static_assert(kSpan == kEvictSpan, "the host sizes the workspace by it");
+constexpr int kBins = kEvictBins;        // of a digit: 11, 11 and 10 bits
 
 // What a sequence is cut down to.
 struct Cut {
@@ -48,276 +49,466 @@ __device__ __forceinline__ uint32_t order_of(float w)
     return b << 1 == 0 ? 0x80000000u : (b >> 31 ? ~b : b | 0x80000000u);
 }
 
-// sum of v over the lanes below, and over all
-__device__ __forceinline__ int wave_before(int v, int lane, int& all)
+// the sum of v over the lanes up to this one
+__device__ __forceinline__ int wave_upto(int v)
 {
-    int upto = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(upto, off, 64);
-        upto += lane >= off ? o : 0;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);  // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);  // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);  // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);  // row_bcast:31
+    return v;
+}
+
+// its sum over the lanes below, and over all
+__device__ __forceinline__ int wave_before(int v, int& all)
+{
+    const int upto = wave_upto(v);
     all = __builtin_amdgcn_readlane(upto, 63);
     return upto - v;
 }
+
+// One head of a sequence.
+struct Head {
+    const float* weight;
+    const int32_t* token;
+    float* weight_out;
+    int32_t* token_out;
+    int32_t* from;  // [keep]: -1 where a position stays
+    int len, keep, filled, shift;
+    int sink, late;  // tokens below and from there on are protected
+
+    __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int s, int64_t head)
+        : Head(a, cut, s, head, a.filled, a.shift)
+    {
+    }
+    __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int s, int64_t head, const int32_t* filled_,
+                                    const int32_t* shift_)
+        : weight(a.weight + head * a.ld), token(a.token + head * a.ld), weight_out(a.weight_out + head * a.ld_out),
+          token_out(a.token_out + head * a.ld_out), from(a.from + head * a.c.cap), len(cut.len), keep(cut.keep),
+          filled(filled_[s]), shift(shift_[s]), sink(a.sink ? a.sink[s] : 0)
+    {
+        // tokens are int32, so a bound past them is the bound
+        const int64_t first = (int64_t)len + shift - (a.recent ? max(a.recent[s], 0) : 0);
+        late = (int)max(min(first, (int64_t)INT_MAX), (int64_t)INT_MIN);
+    }
+    __device__ __forceinline__ int in_order(int j) const { return (int)((uint32_t)j + (uint32_t)shift); }
+    __device__ __forceinline__ int token_at(int j) const { return j < filled ? token[j] : in_order(j); }
+    // position `to` takes what position `src` has
+    __device__ __forceinline__ void put(int to, int src) const
+    {
+        const float w = weight[src];
+        const int t = token_at(src);
+        weight_out[to] = w;
+        token_out[to] = t;
+    }
+};
+
+// A thread's positions of a span: four neighbours at a time, a wave 256 of them.
+struct Each {
+    float w[kEach];
+    int t[kEach];
+    int first;  // position of element 0
+
+    __device__ __forceinline__ int at(int e) const { return first + 256 * (e >> 2) + (e & 3); }
+
+    __device__ __forceinline__ void load(const Head& h, int base, int tid)
+    {
+        first = base + 64 * kEach * (tid >> 6) + 4 * (tid & 63);
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) {
+            const int j = at(e);
+            if (j + 4 <= h.len) {
+                const Four x = *(const Four*)(h.weight + j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[e + i] = __uint_as_float(x.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[e + i] = j + i < h.len ? h.weight[j + i] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) t[e] = h.in_order(at(e));
+        if (base >= h.filled) return;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (at(e) < min(h.filled, h.len)) t[e] = h.token[at(e)];
+    }
+    // protected positions are above every weight
+    __device__ __forceinline__ uint32_t key(const Head& h, int e) const
+    {
+        return t[e] < h.sink || t[e] >= h.late ? 0xFFFFFFFFu : order_of(w[e]);
+    }
+};
+
+// What a workgroup counts with.
+struct Lds {
+    uint32_t bin[kBins];
+    int wave[2][kWaves];
+    uint32_t found[3];
+};
+
+// The sought key, digit by digit from the top: it lies among those whose bits from `low` on
+// are `top`'s, as the left-th largest of them.
+struct Sought {
+    uint32_t top;
+    int left, low;
+    bool all;  // all of those stay
+};
+
+// count(f) hands every key to f.  Narrows x down by one digit.
+template <typename F>
+__device__ __forceinline__ void narrow(Lds& s, Sought& x, int tid, F count)
+{
+    const int low = x.low == 32 ? 21 : (x.low == 21 ? 10 : 0), bins = 1 << (x.low - low);
+    const int lane = tid & 63, wave = tid >> 6;
+    for (int i = tid; i < bins; i += kThreads) s.bin[i] = 0;
+    __syncthreads();
+    count([&](uint32_t key) {
+        if (x.low == 32 || key >> x.low == x.top >> x.low) atomicAdd(&s.bin[key >> low & (uint32_t)(bins - 1)], 1u);
+    });
+    __syncthreads();
+    // thread i has the bins 2 i and 2 i + 1 from the top
+    const uint32_t n0 = 2 * tid < bins ? s.bin[bins - 1 - 2 * tid] : 0, n1 = 2 * tid < bins ? s.bin[bins - 2 - 2 * tid] : 0;
+    int all;
+    int before = wave_before((int)(n0 + n1), all);
+    if (lane == 0) s.wave[0][wave] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) before += w < wave ? s.wave[0][w] : 0;
+    const uint32_t run = (uint32_t)before, left = (uint32_t)x.left;
+    if (run < left && run + n0 + n1 >= left) {
+        const bool one = run + n0 >= left;
+        s.found[0] = (uint32_t)(bins - 1 - 2 * tid - (one ? 0 : 1)) << low;
+        s.found[1] = left - run - (one ? 0 : n0);
+        s.found[2] = one ? n0 : n1;
+    }
+    __syncthreads();
+    x.top |= s.found[0];
+    x.left = (int)s.found[1];
+    x.low = low;
+    x.all = s.found[1] == s.found[2];
+}
+
+// Which of a thread's positions stay, and their places in the order, over a workgroup.
+// equal: equals of the sought key ahead of the span.
+struct Flags {
+    uint32_t same, stays;  // bit e
+};
+
+__device__ __forceinline__ Flags flags_of(Lds& s, const Head& h, const Each& v, const Sought& x, int equal, int tid)
+{
+    const int lane = tid & 63, wave = tid >> 6;
+    Flags f = {0, 0};
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const bool in = v.at(e) < h.len;
+        const uint32_t key = v.key(h, e) >> x.low, top = x.top >> x.low;
+        f.same |= (uint32_t)(in && key == top) << e;
+        f.stays |= (uint32_t)(in && key > top) << e;
+    }
+    if (x.all) {  // no equals to tell apart
+        f.stays |= f.same;
+        return f;
+    }
+    int all = 0, ties[kEach / 4];
+#pragma unroll
+    for (int e = 0; e < kEach; e += 4) {
+        int sum;
+        ties[e / 4] = all + wave_before(__popc(f.same >> e & 15u), sum);
+        all += sum;
+    }
+    if (lane == 0) s.wave[0][wave] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) equal += w < wave ? s.wave[0][w] : 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int t = equal + ties[e / 4] + __popc(f.same >> (e & ~3) & ((1u << (e & 3)) - 1));
+        f.stays |= (f.same >> e & 1u) && t < x.left ? 1u << e : 0u;
+    }
+    return f;
+}
+
+// The places of the marked positions (bit e of is) in the order, over the workgroup.
+struct Ranks {
+    int before[kEach / 4], all;
+
+    __device__ __forceinline__ Ranks(Lds& s, uint32_t is, int tid)
+    {
+        const int lane = tid & 63, wave = tid >> 6;
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) {
+            int sum;
+            before[e / 4] = mine + wave_before(__popc(is >> e & 15u), sum);
+            mine += sum;
+        }
+        if (lane == 0) s.wave[1][wave] = mine;
+        __syncthreads();
+        int ahead = 0;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const int n = s.wave[1][w];
+            ahead += w < wave ? n : 0;
+            all += n;
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) before[e / 4] += ahead;
+    }
+    __device__ __forceinline__ int of(uint32_t is, int e) const
+    {
+        return before[e / 4] + __popc(is >> (e & ~3) & ((1u << (e & 3)) - 1));
+    }
+};
 
 }  // namespace
 
 // ---------------------------------------------------------------------------
 // k_evict_choose
 // ---------------------------------------------------------------------------
-// A workgroup a (sequence, KV head).  The keep-th largest weight is found by counting
-// digits of 12, 10 and 10 bits; then one pass in order ranks holes and sources, and one
-// joins them.  Heads of up to kSpan positions (ONE, by the host's bound) are held in
-// registers between the passes; longer ones are read for each, and what shares the first
-// digit of the sought weight, few of many, is held in LDS after the second.
-// grid nkv * n_seqs, block 1024.
-template <bool ONE>
+// Heads of up to kSpan positions, a workgroup each, the positions in registers.  The
+// keep-th largest weight is found by counting digits of 11, 11 and 10 bits; then holes and
+// sources are ranked in order and joined through LDS.  grid nkv * n_seqs, block 1024.
 __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
 {
-    // the counts of a digit; the keys that share the first one; the sources that move
-    __shared__ uint32_t s_bin[kBins];
-    __shared__ uint32_t s_key[ONE ? 1 : kHeld];
-    __shared__ int s_wave[2][kWaves];
-    __shared__ uint32_t s_found[2], s_count;
-    const Paged& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = (int)(blockIdx.x % (unsigned)c.nkv), s = (int)(blockIdx.x / (unsigned)c.nkv);
+    __shared__ Lds lds;
+    __shared__ int s_source[kSpan / 2];
+    const int tid = threadIdx.x;
+    const int s = (int)(blockIdx.x / (unsigned)a.c.nkv);
     const Cut cut = cut_of(a, s);
     if (!cut.ok) return;
-    const int len = cut.len, keep = cut.keep;
-    const int64_t head = (int64_t)s * c.nkv + h;
-    const float* weight = a.weight + head * a.ld;
-    const int32_t* token = a.token + head * a.ld;
-    float* weight_out = a.weight_out + head * a.ld_out;
-    int32_t* token_out = a.token_out + head * a.ld_out;
-    const int filled = a.filled[s], shift = a.shift[s];
-    const int sink = a.sink ? a.sink[s] : 0;
-    // the first token of the last ones (tokens are int32, so a bound past them is the bound)
-    const int64_t first_late = (int64_t)len + shift - (a.recent ? max(a.recent[s], 0) : 0);
-    const int late = (int)max(min(first_late, (int64_t)INT_MAX), (int64_t)INT_MIN);
-    auto token_at = [&](int j) { return j < filled ? token[j] : (int)((uint32_t)j + (uint32_t)shift); };
-    if (keep == len) {
-        for (int j = tid; j < len; j += kThreads) {
-            const float w = weight[j];
-            const int t = token_at(j);
-            weight_out[j] = w;
-            token_out[j] = t;
-        }
+    const Head h(a, cut, s, blockIdx.x);
+    if (h.keep == h.len) {
+        for (int j = tid; j < h.len; j += kThreads) h.put(j, j);
         return;
     }
-    int32_t* from = a.from + head * a.from_ld;  // [keep]: where a hole's bytes come from; -1: it is none
-    int32_t* movers = a.movers + head * c.cap;  // the sources, behind as many places as there are holes
-
-    // A thread's positions of a span: four neighbours at a time, a wave 256 of them.
-    auto place = [&](int base, int e) { return base + 256 * ((kEach / 4) * wave + e / 4) + 4 * lane + e % 4; };
-    struct Each {
-        float w[kEach];
-        int t[kEach];
-    };
-    auto load = [&](int base, Each& x) {
-#pragma unroll
-        for (int e = 0; e < kEach; e += 4) {
-            const int j = place(base, e);
-            if (j + 4 <= len) {
-                const Four w = *(const Four*)(weight + j);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.w[e + i] = __uint_as_float(w.v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.w[e + i] = j + i < len ? weight[j + i] : 0.0f;
-            }
-        }
-        if (base < filled) {
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int j = place(base, e);
-                x.t[e] = j < min(filled, len) ? token[j] : (int)((uint32_t)j + (uint32_t)shift);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) x.t[e] = (int)((uint32_t)place(base, e) + (uint32_t)shift);
-        }
-    };
-    auto key_of = [&](const Each& x, int e) {
-        return x.t[e] < sink || x.t[e] >= late ? 0xFFFFFFFFu : order_of(x.w[e]);
-    };
-    // f(key, position) of every position, a span's loads ahead of the work on the one before
-    Each x;
-    if (ONE) load(0, x);
-    auto each = [&](auto f) {
-        if (ONE) {
+    if (h.keep == 0) return;
+    Each v;
+    v.load(h, 0, tid);
+    Sought x = {0, h.keep, 32, false};
+    while (x.low > 0 && !x.all)
+        narrow(lds, x, tid, [&](auto f) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e)
-                if (place(0, e) < len) f(key_of(x, e), place(0, e));
-            return;
-        }
-        load(0, x);
-        for (int base = 0; base < len; base += kSpan) {
-            uint32_t key[kEach];
+                if (v.at(e) < h.len) f(v.key(h, e));
+        });
+    const Flags f = flags_of(lds, h, v, x, 0, tid);
+    uint32_t is = 0;  // holes, and behind as many of them the sources
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) key[e] = key_of(x, e);
-            if (base + kSpan < len) load(base + kSpan, x);
+    for (int e = 0; e < kEach; ++e) is |= (v.at(e) < h.keep ? ~f.stays : f.stays) & 1u << e;
+    const Ranks r(lds, is, tid);
+    const int holes = r.all / 2;
 #pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                if (place(base, e) < len) f(key[e], place(base, e));
-        }
-    };
-
-    // the keep-th largest key, digit by digit from the top; `left`: its rank among those that
-    // share the digits so far
-    uint32_t found = 0, left = (uint32_t)keep;
-    int held = -1;  // keys in LDS that share the first digit (-1: they are looked for)
-    for (int digit = 0; digit < 3 && keep > 0; ++digit) {
-        const int low = digit == 0 ? 20 : (digit == 1 ? 10 : 0), bins = digit == 0 ? kBins : 1024;
-        for (int i = tid; i < bins; i += kThreads) s_bin[i] = 0;
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        auto count = [&](uint32_t key) { atomicAdd(&s_bin[key >> low & (uint32_t)(bins - 1)], 1u); };
-        if (digit == 0) {
-            each([&](uint32_t key, int) { count(key); });
-        } else if (held >= 0) {
-            for (int i = tid; i < held; i += kThreads)
-                if (s_key[i] >> (low + 10) == found >> (low + 10)) count(s_key[i]);
+    for (int e = 0; e < kEach; ++e)
+        if (v.at(e) >= h.keep && (is >> e & 1u)) s_source[r.of(is, e) - holes] = v.at(e);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int j = v.at(e);
+        if (j >= h.keep) continue;
+        if (is >> e & 1u) {
+            const int src = s_source[r.of(is, e)];
+            h.from[j] = src;
+            h.put(j, src);
         } else {
-            each([&](uint32_t key, int) {
-                if (key >> (low + 10) != found >> (low + 10)) return;
-                count(key);
-                if (!ONE && digit == 1) {
-                    const uint32_t at = atomicAdd(&s_count, 1u);
-                    if (at < kHeld) s_key[at] = key;
-                }
-            });
+            h.from[j] = -1;
+            h.weight_out[j] = v.w[e];
+            h.token_out[j] = v.t[e];
         }
-        __syncthreads();
-        if (!ONE && digit == 1 && s_count <= kHeld) held = (int)s_count;
-        // thread i has the bins from the top: per thread, then over the threads
-        const int per = bins / kThreads;
-        uint32_t mine[kBins / kThreads];
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBins / kThreads; ++i) {
-            mine[i] = i < per ? s_bin[bins - 1 - (per * tid + i)] : 0;
-            sum += (int)mine[i];
-        }
-        int all;
-        int before = wave_before(sum, lane, all);
-        if (lane == 0) s_wave[0][wave] = all;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) before += w < wave ? s_wave[0][w] : 0;
-        uint32_t run = (uint32_t)before;
-#pragma unroll
-        for (int i = 0; i < kBins / kThreads; ++i) {
-            if (run < left && run + mine[i] >= left) {
-                s_found[0] = (uint32_t)(bins - 1 - (per * tid + i)) << low;
-                s_found[1] = left - run;
-            }
-            run += mine[i];
-        }
-        __syncthreads();
-        found |= s_found[0];
-        left = s_found[1];
     }
+}
 
-    // in order: what is above the key stays, and the first `left` of its equals
-    int equal = 0, moved = 0;  // so far
-    if (!ONE) load(0, x);
-    for (int base = 0; base < len; base += kSpan) {
-        uint32_t same = 0, above = 0;  // bit e: of this thread's positions
+// ---------------------------------------------------------------------------
+// k_evict_count, k_evict_collect, k_evict_rank
+// ---------------------------------------------------------------------------
+// Longer heads, a workgroup a span of kSpan positions, block 1024, grid spans * nkv *
+// n_seqs each.  k_evict_count counts the first digit; k_evict_collect finds the sought
+// key's from all spans' counts and puts down the keys that share it; k_evict_rank finds
+// the key among those and ranks its span's holes from the first on and its sources from
+// the last back, which it knows from what stays in the spans before and behind.  The span
+// that `keep` falls into puts down how many holes there are; k_evict_move joins them.
+namespace {
+
+struct Span {
+    int h, s, part, base;
+    int64_t head;
+};
+
+__device__ __forceinline__ Span span_of(const PagedEvict& a)
+{
+    Span p;
+    p.h = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const unsigned b = blockIdx.x / (unsigned)a.c.nkv;
+    p.part = (int)(b % (unsigned)a.spans);
+    p.s = (int)(b / (unsigned)a.spans);
+    p.base = kSpan * p.part;
+    p.head = (int64_t)p.s * a.c.nkv + p.h;
+    return p;
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(kThreads) void k_evict_count(PagedEvict a)
+{
+    __shared__ uint32_t s_bin[kBins];
+    const int tid = threadIdx.x;
+    const Span p = span_of(a);
+    const Cut cut = cut_of(a, p.s);
+    if (!cut.ok || p.base >= cut.len || cut.keep == cut.len || cut.keep == 0) return;
+    const Head h(a, cut, p.s, p.head);
+    // k_evict_move may put out over what came in
+    if (p.h == 0 && p.part == 0 && tid == 0) {
+        a.was[p.s] = h.filled;
+        a.was[a.c.n_seqs + p.s] = h.shift;
+    }
+    Each v;
+    v.load(h, p.base, tid);
+    for (int i = tid; i < kBins; i += kThreads) s_bin[i] = 0;
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const uint32_t key = key_of(x, e);
-            const bool in = keep > 0 && place(base, e) < len;
-            same |= (uint32_t)(in && key == found) << e;
-            above |= (uint32_t)(in && key > found) << e;
-        }
-        if (!ONE && base + kSpan < len) load(base + kSpan, x);
-        int all = 0, ties[kEach / 4];  // equals ahead of each four
+    for (int e = 0; e < kEach; ++e)
+        if (v.at(e) < h.len) atomicAdd(&s_bin[v.key(h, e) >> 21], 1u);
+    __syncthreads();
+    // two counts of at most kSpan a word
+    uint32_t* to = a.counts + (p.head * a.spans + p.part) * (kBins / 2);
+    for (int i = tid; i < kBins / 2; i += kThreads) to[i] = s_bin[2 * i] | s_bin[2 * i + 1] << 16;
+}
+
+__global__ __launch_bounds__(kThreads) void k_evict_collect(PagedEvict a)
+{
+    __shared__ Lds lds;
+    __shared__ int s_above, s_count;
+    const int tid = threadIdx.x;
+    const Span p = span_of(a);
+    const Cut cut = cut_of(a, p.s);
+    if (!cut.ok || p.base >= cut.len || cut.keep == cut.len || cut.keep == 0) return;
+    const Head h(a, cut, p.s, p.head);
+    Each v;
+    v.load(h, p.base, tid);
+    const int spans = (h.len + kSpan - 1) / kSpan;
+    if (tid == 0) s_above = s_count = 0;
+    // the first digit of the sought key, from the sums of the spans' counts
+    Sought x = {0, h.keep, 32, false};
+    {
+        const uint32_t* from = a.counts + p.head * a.spans * (kBins / 2) + tid;
+        uint32_t n0 = 0, n1 = 0;
+        for (int i0 = 0; i0 < spans; i0 += 16) {
+            uint32_t n[16];
 #pragma unroll
-        for (int e = 0; e < kEach; e += 4) {
-            int sum;
-            ties[e / 4] = all + wave_before(__popc(same >> e & 15u), lane, sum);
-            all += sum;
-        }
-        if (lane == 0) s_wave[0][wave] = all;
-        __syncthreads();
-        int ahead = equal;
+            for (int i = 0; i < 16; ++i) n[i] = from[(int64_t)min(i0 + i, spans - 1) * (kBins / 2)];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const int n = s_wave[0][w];
-            ahead += w < wave ? n : 0;
-            equal += n;
-        }
-        uint32_t is = 0;  // a hole, or a source
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int j = place(base, e), t = ahead + ties[e / 4] + __popc(same >> (e & ~3) & ((1u << (e & 3)) - 1));
-            const bool stays = (above >> e & 1) || ((same >> e & 1) && t < (int)left);
-            is |= (uint32_t)(j < keep ? !stays : stays) << e;
-        }
-        int before[kEach / 4];
-        all = 0;
-#pragma unroll
-        for (int e = 0; e < kEach; e += 4) {
-            int sum;
-            before[e / 4] = all + wave_before(__popc(is >> e & 15u), lane, sum);
-            all += sum;
-        }
-        if (lane == 0) s_wave[1][wave] = all;
-        __syncthreads();
-        int rank = moved;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const int n = s_wave[1][w];
-            rank += w < wave ? n : 0;
-            moved += n;
-        }
-        // the n-th hole or source in order
-        auto nth = [&](int e) { return rank + before[e / 4] + __popc(is >> (e & ~3) & ((1u << (e & 3)) - 1)); };
-        if (ONE) {
-            // the sources are joined with the holes through LDS
-            const int holes = moved / 2;  // the sources stand behind as many holes
-#pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                if (place(0, e) >= keep && (is >> e & 1)) s_bin[nth(e) - holes] = (uint32_t)place(0, e);
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int j = place(0, e);
-                if (j >= keep) continue;
-                if (is >> e & 1) {
-                    const int src = (int)s_bin[nth(e)];
-                    from[j] = src;
-                    weight_out[j] = weight[src];
-                    token_out[j] = token_at(src);
-                } else {
-                    from[j] = -1;
-                    weight_out[j] = x.w[e];
-                    token_out[j] = x.t[e];
-                }
+            for (int i = 0; i < 16; ++i) {
+                n0 += i0 + i < spans ? n[i] & 0xFFFFu : 0;
+                n1 += i0 + i < spans ? n[i] >> 16 : 0;
             }
-            return;
         }
+        // thread i has the bins 2 i and 2 i + 1
+        const int mine = (int)(n0 + n1), upto = wave_upto(mine), all = __builtin_amdgcn_readlane(upto, 63);
+        if ((tid & 63) == 0) lds.wave[0][tid >> 6] = all;
+        __syncthreads();
+        int above = all - upto;  // in bins above this thread's
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int j = place(base, e);
-            if (j < keep) from[j] = is >> e & 1 ? nth(e) : -1;
-            else if (is >> e & 1) movers[nth(e)] = j;
+        for (int w = 0; w < kWaves; ++w) above += w > tid >> 6 ? lds.wave[0][w] : 0;
+        if (above < h.keep && above + mine >= h.keep) {
+            const bool high = above + (int)n1 >= h.keep;
+            lds.found[0] = (uint32_t)(2 * tid + (high ? 1 : 0)) << 21;
+            lds.found[1] = (uint32_t)(h.keep - above - (high ? 0 : (int)n1));
+        }
+        __syncthreads();
+        x.top = lds.found[0];
+        x.left = (int)lds.found[1];
+    }
+    uint32_t* keys = a.keys + p.head * a.c.cap + p.base;
+    int above = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (v.at(e) >= h.len) continue;
+        const uint32_t key = v.key(h, e);
+        above += key >> 21 > x.top >> 21;
+        // in no order: of equals only the number counts
+        if (key >> 21 == x.top >> 21) keys[atomicAdd(&s_count, 1)] = key;
+    }
+    above = wave_upto(above);
+    if ((tid & 63) == 63) atomicAdd(&s_above, above);
+    __syncthreads();
+    if (tid) return;
+    int32_t* to = a.spanned + 4 * (p.head * a.spans + p.part);
+    to[0] = s_above;
+    to[1] = s_count;
+    to[2] = (int)x.top;
+    to[3] = x.left;
+}
+
+__global__ __launch_bounds__(kThreads) void k_evict_rank(PagedEvict a)
+{
+    __shared__ Lds lds;
+    __shared__ int s_ahead[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Span p = span_of(a);
+    const Cut cut = cut_of(a, p.s);
+    if (!cut.ok || p.base >= cut.len || cut.keep == 0) return;
+    const Head h(a, cut, p.s, p.head);
+    const int end = min(p.base + kSpan, h.len);
+    if (h.keep == h.len) {
+        for (int j = p.base + tid; j < end; j += kThreads) h.put(j, j);
+        return;
+    }
+    Each v;
+    v.load(h, p.base, tid);
+    const int spans = (h.len + kSpan - 1) / kSpan;
+    const int32_t* spanned = a.spanned + 4 * p.head * a.spans;
+    const uint32_t* keys = a.keys + p.head * a.c.cap;
+    Sought x = {(uint32_t)spanned[2], spanned[3], 21, false};
+    while (x.low > 0 && !x.all)
+        narrow(lds, x, tid, [&](auto f) {
+            for (int i = wave; i < spans; i += kWaves)
+                for (int n = spanned[4 * i + 1], y = lane; y < n; y += 64) f(keys[(int64_t)i * kSpan + y]);
+        });
+    // what is above the key ahead of this span, and its equals
+    if (tid < 2) s_ahead[tid] = 0;
+    __syncthreads();
+    for (int i = wave; i < p.part; i += kWaves) {
+        int above = 0, same = 0;
+        for (int n = spanned[4 * i + 1], y = lane; y < n; y += 64) {
+            const uint32_t key = keys[(int64_t)i * kSpan + y] >> x.low, top = x.top >> x.low;
+            above += key > top;
+            same += key == top;
+        }
+        above = __builtin_amdgcn_readlane(wave_upto(above), 63) + spanned[4 * i];
+        same = __builtin_amdgcn_readlane(wave_upto(same), 63);
+        if (lane == 0) {
+            atomicAdd(&s_ahead[0], above);
+            atomicAdd(&s_ahead[1], same);
         }
     }
     __syncthreads();
-    // as many sources as holes, behind them in the count
-    const int holes = moved / 2;
-    for (int j = tid; j < keep; j += kThreads) {
-        const int r = from[j];
-        const int src = r < 0 ? j : movers[holes + r];
-        if (r >= 0) from[j] = src;
-        const float w = weight[src];
-        const int t = token_at(src);
-        weight_out[j] = w;
-        token_out[j] = t;
+    const int equal = s_ahead[1], stay_ahead = s_ahead[0] + min(equal, x.left);
+    const Flags f = flags_of(lds, h, v, x, equal, tid);
+    uint32_t hole = 0, source = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const bool below = v.at(e) < h.keep;
+        hole |= (below ? ~f.stays : 0u) & 1u << e;
+        source |= (below ? 0u : f.stays) & 1u << e;
     }
+    const Ranks holes(lds, hole, tid);
+    __syncthreads();
+    const Ranks sources(lds, source, tid);
+    // ahead of a span that has holes all positions lie below keep; behind one that has sources
+    // all that stays is a source
+    const int holes_ahead = p.base - stay_ahead, below = max(min(h.keep, end) - p.base, 0);
+    const int behind = h.keep - stay_ahead - (below - holes.all + sources.all);
+    int32_t* movers = a.movers + p.head * a.c.cap;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int j = v.at(e);
+        if (j < h.keep) h.from[j] = hole >> e & 1u ? holes_ahead + holes.of(hole, e) : -1;
+        else if (source >> e & 1u) movers[behind + sources.all - 1 - sources.of(source, e)] = j;
+    }
+    if (tid == 0 && p.base < h.keep && h.keep <= end) a.holes[p.head] = holes_ahead + holes.all;
 }
 
 // ---------------------------------------------------------------------------
@@ -325,7 +516,10 @@ __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
 // ---------------------------------------------------------------------------
 // A wave a block of 16 slots below `keep` of a (sequence, KV head): the holes' keys row by
 // row, and its values' block made anew from the bytes of the slots that are to lie in it
-// (a slot that stays gives its own).  grid nkv * ceil(max_keep / 64) * n_seqs, block 256.
+// (a slot that stays gives its own).  LONG: after k_evict_rank, whose holes and sources are
+// joined here, with their weights and tokens.  grid nkv * ceil(max_keep / 64) * n_seqs,
+// block 256.
+template <bool LONG>
 __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
 {
     const Paged& c = a.c;
@@ -348,7 +542,13 @@ __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
     const int32_t* table = c.pages + (int64_t)s * c.max_pages;
     // lane r < 16: where the slot j0 + r comes from (-1: stays)
     const int r = lane & 15;
-    const int src = j0 + r < cut.keep ? a.from[((int64_t)s * c.nkv + h) * a.from_ld + j0 + r] : -1;
+    const int64_t head = (int64_t)s * c.nkv + h;
+    int src = j0 + r < cut.keep ? a.from[head * c.cap + j0 + r] : -1;
+    if (LONG) {
+        if (src >= 0) src = a.movers[head * c.cap + a.holes[head] - 1 - src];
+        if (lane < 16 && j0 + r < cut.keep)
+            Head(a, cut, s, head, a.was, a.was + c.n_seqs).put(j0 + r, src >= 0 ? src : j0 + r);
+    }
     if (!__any(src >= 0)) return;
     int in;
     const int page = page_of(c, table, block, &in);
@@ -425,11 +625,19 @@ __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
 
 hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st)
 {
-    const dim3 heads((unsigned)(a.c.nkv * a.c.n_seqs));
-    if (a.c.cap > kSpan) hipLaunchKernelGGL(k_evict_choose<false>, heads, dim3(kThreads), 0, st, a);
-    else if (a.c.cap) hipLaunchKernelGGL(k_evict_choose<true>, heads, dim3(kThreads), 0, st, a);
+    const unsigned heads = (unsigned)(a.c.nkv * a.c.n_seqs);
     const int blocks = evict_blocks(a);
-    hipLaunchKernelGGL(k_evict_move, dim3((unsigned)(a.c.nkv * blocks * a.c.n_seqs)), dim3(256), 0, st, a, blocks);
+    const dim3 move(heads * blocks);
+    if (a.spans > 1) {
+        const dim3 spans(heads * a.spans);
+        hipLaunchKernelGGL(k_evict_count, spans, dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(k_evict_collect, spans, dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(k_evict_rank, spans, dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(k_evict_move<true>, move, dim3(256), 0, st, a, blocks);
+    } else {
+        if (a.spans) hipLaunchKernelGGL(k_evict_choose, dim3(heads), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(k_evict_move<false>, move, dim3(256), 0, st, a, blocks);
+    }
     return hipGetLastError();
 }
 

@@ -116,10 +116,19 @@ struct PagedEvict {
     const int32_t* sink;    // or NULL
     const int32_t* recent;  // or NULL
     int32_t* held;
-    int max_keep, from_ld;
-    int32_t* from;    // [n_seqs][nkv][from_ld]
-    int32_t* movers;  // [n_seqs][nkv][cap]
+    int max_keep;
+    int spans;         // of kEvictSpan positions: ceil(cap / kEvictSpan)
+    int32_t* from;     // [n_seqs][nkv][cap]
+    // where there are several spans
+    int32_t* movers;   // [n_seqs][nkv][cap]
+    uint32_t* keys;    // [n_seqs][nkv][cap]
+    uint32_t* counts;  // [n_seqs][nkv][spans][kEvictBins / 2]
+    int32_t* spanned;  // [n_seqs][nkv][spans][4]
+    int32_t* holes;    // [n_seqs][nkv]
+    int32_t* was;      // [2][n_seqs]: filled and shift as they came in
 };
+constexpr int kEvictSpan = 8192;
+constexpr int kEvictBins = 2048;
 // workgroups along the slots that may be written to
 inline int evict_blocks(const PagedEvict& a)
 {

@@ -350,18 +350,33 @@ int btl_paged_attention_account(const void* q, int dtype, int64_t n_heads, const
     return attention_share(q, dtype, n_heads, cache, batch, prefix, account, out, ws, ws_bytes, stream);
 }
 
-static size_t evict_bytes(const btl::Paged& c, size_t* movers)
+// Lays out a's workspace from `p` on; returns its bytes.
+static size_t evict_workspace(btl::PagedEvict& a, uint8_t* p)
 {
-    const size_t n = (size_t)c.n_seqs * c.nkv * c.cap * 4;
-    *movers = up256(n);
-    return 2 * up256(n);
+    const size_t heads = (size_t)a.c.n_seqs * a.c.nkv, each = up256(heads * a.c.cap * 4);
+    a.spans = (a.c.cap + btl::kEvictSpan - 1) / btl::kEvictSpan;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        uint8_t* q = p + at;
+        at += up256(n);
+        return q;
+    };
+    a.from = (int32_t*)take(each);
+    if (a.spans > 1) {
+        a.movers = (int32_t*)take(each);
+        a.keys = (uint32_t*)take(each);
+        a.counts = (uint32_t*)take(heads * a.spans * (btl::kEvictBins / 2) * 4);
+        a.spanned = (int32_t*)take(heads * a.spans * 16);
+        a.holes = (int32_t*)take(heads * 4);
+        a.was = (int32_t*)take((size_t)a.c.n_seqs * 8);
+    }
+    return at;
 }
 
 size_t btl_paged_evict_workspace_bytes(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch)
 {
-    btl::Paged c{};
-    size_t movers;
-    return check_sizes(cache, batch, &c) ? 0 : evict_bytes(c, &movers);
+    btl::PagedEvict a{};
+    return check_sizes(cache, batch, &a.c) ? 0 : evict_workspace(a, nullptr);
 }
 
 int btl_paged_evict(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, const btl_kv_account_t* account,
@@ -380,7 +395,7 @@ int btl_paged_evict(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch,
     if (a.c.n_seqs == 0) return BTL_OK;
     a.max_keep = (int)std::min<int64_t>(max_keep, INT_MAX);
     const int64_t threads = ((int64_t)1 << 32) - 1;
-    if ((int64_t)a.c.nkv * a.c.n_seqs * 1024 > threads ||
+    if ((int64_t)a.c.nkv * a.c.n_seqs * std::max((a.c.cap + btl::kEvictSpan - 1) / btl::kEvictSpan, 1) * 1024 > threads ||
         (int64_t)a.c.nkv * a.c.n_seqs * btl::evict_blocks(a) * 256 > threads)
         return fail_msg(BTL_ERR_SHAPE, "batch too large for one launch");
     if ((rc = check_pointers(cache, batch, &a.c))) return rc;
@@ -415,13 +430,10 @@ int btl_paged_evict(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch,
     }
     int dev;
     if ((rc = btl::host::device(&dev))) return rc;
-    size_t movers;
     void* p = nullptr;
-    const size_t need = evict_bytes(a.c, &movers);
+    const size_t need = evict_workspace(a, nullptr);
     if (need && (rc = btl::host::workspace(dev, ws, ws_bytes, need, &p, (hipStream_t)stream))) return rc;
-    a.from = (int32_t*)p;
-    a.movers = (int32_t*)((uint8_t*)p + movers);
-    a.from_ld = a.c.cap;
+    evict_workspace(a, (uint8_t*)p);
     a.weight = account->weight;
     a.token = account->token;
     a.filled = account->filled;

@@ -62,11 +62,13 @@ __global__ __launch_bounds__(256, 2) void k_share(ShareArgs, unsigned prefix_tok
 // k_paged_merge for rows of at most U parts: half a wave a (row, head), four values a
 // lane, every lane holding all the parts' maxima; N heads one after the other, so that
 // what is known of the row serves them all.  grid (rows, ceil(nh / (8 N))), block 256.
+namespace {
+
 template <int N, int U, bool BF>
-__global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
+__device__ __forceinline__ void share_merge(const PagedShare& a, int t, int block)
 {
     const Paged& c = a.c;
-    const int t = blockIdx.x, lane = threadIdx.x & 63, d = 4 * (lane & 31), hd = c.hd;
+    const int lane = threadIdx.x & 63, d = 4 * (lane & 31), hd = c.hd;
     const int s = find_seq(c, t, lane);
     if (s < 0 || s >= c.n_seqs) return;
     const Seq q = seq_at(c, s);
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
     const int nc = p.parts + (q.p0 + i) / C + 1;
 #pragma unroll
     for (int x = 0; x < N; ++x) {
-        const int head = (int)blockIdx.y * 8 * N + 8 * x + (int)(threadIdx.x >> 5);
+        const int head = block * 8 * N + 8 * x + (int)(threadIdx.x >> 5);
         if (head >= a.nh) return;
         const int64_t r = (int64_t)t * a.nh + head, at = r * a.parts;
         float2 ml[U];
@@ -111,6 +113,14 @@ __global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
             store4<BF>(a.out, r * hd + d, v);
         }
     }
+}
+
+}  // namespace
+
+template <int N, int U, bool BF>
+__global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
+{
+    share_merge<N, U, BF>(a, blockIdx.x, blockIdx.y);
 }
 
 // ---------------------------------------------------------------------------
@@ -343,48 +353,79 @@ __global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a)
 // ---------------------------------------------------------------------------
 // Four positions a thread: the weights from the scores of at most 16 rows, or the sum of
 // the shares of k_account_tile, in order.  grid nkv * ceil(cap / 1024) * n_seqs, block 256.
-__global__ __launch_bounds__(256) void k_account_sum(PagedShare a)
+// U: the rows' maxima and sums are taken from their parts, at most U of them, beside the
+// merge that does the same (0: they lie in a.ml).
+namespace {
+
+template <int U>
+__device__ __forceinline__ void account_sum(const PagedShare& a, unsigned block)
 {
+    __shared__ float2 s_ml[kTokRows];
     const Paged& c = a.c;
-    const int h = (int)(blockIdx.x % (unsigned)c.nkv);
-    const unsigned at = blockIdx.x / (unsigned)c.nkv, blocks = (unsigned)(c.cap + 1023) / 1024;
-    const int key = 4 * (256 * (int)(at % blocks) + threadIdx.x), s = (int)(at / blocks);
+    const int h = (int)(block % (unsigned)c.nkv);
+    const unsigned at = block / (unsigned)c.nkv, blocks = (unsigned)(c.cap + 1023) / 1024;
+    const int key0 = 1024 * (int)(at % blocks), key = key0 + 4 * (int)threadIdx.x, s = (int)(at / blocks);
     const Seq q = seq_at(c, s);
-    const int64_t M = (int64_t)q.n * a.group, head = (int64_t)s * c.nkv + h;
+    const int64_t M = (int64_t)q.n * a.group, head = (int64_t)s * c.nkv + h, row0 = (int64_t)q.a * a.nh + h * a.group;
     const int seen = q.p0 + q.n;
-    if (M == 0 || !q.ok || key >= seen) return;
+    if (M == 0 || !q.ok || key0 >= seen) return;
+    const bool scores = has_scores(a, M);
+    if (!scores && a.splits == 1) return;  // put out where they were summed
+    if (scores) {
+        const int lane = threadIdx.x & 63;
+        for (int i = threadIdx.x >> 6; i < q.n; i += 4) {
+            const int64_t r = row0 + (int64_t)i * a.nh + min(lane, a.group - 1);
+            const bool whole = U == 0 || whole_of<kOwn>(a, seen, a.p.tok_c);
+            const Behind p = whole ? Behind{} : behind(a, q.a + i, lane);
+            float2 ml;
+            if (whole) {
+                ml = *(const float2*)(a.ml + 2 * r);
+            } else {
+                const int n = p.parts + (q.p0 + i) / a.p.tok_c + 1;
+                float2 part[U ? U : 1];
+                float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+                for (int y = 0; y < U; ++y)
+                    if (y < n) {
+                        part[y] = *(const float2*)(a.part_ml + 2 * (r * a.parts + (y < p.parts ? y : a.own0 - p.parts + y)));
+                        top = fmaxf(top, part[y].x);
+                    }
+#pragma unroll
+                for (int y = 0; y < U; ++y)
+                    if (y < n) sum = __fmaf_rn(__builtin_amdgcn_exp2f(__fsub_rn(part[y].x, top)), part[y].y, sum);
+                ml = make_float2(top, p.lost ? __builtin_nanf("") : sum);
+            }
+            // a row that came back as NaN adds nothing
+            const bool good = ml.y > 0.0f && ml.y < __builtin_inff();
+            if (lane < a.group) s_ml[i * a.group + lane] = make_float2(ml.x, good ? __fdiv_rn(1.0f, ml.y) : 0.0f);
+        }
+        __syncthreads();
+    }
+    if (key >= seen) return;
     float* to = a.weight + head * a.ld + key;
     const bool four = key + 4 <= a.ld;
     Four old = {};  // asked for beside the scores
     if (four) old = *(const Four*)to;
     f4 w = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (has_scores(a, M)) {
+    if (scores) {
         const float* sc = a.scores + head * a.score_rows * a.score_ld + key;
-        const int64_t row0 = (int64_t)q.a * a.nh + h * a.group;
-        constexpr int U = 4;
-        for (int m0 = 0; m0 < (int)M; m0 += U) {
-            f4 y[U];
-            float2 ml[U];
+        constexpr int V = 4;  // rows at a time
+        for (int m0 = 0; m0 < (int)M; m0 += V) {
+            f4 y[V];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int m = min(m0 + u, (int)M - 1), i = row_of(a, m);
-                y[u] = *(const f4*)(sc + (int64_t)m * a.score_ld);
-                ml[u] = *(const float2*)(a.ml + 2 * (row0 + (int64_t)i * a.nh + (m - i * a.group)));
-            }
+            for (int u = 0; u < V; ++u) y[u] = *(const f4*)(sc + (int64_t)min(m0 + u, (int)M - 1) * a.score_ld);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                // a row that came back as NaN adds nothing
-                const bool good = m0 + u < (int)M && ml[u].y > 0.0f && ml[u].y < __builtin_inff();
-                const float part = good ? __fdiv_rn(1.0f, ml[u].y) : 0.0f;
+            for (int u = 0; u < V; ++u) {
+                const float2 ml = s_ml[min(m0 + u, (int)M - 1)];
+                const bool good = m0 + u < (int)M && ml.y > 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(__fsub_rn(y[u][e], ml[u].x));
-                    w[e] = good ? __fmaf_rn(p, part, w[e]) : w[e];
+                    const float p = __builtin_amdgcn_exp2f(__fsub_rn(y[u][e], ml.x));
+                    w[e] = good ? __fmaf_rn(p, ml.y, w[e]) : w[e];
                 }
             }
         }
     } else {
-        if (a.splits == 1) return;  // put out where they were summed
         for (int x = 0; x < a.splits; ++x) {
             const f4 y = *(const f4*)(a.sums + ((int64_t)x * c.n_seqs * c.nkv + head) * a.score_ld + key);
 #pragma unroll
@@ -401,6 +442,19 @@ __global__ __launch_bounds__(256) void k_account_sum(PagedShare a)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (key + e < seen) put_weight(a, q, s, h, key + e, w[e]);
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(256) void k_account_sum(PagedShare a) { account_sum<0>(a, blockIdx.x); }
+
+// The merge and the weights from the token form's scores in one launch, where nothing else
+// is to be done between them.  grid merge + nkv * ceil(cap / 1024) * n_seqs, block 256.
+template <int U, bool BF>
+__global__ __launch_bounds__(256) void k_share_finish(PagedShare a, unsigned merge)
+{
+    if (blockIdx.x < merge) share_merge<1, U, BF>(a, (int)(blockIdx.x % (unsigned)a.c.rows), (int)(blockIdx.x / (unsigned)a.c.rows));
+    else account_sum<U>(a, blockIdx.x - merge);
 }
 
 bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
@@ -497,23 +551,27 @@ static hipError_t launch_share(const PagedShare& a, hipStream_t st)
     if (a.p.tok_w == 8) hipLaunchKernelGGL((k_paged_tok<DT, 8, BF, kScored>), dim3(own_tok), dim3(512), 0, st, a);
     else if (a.weight && a.scored) go(k_share<DT, BF, true>);
     else go(k_share<DT, BF, false>);
-    const bool many = (int64_t)a.c.rows * a.nh > 8192;
+    const bool account = a.weight && a.c.cap, tiles = a.p.lo != INT_MAX || !a.scored;
+    const unsigned heads = (unsigned)(a.c.nkv * a.c.n_seqs), sums = heads * ((a.c.cap + 1023) / 1024);
     const dim3 one((unsigned)a.c.rows, (unsigned)((a.nh + 7) / 8)), four((unsigned)a.c.rows, (unsigned)((a.nh + 31) / 32));
+    if (account && !tiles && a.parts > 1 && a.parts <= 16) {
+        const unsigned merge = one.x * one.y;
+        if (a.parts > 8) hipLaunchKernelGGL((k_share_finish<16, BF>), dim3(merge + sums), dim3(256), 0, st, a, merge);
+        else hipLaunchKernelGGL((k_share_finish<8, BF>), dim3(merge + sums), dim3(256), 0, st, a, merge);
+        return hipGetLastError();
+    }
     if (a.parts > 16)
         hipLaunchKernelGGL((k_paged_merge<4, BF, kOwn>), dim3((unsigned)a.c.rows, (unsigned)a.nh), dim3(256), 0, st, a);
     else if (a.parts > 8)
         hipLaunchKernelGGL((k_share_merge<1, 16, BF>), one, dim3(256), 0, st, a);
-    else if (a.parts > 1 && many)
+    else if (a.parts > 1 && (int64_t)a.c.rows * a.nh > 8192)
         hipLaunchKernelGGL((k_share_merge<4, 8, BF>), four, dim3(256), 0, st, a);
     else if (a.parts > 1)
         hipLaunchKernelGGL((k_share_merge<1, 8, BF>), one, dim3(256), 0, st, a);
-    if (a.weight && a.c.cap) {
-        const unsigned heads = (unsigned)(a.c.nkv * a.c.n_seqs);
-        const bool tiles = a.p.lo != INT_MAX || !a.scored;
+    if (account) {
         if (tiles)
             hipLaunchKernelGGL((k_account_tile<DT, BF>), dim3(heads * ((a.c.cap + 255) / 256) * a.splits), dim3(256), 0, st, a);
-        if (a.scored || a.splits > 1)
-            hipLaunchKernelGGL(k_account_sum, dim3(heads * ((a.c.cap + 1023) / 1024)), dim3(256), 0, st, a);
+        if (a.scored || a.splits > 1) hipLaunchKernelGGL(k_account_sum, dim3(sums), dim3(256), 0, st, a);
     }
     return hipGetLastError();
 }

@@ -143,7 +143,8 @@ def test_workspaces():
     # scores of 2^28 and more are not kept: the workspace stays small
     assert size(n_seqs=64, rows=64, max_rows=1, max_len=1 << 20, max_pages=1 << 17) < 1 << 32
     c, b = cache(), batch()
-    assert bl.lib.btl_paged_evict_workspace_bytes(by(c), by(b)) >= 2 * 3 * 2 * 50 * 4
+    assert bl.lib.btl_paged_evict_workspace_bytes(by(c), by(b)) >= 3 * 2 * 50 * 4
+    assert bl.lib.btl_paged_evict_workspace_bytes(by(cache()), by(batch(max_len=10 ** 5, max_pages=10 ** 4))) >= 3 * 3 * 2 * 10 ** 5 * 4
     assert bl.lib.btl_paged_evict_workspace_bytes(None, by(b)) == 0
 
 

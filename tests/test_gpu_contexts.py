@@ -280,6 +280,11 @@ EVICTS = [
     (3, 96, 256, [2000, 1], [999, 1], 0, 2000, False),        # all of them among the last
     (1, 32, 128, [20000, 8192, 8193], [5000, 100, 8191], 4, 100, True),  # several spans
     (4, 48, 16, [50] * 7, [25] * 7, 0, 3, True),
+    # spans: keep at their ends and beside them, whole and empty sequences among long ones, few that go
+    (1, 16, 64, [30000, 24577, 16384, 8192, 100], [24576, 8192, 16383, 1, 50], 0, 0, False),
+    (2, 32, 256, [9000, 20001, 0, 8200], [-1, 0, 5, 9000], 10, 7, True),
+    (1, 16, 128, [50000], [49999], 3, 1000, True),
+    (1, 16, 128, [40000, 40000], [8193, 33000], 20000, 9000, False),
 ]
 
 
