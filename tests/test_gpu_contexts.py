@@ -53,6 +53,9 @@ PREFIXES = [
     (8, 2, 112, 256, [(70, 0)], [(0, 70, 2049)]),             # chunks of the prefix
     (12, 4, 48, 32, [(2, 600), (1, 511), (1, 512)], [(0, 4, 512)]),               # chunks of both
     (3, 1, 32, 16, [(0, 9), (1, 0), (0, 0), (150, 3)], [(0, 151, 64)]),           # sequences without rows
+    (4, 2, 16, 128, [(1, 40), (1, 3000)], [(0, 1, 6001), (1, 1, 5)]),             # many chunks of few tokens
+    (32, 8, 128, 64, [(395, 30), (5, 100)], [(0, 400, 330)]),                     # tiles of 128 rows in bf16
+    (2, 2, 64, 16, [(9, 2)], [(0, 3, 40), (3, 0, 9), (3, 6, 80)]),                # a list without rows
 ]
 
 
@@ -156,6 +159,10 @@ ACCOUNTS = [
     (12, 4, 48, 16, [(65, 511), (1, 1), (2, 700)], [(0, 65, 100), (65, 3, 31)]),
     (8, 2, 64, 32, [(1, 20), (1, 3), (2, 40), (1, 100)], [(0, 2, 300), (2, 2, 0)]),
     (2, 2, 128, 16, [(100, 1)], [(0, 50, 17)]),                # rows of no list
+    (8, 2, 64, 128, [(1, 5003)], []),                          # many chunks
+    (4, 2, 32, 64, [(2, 3100), (1, 7)], []),                   # of two rows, and of some
+    (32, 8, 128, 64, [(390, 300), (20, 0)], [(0, 390, 150)]),  # tiles of 128 rows in bf16
+    (15, 1, 112, 16, [(1, 200), (1, 0), (3, 64)], [(0, 2, 100)]),  # groups of 15
 ]
 
 
