@@ -24,17 +24,21 @@ constexpr int kSpan = kThreads * kEach;  // positions of a workgroup at a time
 static_assert(kSpan == kEvictSpan, "the host sizes the workspace by it");
 constexpr int kBins = kEvictBins;        // of a digit: 11, 11 and 10 bits
 
-// What a sequence is cut down to.
+// What a sequence is cut down to, and what its arguments say: all read at once.
 struct Cut {
-    int len, keep;
+    int len, keep, filled, shift, sink, recent;
     bool ok;
 };
 
-__device__ __forceinline__ Cut cut_of(const PagedEvict& a, int s)
+__device__ __forceinline__ Cut cut_of(const PagedEvict& a, int s, const int32_t* filled, const int32_t* shift)
 {
     const Seq q = seq_at(a.c, s);
     const int keep = a.keep[s];
     Cut x;
+    x.filled = filled[s];
+    x.shift = shift[s];
+    x.sink = a.sink ? a.sink[s] : 0;
+    x.recent = a.recent ? max(a.recent[s], 0) : 0;
     x.len = q.p0 + q.n;
     x.ok = q.ok && (keep < 0 || keep >= x.len || keep <= a.max_keep);
     x.keep = keep < 0 ? x.len : min(keep, x.len);
@@ -79,19 +83,13 @@ struct Head {
     int len, keep, filled, shift;
     int sink, late;  // tokens below and from there on are protected
 
-    __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int s, int64_t head)
-        : Head(a, cut, s, head, a.filled, a.shift)
-    {
-    }
-    __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int s, int64_t head, const int32_t* filled_,
-                                    const int32_t* shift_)
+    __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int64_t head)
         : weight(a.weight + head * a.ld), token(a.token + head * a.ld), weight_out(a.weight_out + head * a.ld_out),
           token_out(a.token_out + head * a.ld_out), from(a.from + head * a.c.cap), len(cut.len), keep(cut.keep),
-          filled(filled_[s]), shift(shift_[s]), sink(a.sink ? a.sink[s] : 0)
+          filled(cut.filled), shift(cut.shift), sink(cut.sink)
     {
         // tokens are int32, so a bound past them is the bound
-        const int64_t first = (int64_t)len + shift - (a.recent ? max(a.recent[s], 0) : 0);
-        late = (int)max(min(first, (int64_t)INT_MAX), (int64_t)INT_MIN);
+        late = (int)max(min((int64_t)len + shift - cut.recent, (int64_t)INT_MAX), (int64_t)INT_MIN);
     }
     __device__ __forceinline__ int in_order(int j) const { return (int)((uint32_t)j + (uint32_t)shift); }
     __device__ __forceinline__ int token_at(int j) const { return j < filled ? token[j] : in_order(j); }
@@ -275,12 +273,13 @@ struct Ranks {
 __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
 {
     __shared__ Lds lds;
-    __shared__ int s_source[kSpan / 2];
+    __shared__ int s_source[kSpan / 2], s_token[kSpan / 2];  // of the positions that move: where, and what lies there
+    __shared__ float s_weight[kSpan / 2];
     const int tid = threadIdx.x;
     const int s = (int)(blockIdx.x / (unsigned)a.c.nkv);
-    const Cut cut = cut_of(a, s);
+    const Cut cut = cut_of(a, s, a.filled, a.shift);
     if (!cut.ok) return;
-    const Head h(a, cut, s, blockIdx.x);
+    const Head h(a, cut, blockIdx.x);
     if (h.keep == h.len) {
         for (int j = tid; j < h.len; j += kThreads) h.put(j, j);
         return;
@@ -303,21 +302,22 @@ __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
     const int holes = r.all / 2;
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
-        if (v.at(e) >= h.keep && (is >> e & 1u)) s_source[r.of(is, e) - holes] = v.at(e);
+        if (v.at(e) >= h.keep && (is >> e & 1u)) {
+            const int at = r.of(is, e) - holes;
+            s_source[at] = v.at(e);
+            s_token[at] = v.t[e];
+            s_weight[at] = v.w[e];
+        }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int j = v.at(e);
         if (j >= h.keep) continue;
-        if (is >> e & 1u) {
-            const int src = s_source[r.of(is, e)];
-            h.from[j] = src;
-            h.put(j, src);
-        } else {
-            h.from[j] = -1;
-            h.weight_out[j] = v.w[e];
-            h.token_out[j] = v.t[e];
-        }
+        const bool hole = is >> e & 1u;
+        const int at = hole ? r.of(is, e) : 0;
+        h.from[j] = hole ? s_source[at] : -1;
+        h.weight_out[j] = hole ? s_weight[at] : v.w[e];
+        h.token_out[j] = hole ? s_token[at] : v.t[e];
     }
 }
 
@@ -356,9 +356,9 @@ __global__ __launch_bounds__(kThreads) void k_evict_count(PagedEvict a)
     __shared__ uint32_t s_bin[kBins];
     const int tid = threadIdx.x;
     const Span p = span_of(a);
-    const Cut cut = cut_of(a, p.s);
+    const Cut cut = cut_of(a, p.s, a.filled, a.shift);
     if (!cut.ok || p.base >= cut.len || cut.keep == cut.len || cut.keep == 0) return;
-    const Head h(a, cut, p.s, p.head);
+    const Head h(a, cut, p.head);
     // k_evict_move may put out over what came in
     if (p.h == 0 && p.part == 0 && tid == 0) {
         a.was[p.s] = h.filled;
@@ -383,9 +383,9 @@ __global__ __launch_bounds__(kThreads) void k_evict_collect(PagedEvict a)
     __shared__ int s_above, s_count;
     const int tid = threadIdx.x;
     const Span p = span_of(a);
-    const Cut cut = cut_of(a, p.s);
+    const Cut cut = cut_of(a, p.s, a.filled, a.shift);
     if (!cut.ok || p.base >= cut.len || cut.keep == cut.len || cut.keep == 0) return;
-    const Head h(a, cut, p.s, p.head);
+    const Head h(a, cut, p.head);
     Each v;
     v.load(h, p.base, tid);
     const int spans = (h.len + kSpan - 1) / kSpan;
@@ -448,9 +448,9 @@ __global__ __launch_bounds__(kThreads) void k_evict_rank(PagedEvict a)
     __shared__ int s_ahead[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Span p = span_of(a);
-    const Cut cut = cut_of(a, p.s);
+    const Cut cut = cut_of(a, p.s, a.filled, a.shift);
     if (!cut.ok || p.base >= cut.len || cut.keep == 0) return;
-    const Head h(a, cut, p.s, p.head);
+    const Head h(a, cut, p.head);
     const int end = min(p.base + kSpan, h.len);
     if (h.keep == h.len) {
         for (int j = p.base + tid; j < end; j += kThreads) h.put(j, j);
@@ -527,7 +527,18 @@ __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
     const int h = (int)(blockIdx.x % (unsigned)c.nkv);
     const unsigned at = blockIdx.x / (unsigned)c.nkv;
     const int block = 4 * (int)(at % (unsigned)blocks) + wave, s = (int)(at / (unsigned)blocks);
-    const Cut cut = cut_of(a, s);
+    const int hd = c.hd, j0 = 16 * block, r = lane & 15;
+    const int64_t head = (int64_t)s * c.nkv + h;
+    // asked for beside the sequence's size, not after it: where the slot j0 + r comes from (-1:
+    // stays), if it is one that is held, and the page of the block
+    const int32_t* table = c.pages + (int64_t)s * c.max_pages;
+    int src = -1, in = 0, page = -1;
+    if (j0 < c.cap) {
+        src = a.from[head * c.cap + min(j0 + r, c.cap - 1)];
+        page = page_of(c, table, block, &in);
+    }
+    // (over the account that came in: what k_evict_count has put by)
+    const Cut cut = cut_of(a, s, LONG ? a.was : a.filled, LONG ? a.was + c.n_seqs : a.shift);
     if (h == 0 && block == 0 && lane == 0) {
         a.held[s] = cut.ok ? cut.keep : -1;
         if (cut.ok) {
@@ -536,22 +547,13 @@ __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
             a.shift_out[s] = (int)((uint32_t)shift + (uint32_t)(cut.len - cut.keep));
         }
     }
-    const int j0 = 16 * block;
     if (!cut.ok || cut.keep == cut.len || j0 >= cut.keep) return;
-    const int hd = c.hd;
-    const int32_t* table = c.pages + (int64_t)s * c.max_pages;
-    // lane r < 16: where the slot j0 + r comes from (-1: stays)
-    const int r = lane & 15;
-    const int64_t head = (int64_t)s * c.nkv + h;
-    int src = j0 + r < cut.keep ? a.from[head * c.cap + j0 + r] : -1;
+    if (j0 + r >= cut.keep) src = -1;
     if (LONG) {
         if (src >= 0) src = a.movers[head * c.cap + a.holes[head] - 1 - src];
-        if (lane < 16 && j0 + r < cut.keep)
-            Head(a, cut, s, head, a.was, a.was + c.n_seqs).put(j0 + r, src >= 0 ? src : j0 + r);
+        if (lane < 16 && j0 + r < cut.keep) Head(a, cut, head).put(j0 + r, src >= 0 ? src : j0 + r);
     }
     if (!__any(src >= 0)) return;
-    int in;
-    const int page = page_of(c, table, block, &in);
     if (page < 0) return;  // no slot to write
     const int64_t blk = ((int64_t)page * c.nkv + h) * c.ps + 16 * in;
     int src_in;

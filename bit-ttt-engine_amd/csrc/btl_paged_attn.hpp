@@ -426,14 +426,19 @@ struct Behind {
     bool lost;
 };
 
-__device__ __forceinline__ Behind behind(const PagedShare& a, int t, int lane)
+// list: the last that starts at or before the row
+__device__ __forceinline__ Behind behind_of(const PagedShare& a, int t, int list)
 {
-    const int list = a.g.n_seqs ? find_seq(a.g, t, lane) : -1;
     if (list < 0 || list >= a.g.n_seqs) return {0, false};
     const Seq p = seq_of<kPrefix>(a.g, list);
     if (t < p.a || t >= p.a + p.n) return {0, false};
     const int C = (int64_t)p.n * a.group > a.gp.lo ? a.gp.tile_c : a.gp.tok_c;
     return {p.ok ? (p.p0 + C - 1) / C : 0, !p.ok};
+}
+
+__device__ __forceinline__ Behind behind(const PagedShare& a, int t, int lane)
+{
+    return behind_of(a, t, a.g.n_seqs ? find_seq(a.g, t, lane) : -1);
 }
 
 // The rows of a refused sequence.

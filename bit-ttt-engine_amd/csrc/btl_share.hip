@@ -69,14 +69,23 @@ __device__ __forceinline__ void share_merge(const PagedShare& a, int t, int bloc
 {
     const Paged& c = a.c;
     const int lane = threadIdx.x & 63, d = 4 * (lane & 31), hd = c.hd;
-    const int s = find_seq(c, t, lane);
+    int s, list = -1;
+    if (a.g.n_seqs && c.n_seqs < 64 && a.g.n_seqs < 64) {
+        // both in the time of one: 64 starts of each at once
+        const int v = lane <= c.n_seqs ? c.row_start[lane] : INT_MAX, w = lane <= a.g.n_seqs ? a.g.row_start[lane] : INT_MAX;
+        s = 63 - __clzll(__ballot(lane <= c.n_seqs && v <= t));
+        list = 63 - __clzll(__ballot(lane <= a.g.n_seqs && w <= t));
+    } else {
+        s = find_seq(c, t, lane);
+        if (a.g.n_seqs) list = find_seq(a.g, t, lane);
+    }
     if (s < 0 || s >= c.n_seqs) return;
     const Seq q = seq_at(c, s);
+    const Behind p = behind_of(a, t, list);
     const int i = t - q.a;
     if (i < 0 || i >= q.n || !q.ok) return;
     const int C = (int64_t)q.n * a.group > a.p.lo ? a.p.tile_c : a.p.tok_c;
     if (whole_of<kOwn>(a, q.p0 + q.n, C)) return;  // written by its one chunk
-    const Behind p = behind(a, t, lane);
     const int nc = p.parts + (q.p0 + i) / C + 1;
 #pragma unroll
     for (int x = 0; x < N; ++x) {
