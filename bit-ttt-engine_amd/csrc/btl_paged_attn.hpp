@@ -765,8 +765,7 @@ __device__ __forceinline__ void paged_tile(const PagedArgs<MODE>& a, unsigned bl
 
     Running<DT, MODE != kPlain> r[NT];
     Queries<NJ, NT, BF> qs;
-    auto step = [&](int kb, int b, auto masked) {
-        if (kb + 64 < key1) fetch(kb + 64);
+    auto work = [&](int kb, int b, auto masked) {
         f4 sc[NT][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -838,6 +837,12 @@ __device__ __forceinline__ void paged_tile(const PagedArgs<MODE>& a, unsigned bl
             __builtin_amdgcn_sched_group_barrier(0x008, PARTS * NT, 1);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
         }
+    };
+    // a wave behind the tile's last row widens its share and leaves the rest to the others
+    const bool busy = MODE == kPlain || m_wave <= m_last;
+    auto step = [&](int kb, int b, auto masked) {
+        if (kb + 64 < key1) fetch(kb + 64);
+        if (busy) work(kb, b, masked);
         if (kb + 64 < key1) put(b ^ 1);
         __syncthreads();
     };
