@@ -484,7 +484,10 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
     const int hd = c.hd, ndt = hd >> 4, C = a.p.tok_c;
-    const Place at = place_of(c, a.p.tok_n, block);
+    Place at = place_of(c, a.p.tok_n, block);
+    // over a prefix a list may have several tiles of 16 rows
+    const int m0 = MODE == kPrefix ? 16 * (at.tile % a.p.tiles) : 0;
+    if (MODE == kPrefix) at.s = at.tile / a.p.tiles;
     const int key0 = at.chunk * C;
     const int32_t* table = c.pages + (int64_t)at.s * c.max_pages;
     // the pages are looked up beside the sequence's size, not after it: what the table holds
@@ -494,7 +497,7 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
     if (c.cap > 0) slots.find(c, table, (key0 + 64 * wave) >> 4, last_grp, at.h, lane);
     const Seq q = seq_of<MODE>(c, at.s);
     const int64_t M = (int64_t)q.n * a.group;
-    if (M == 0 || M > a.p.lo) return;
+    if (M <= m0 || M > a.p.lo) return;
     const int64_t row0 = (int64_t)q.a * a.nh + at.h * a.group;  // output row of m: row0 + (m / group) * nh + m % group
     if (!q.ok) {
         if (MODE != kPrefix && at.chunk == 0) fill_nan<BF>(a, q, at.h, wave, NW, lane);
@@ -505,7 +508,7 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
     if (key0 >= key1) return;
 
     Queries<NJ, 1, BF> qs;
-    qs.load(a, q, row0, 0, (int)M - 1, lane, MODE == kPlain ? a.scale_log2 : 1.0f);
+    qs.load(a, q, row0, m0, (int)M - 1, lane, MODE == kPlain ? a.scale_log2 : 1.0f);
     Running<DT, MODE != kPlain> r;
     r.clear();
     f4 kept[4];  // the last step's scores
@@ -604,7 +607,7 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
     __syncthreads();
     const PagedArgs<MODE>& z = at_the_end<MODE>(a);
     const bool whole = whole_of<MODE>(z, seen, C);
-    for (int x = threadIdx.x; x < (int)M * (hd >> 2); x += 64 * NW) {
+    for (int x = threadIdx.x; x < min((int)M - m0, 16) * (hd >> 2); x += 64 * NW) {
         const int m = x / (hd >> 2), d = 4 * (x - m * (hd >> 2));
         float top = s_m[0][m];
 #pragma unroll
@@ -620,8 +623,8 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, ow[e], v[e]);
         }
-        const int i = row_of(a, m);
-        const int64_t row = row0 + (int64_t)i * a.nh + (m - i * a.group);
+        const int i = row_of(a, m0 + m);
+        const int64_t row = row0 + (int64_t)i * a.nh + (m0 + m - i * a.group);
         if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);

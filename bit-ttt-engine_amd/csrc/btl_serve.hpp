@@ -56,7 +56,7 @@ struct AttnPlan {
     int tok_c, tile_c;    // keys a chunk
     int tok_n, tile_n;    // chunks of max_len keys
     int tile_rows;        // rows times heads of one workgroup of the tile form: 64 or 128
-    int tiles;            // workgroups along the rows of the tile form, at most
+    int tiles;            // workgroups along the rows of the tile form, at most; over a prefix a list's of the token form
     int parts() const { return tok_n > tile_n ? tok_n : tile_n; }
 };
 AttnPlan plan_paged_attention(int64_t n_heads, const Paged& c, bool bf);

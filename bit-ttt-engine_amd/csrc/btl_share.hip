@@ -492,22 +492,27 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
     a.own0 = 0;
     a.gp = AttnPlan{};
     if (a.split) {
-        // One form for all lists: tokens where every list is that short.
+        // One form for all lists: the token form, in tiles of 16 rows, where every list is of at most
+        // two (8 rows of 4 heads behind 4000 positions: 15.7 us, 16.5 in the tile form, in f32 14.8
+        // and 17.2; of three 19.1 and 16.7), in chunks for 256 workgroups (8 sequences behind 16000:
+        // 21.6 us, 24.4 with 192 or 512).
         AttnPlan& r = a.gp;
         const int64_t far = std::max(g.cap, 1), all = up(far, 256);
         r.tok_w = 4;
-        r.lo = g.max_rows * group <= kTokRows ? INT_MAX : 0;
+        const int64_t per_list = (int64_t)g.max_rows * group;
+        r.lo = per_list <= 2 * kTokRows ? INT_MAX : 0;
         r.tile_rows = p.tile_rows;
         r.tok_c = r.tile_c = (int)all;
         if (r.lo) {
-            r.tok_c = (int)std::min(all, up(far * g.n_seqs * g.nkv / 512 + 1, 256));
+            r.tiles = (int)std::max<int64_t>(1, (per_list + 15) / 16);
+            r.tok_c = (int)std::min(all, up(far * g.n_seqs * g.nkv * r.tiles / 256 + 1, 256));
             r.tok_n = (int)((far + r.tok_c - 1) / r.tok_c);
         } else {
             // Chunks so that there are about 256 workgroups, one a CU beside the sequences' own (64
             // tokens behind 8192 positions: 42.4 us, 48.5 with 192, 48.9 with 512, 58.9 with 1024);
             // of many tiles 2048, as long as a chunk has 2048 positions (12 questions behind 16001:
             // 406 us, 433 with 1024, 626 with one chunk).
-            const int64_t per = ((int64_t)g.max_rows * group + r.tile_rows - 1) / r.tile_rows;
+            const int64_t per = (per_list + r.tile_rows - 1) / r.tile_rows;
             r.tiles = (int)std::min<int64_t>((int64_t)g.n_seqs * per, (int64_t)g.rows * group / r.tile_rows + g.n_seqs);
             const int64_t base = (int64_t)r.tiles * g.nkv;
             const int64_t n = std::max<int64_t>({1, (256 + base / 2) / base, std::min(far / 2048, (2048 + base - 1) / base)});
@@ -520,7 +525,7 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
     a.splits = 1;
     const int64_t threads = ((int64_t)1 << 32) - 1;  // of a grid
     const int64_t blocks = (int64_t)c.nkv * p.tok_n * c.n_seqs + (int64_t)c.nkv * p.tile_n * p.tiles +
-                           (int64_t)g.nkv * a.gp.tok_n * g.n_seqs + (int64_t)g.nkv * a.gp.tile_n * a.gp.tiles;
+                           (int64_t)g.nkv * (a.gp.tok_n * (int64_t)g.n_seqs + a.gp.tile_n) * a.gp.tiles;
     if (blocks * 64 * p.tok_w > threads) return false;
     if (!account) return true;
 
@@ -539,7 +544,7 @@ template <int DT, bool BF>
 static hipError_t launch_share(const PagedShare& a, hipStream_t st)
 {
     const bool prefix = a.g.n_seqs && a.g.cap;
-    const unsigned prefix_tok = prefix ? (unsigned)(a.g.nkv * a.gp.tok_n * a.g.n_seqs) : 0;
+    const unsigned prefix_tok = prefix ? (unsigned)(a.g.nkv * a.gp.tok_n * a.g.n_seqs * a.gp.tiles) : 0;
     unsigned prefix_tile = prefix ? (unsigned)(a.g.nkv * a.gp.tile_n * a.gp.tiles) : 0;
     unsigned own_tile = (unsigned)(a.c.nkv * a.p.tile_n * a.p.tiles);
     const unsigned own_tok = (unsigned)(a.c.nkv * a.p.tok_n * a.c.n_seqs);

@@ -162,8 +162,8 @@ int btl_paged_attention(const void* q, int dtype, int64_t n_heads, const btl_kv_
  * all its rows; so has a row that needs a page outside the pool.
  * Lists end where the caller says, between sequences or inside one; prefix pages are
  * only read.
- * The arithmetic is btl_paged_attention's; which of its forms takes a prefix goes by the
- * rows times heads of its list.  ws: btl_paged_attention_prefix_workspace_bytes (or
+ * The arithmetic is btl_paged_attention's; of its forms the one of few rows takes a
+ * prefix where max_rows times the heads of a group is at most 32.  ws: btl_paged_attention_prefix_workspace_bytes (or
  * NULL: the library's).
  */
 size_t btl_paged_attention_prefix_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,

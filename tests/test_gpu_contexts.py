@@ -56,6 +56,8 @@ PREFIXES = [
     (4, 2, 16, 128, [(1, 40), (1, 3000)], [(0, 1, 6001), (1, 1, 5)]),             # many chunks of few tokens
     (32, 8, 128, 64, [(395, 30), (5, 100)], [(0, 400, 330)]),                     # tiles of 128 rows in bf16
     (2, 2, 64, 16, [(9, 2)], [(0, 3, 40), (3, 0, 9), (3, 6, 80)]),                # a list without rows
+    (6, 2, 48, 32, [(1, 9 * n) for n in range(11)], [(0, 7, 700), (7, 1, 300), (8, 2, 31)]),  # tiles of 16 rows: 21 of 32
+    (16, 2, 128, 16, [(2, 30), (2, 0)], [(0, 4, 1500)]),                          # two full ones
 ]
 
 
