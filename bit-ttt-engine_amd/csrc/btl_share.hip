@@ -568,7 +568,9 @@ static hipError_t launch_share(const PagedShare& a, hipStream_t st)
     const bool account = a.weight && a.c.cap, tiles = a.p.lo != INT_MAX || !a.scored;
     const unsigned heads = (unsigned)(a.c.nkv * a.c.n_seqs), sums = heads * ((a.c.cap + 1023) / 1024);
     const dim3 one((unsigned)a.c.rows, (unsigned)((a.nh + 7) / 8)), four((unsigned)a.c.rows, (unsigned)((a.nh + 31) / 32));
-    if (account && !tiles && a.parts > 1 && a.parts <= 16) {
+    // of both kinds of blocks fewer than a grid of 2^32 threads has: 2^21 rows of 64 heads are as many
+    const bool fits = (int64_t)one.x * one.y + sums < (int64_t)1 << 24;
+    if (account && !tiles && fits && a.parts > 1 && a.parts <= 16) {
         const unsigned merge = one.x * one.y;
         if (a.parts > 8) hipLaunchKernelGGL((k_share_finish<16, BF>), dim3(merge + sums), dim3(256), 0, st, a, merge);
         else hipLaunchKernelGGL((k_share_finish<8, BF>), dim3(merge + sums), dim3(256), 0, st, a, merge);

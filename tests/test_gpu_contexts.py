@@ -225,6 +225,32 @@ def test_weights_of_bounds_far_above_the_lengths():
         assert (account.weight[s, :, r + p:] == 0).all()
 
 
+def test_weights_beside_more_rows_than_a_grid_merges():
+    """2^21 rows of 64 heads, all but two behind the last sequence: their merges alone are 2^24
+    workgroups of 256 threads, one more than a grid has."""
+    nh, nkv, hd, ps, rows = 64, 4, 16, 16, 1 << 21
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GiB of free memory")
+    rng = np.random.default_rng(12)
+    sizes = [(1, 900), (1, 300)]
+    table, n_pages = ref.pages_for(sizes, ps, rng)
+    cache = ref.rand_cache(rng, n_pages, nkv, ps, hd)
+    batch, starts = batch_of(table, sizes, rows=rows)
+    q = torch.empty((rows, nh * hd), dtype=torch.bfloat16, device=DEV)
+    q[:2] = dev(rng.standard_normal((2, nh * hd)).astype(np.float32), torch.bfloat16)
+    out = torch.empty_like(q)
+    out[2:4], out[-1] = 7, 7
+    account = bl.KVAccount(2, nkv, 901, DEV)
+    workspace = bl.paged_attention_account_workspace(on_gpu(cache), batch, nh)
+    bl.paged_attention_account(q, on_gpu(cache), batch, account, out=out, workspace=workspace)
+    assert (out[2:4] == 7).all() and (out[-1] == 7).all()
+    want, bound, weights, wbounds = cref.attention(host(q[:2]).reshape(2, nh, hd), cache, table, sizes, starts, True)
+    within(host(out[:2]).reshape(2, nh, hd), want, bound)
+    for s, (r, p) in enumerate(sizes):
+        within(host(account.weight)[s, :, :r + p], weights[s], wbounds[s] + cref.U * weights[s])
+
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("size", [1e-30, 1e6, 1e12, 1e30])
