@@ -4,13 +4,9 @@
 // Kernels:
 //   k_paged_append   RoPE of the new q and k rows, Q8 of k and v into their slots.
 //   k_paged_read     rows of the cache dequantised.
-//   k_paged_attn     attention of a tile of rows over a chunk of keys.
-//   k_paged_merge    the chunks of a row merged.
-//
-// The sequences' sizes, positions and pages are read on the device, so a captured
-// launch follows them; whatever they hold, every address stays inside the arrays
-// (rows are clamped to `rows`, page ids checked, slots clamped to the last visible
-// one).
+// and those of btl_paged_attn.hpp in their form for a batch:
+//   k_paged_tok, k_paged_tile   attention of rows over a chunk of keys.
+//   k_paged_merge               the chunks of a row merged.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -215,7 +211,7 @@ __global__ __launch_bounds__(256) void k_paged_append_runs(PagedAppend a, int gr
     if (page < 0) return;
     // tokens r0 <= r < r1 of the group are rows of the call with a RoPE position
     const int64_t turn = rope_pos(a, s, 16 * grp);  // of the group's first position
-    const int r0 = max(max(0, -i0), (int)min(-turn, (int64_t)16));
+    const int r0 = max(max(0, -i0), (int)max(min(-turn, (int64_t)16), (int64_t)0));
     const int r1 = min(min(16, q.n - i0), (int)max(min(a.rope_len - turn, (int64_t)16), (int64_t)0));
     if (r0 >= r1) return;
     const int64_t blk = ((int64_t)page * nkv + head) * c.ps + 16 * in;
