@@ -270,6 +270,10 @@ struct Ranks {
 // Heads of up to kSpan positions, a workgroup each, the positions in registers.  The
 // keep-th largest weight is found by counting digits of 11, 11 and 10 bits; then holes and
 // sources are ranked in order and joined through LDS.  grid nkv * n_seqs, block 1024.
+//
+// Bound by latency: one reading, and a barrier after each of some fifteen steps; 11 us for
+// 64 heads of 1025, 15.4 for 256 of up to 8192.  Counting stops where all that share the
+// digits so far stay.  Read from memory once a digit the latter took 5 us more.
 __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
 {
     __shared__ Lds lds;
@@ -330,6 +334,11 @@ __global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
 // the key among those and ranks its span's holes from the first on and its sources from
 // the last back, which it knows from what stays in the spans before and behind.  The span
 // that `keep` falls into puts down how many holes there are; k_evict_move joins them.
+//
+// Bound by latency: 8 heads of 100001, 104 workgroups, 4.8, 7.1 and 10.1 us (one workgroup a
+// head, which goes through its head span by span, took 101 for all three).  A launch between
+// them is the cheapest way to have all spans' counts; a wait inside one kernel would need all
+// its workgroups to be resident.
 namespace {
 
 struct Span {
@@ -519,6 +528,12 @@ __global__ __launch_bounds__(kThreads) void k_evict_rank(PagedEvict a)
 // (a slot that stays gives its own).  LONG: after k_evict_rank, whose holes and sources are
 // joined here, with their weights and tokens.  grid nkv * ceil(max_keep / 64) * n_seqs,
 // block 256.
+//
+// A value's bytes of 16 slots lie together, so a moved slot is a byte in each of hd lines:
+// bytes one by one were 160 us for 32 sequences of up to 8192 cut down to 2048 (8 heads of
+// 128); whole blocks, each loaded once and picked from by byte permutes, four in flight, 82
+// (64 at best).  Up to 17 blocks of 2 KB are read for one that is put out, which is the bound
+// there: nearly every block behind `keep` has a slot that stays.
 template <bool LONG>
 __global__ __launch_bounds__(256) void k_evict_move(PagedEvict a, int blocks)
 {
