@@ -18,7 +18,7 @@ namespace btl {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the largest workgroups
 constexpr int kEach = 8;                 // positions of a thread at a time
 constexpr int kSpan = kThreads * kEach;  // positions of a workgroup at a time
 static_assert(kSpan == kEvictSpan, "the host sizes the workspace by it");
@@ -140,10 +140,11 @@ struct Each {
     }
 };
 
-// What a workgroup counts with.
+// What a workgroup of T threads counts with.
+template <int T = kThreads>
 struct Lds {
     uint32_t bin[kBins];
-    int wave[2][kWaves];
+    int wave[2][T / 64];
     uint32_t found[3];
 };
 
@@ -156,31 +157,46 @@ struct Sought {
 };
 
 // count(f) hands every key to f.  Narrows x down by one digit.
-template <typename F>
-__device__ __forceinline__ void narrow(Lds& s, Sought& x, int tid, F count)
+template <int T, typename F>
+__device__ __forceinline__ void narrow(Lds<T>& s, Sought& x, int tid, F count)
 {
+    constexpr int B = kBins / T;  // of a thread
     const int low = x.low == 32 ? 21 : (x.low == 21 ? 10 : 0), bins = 1 << (x.low - low);
     const int lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < bins; i += kThreads) s.bin[i] = 0;
+    for (int i = tid; i < bins; i += T) s.bin[i] = 0;
     __syncthreads();
     count([&](uint32_t key) {
         if (x.low == 32 || key >> x.low == x.top >> x.low) atomicAdd(&s.bin[key >> low & (uint32_t)(bins - 1)], 1u);
     });
     __syncthreads();
-    // thread i has the bins 2 i and 2 i + 1 from the top
-    const uint32_t n0 = 2 * tid < bins ? s.bin[bins - 1 - 2 * tid] : 0, n1 = 2 * tid < bins ? s.bin[bins - 2 - 2 * tid] : 0;
+    // thread i has the bins B i .. B i + B - 1 from the top
+    uint32_t n[B];
+    int mine = 0;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+        n[b] = B * tid < bins ? s.bin[bins - 1 - B * tid - b] : 0;
+        mine += (int)n[b];
+    }
     int all;
-    int before = wave_before((int)(n0 + n1), all);
+    int before = wave_before(mine, all);
     if (lane == 0) s.wave[0][wave] = all;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) before += w < wave ? s.wave[0][w] : 0;
-    const uint32_t run = (uint32_t)before, left = (uint32_t)x.left;
-    if (run < left && run + n0 + n1 >= left) {
-        const bool one = run + n0 >= left;
-        s.found[0] = (uint32_t)(bins - 1 - 2 * tid - (one ? 0 : 1)) << low;
-        s.found[1] = left - run - (one ? 0 : n0);
-        s.found[2] = one ? n0 : n1;
+    for (int w = 0; w < T / 64; ++w) before += w < wave ? s.wave[0][w] : 0;
+    uint32_t run = (uint32_t)before;
+    const uint32_t left = (uint32_t)x.left;
+    if (run < left && run + (uint32_t)mine >= left) {
+        bool open = true;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (open && run + n[b] >= left) {
+                s.found[0] = (uint32_t)(bins - 1 - B * tid - b) << low;
+                s.found[1] = left - run;
+                s.found[2] = n[b];
+                open = false;
+            }
+            run += n[b];
+        }
     }
     __syncthreads();
     x.top |= s.found[0];
@@ -195,7 +211,8 @@ struct Flags {
     uint32_t same, stays;  // bit e
 };
 
-__device__ __forceinline__ Flags flags_of(Lds& s, const Head& h, const Each& v, const Sought& x, int equal, int tid)
+template <int T>
+__device__ __forceinline__ Flags flags_of(Lds<T>& s, const Head& h, const Each& v, const Sought& x, int equal, int tid)
 {
     const int lane = tid & 63, wave = tid >> 6;
     Flags f = {0, 0};
@@ -220,7 +237,7 @@ __device__ __forceinline__ Flags flags_of(Lds& s, const Head& h, const Each& v, 
     if (lane == 0) s.wave[0][wave] = all;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) equal += w < wave ? s.wave[0][w] : 0;
+    for (int w = 0; w < T / 64; ++w) equal += w < wave ? s.wave[0][w] : 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int t = equal + ties[e / 4] + __popc(f.same >> (e & ~3) & ((1u << (e & 3)) - 1));
@@ -233,7 +250,8 @@ __device__ __forceinline__ Flags flags_of(Lds& s, const Head& h, const Each& v, 
 struct Ranks {
     int before[kEach / 4], all;
 
-    __device__ __forceinline__ Ranks(Lds& s, uint32_t is, int tid)
+    template <int T>
+    __device__ __forceinline__ Ranks(Lds<T>& s, uint32_t is, int tid)
     {
         const int lane = tid & 63, wave = tid >> 6;
         int mine = 0;
@@ -248,7 +266,7 @@ struct Ranks {
         int ahead = 0;
         all = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < T / 64; ++w) {
             const int n = s.wave[1][w];
             ahead += w < wave ? n : 0;
             all += n;
@@ -269,23 +287,30 @@ struct Ranks {
 // ---------------------------------------------------------------------------
 // Heads of up to kSpan positions, a workgroup each, the positions in registers.  The
 // keep-th largest weight is found by counting digits of 11, 11 and 10 bits; then holes and
-// sources are ranked in order and joined through LDS.  grid nkv * n_seqs, block 1024.
+// sources are ranked in order and joined through LDS.  grid nkv * n_seqs, block T.
 //
-// Bound by latency: one reading, and a barrier after each of some fifteen steps; 11 us for
+// Bound by latency: one reading, and a barrier after each of some fifteen steps; 9.4 us for
 // 64 heads of 1025, 15.4 for 256 of up to 8192.  Counting stops where all that share the
 // digits so far stay.  Read from memory once a digit the latter took 5 us more.
-__global__ __launch_bounds__(kThreads) void k_evict_choose(PagedEvict a)
+//
+// T is 512 where that takes sequences of the batch's bounds, up to 4096: fewer waves meet at a
+// barrier, and two workgroups share a CU.  An eviction and its reading back, 64 heads of 1025
+// cut by one 27.6 us so and 28.6 with 1024; 512 heads of 4000 cut down to 40 29.2 and 34.6
+// (256 threads, up to 2048: 28.0 the first).
+template <int T>
+__global__ __launch_bounds__(T) void k_evict_choose(PagedEvict a)
 {
-    __shared__ Lds lds;
-    __shared__ int s_source[kSpan / 2], s_token[kSpan / 2];  // of the positions that move: where, and what lies there
-    __shared__ float s_weight[kSpan / 2];
+    constexpr int kMoves = kEach * T / 2;
+    __shared__ Lds<T> lds;
+    __shared__ int s_source[kMoves], s_token[kMoves];  // of the positions that move: where, and what lies there
+    __shared__ float s_weight[kMoves];
     const int tid = threadIdx.x;
     const int s = (int)(blockIdx.x / (unsigned)a.c.nkv);
     const Cut cut = cut_of(a, s, a.filled, a.shift);
     if (!cut.ok) return;
     const Head h(a, cut, blockIdx.x);
     if (h.keep == h.len) {
-        for (int j = tid; j < h.len; j += kThreads) h.put(j, j);
+        for (int j = tid; j < h.len; j += T) h.put(j, j);
         return;
     }
     if (h.keep == 0) return;
@@ -388,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void k_evict_count(PagedEvict a)
 
 __global__ __launch_bounds__(kThreads) void k_evict_collect(PagedEvict a)
 {
-    __shared__ Lds lds;
+    __shared__ Lds<> lds;
     __shared__ int s_above, s_count;
     const int tid = threadIdx.x;
     const Span p = span_of(a);
@@ -453,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void k_evict_collect(PagedEvict a)
 
 __global__ __launch_bounds__(kThreads) void k_evict_rank(PagedEvict a)
 {
-    __shared__ Lds lds;
+    __shared__ Lds<> lds;
     __shared__ int s_ahead[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Span p = span_of(a);
@@ -652,7 +677,8 @@ hipError_t launch_paged_evict(const PagedEvict& a, hipStream_t st)
         hipLaunchKernelGGL(k_evict_rank, spans, dim3(kThreads), 0, st, a);
         hipLaunchKernelGGL(k_evict_move<true>, move, dim3(256), 0, st, a, blocks);
     } else {
-        if (a.spans) hipLaunchKernelGGL(k_evict_choose, dim3(heads), dim3(kThreads), 0, st, a);
+        if (a.c.cap > kSpan / 2) hipLaunchKernelGGL(k_evict_choose<kThreads>, dim3(heads), dim3(kThreads), 0, st, a);
+        else if (a.spans) hipLaunchKernelGGL(k_evict_choose<kThreads / 2>, dim3(heads), dim3(kThreads / 2), 0, st, a);
         hipLaunchKernelGGL(k_evict_move<false>, move, dim3(256), 0, st, a, blocks);
     }
     return hipGetLastError();

@@ -320,6 +320,10 @@ EVICTS = [
     (2, 32, 256, [9000, 20001, 0, 8200], [-1, 0, 5, 9000], 10, 7, True),
     (1, 16, 128, [50000], [49999], 3, 1000, True),
     (1, 16, 128, [40000, 40000], [8193, 33000], 20000, 9000, False),
+    # both sizes of the workgroups that hold a head: the most of each, and one more than the smaller's
+    (2, 32, 64, [8192, 4097, 8191, 40], [4096, 2049, 1, 8], 4, 50, True),
+    (2, 48, 32, [4096, 4095, 3], [2048, 4094, 1], 4, 50, True),
+    (1, 16, 128, [4097, 4096], [4096, 2048], 0, 0, False),
 ]
 
 
