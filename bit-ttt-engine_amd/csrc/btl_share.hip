@@ -3,11 +3,11 @@
 //
 // Kernels: those of btl_paged_attn.hpp in their forms for a prefix, for the sequences
 // beside it and for scores that are kept, and
-//   k_share          these forms side by side in one launch.
-//   k_share_merge    a row's parts joined.
-//   k_account_tile   the weights of 256 positions from many rows.
-//   k_account_sum    the weights from the token form's scores, or from the shares of rows.
-//   k_share_finish   the merge and the weights from scores in one launch.
+//   k_share, k_share_tiles      these forms side by side in one launch.
+//   k_share_merge               a row's parts joined.
+//   k_account_tile              the weights of 256 positions from many rows.
+//   k_account_sum               the weights from the token form's scores, or from the shares of rows.
+//   k_share_finish              the merge and the weights from scores in one launch.
 //
 // A prefix is a batch of its own: lists of rows, each of which sees every position of its
 // list's pages.  Its rows' softmax parts lie beside their sequences' own, and one merge
@@ -28,7 +28,7 @@ namespace btl {
 // lists of rows over the prefix (token form, or tile form), then sequences over their own
 // positions (tile form, token form).  The tiles are bound by the vector unit and the
 // tokens by the cache's bytes, and two workgroups a CU is what either's registers allow.
-// Tiles of 128 rows, which fill all of them, have launches of their own.
+// Tiles of 128 rows, which fill all of them, have a launch of their own.
 //
 // Times by trace, 32 heads over 8 of 128.  64 tokens behind 8192 positions, own ones up to
 // 700, bf16: 34.7 us, vector unit busy 51 %, matrix units 15 %: one prefix tile a CU waits
@@ -36,8 +36,7 @@ namespace btl {
 // positions, scores kept, bf16: 87.3 us where the form without scores takes 75.4; with 4
 // heads a KV head the scores are 16 bytes a position beside the cache's 272, put out a step
 // late, behind the next step's loads (without that 98).  4 tokens behind 515, f32: 8.1 us,
-// latency.  In tiles of 128 rows, 12 times up to 130 rows behind 16001: 270 GFLOP in 396 us,
-// 680 TFLOP/s; vector unit busy 64 %, matrix units 33 %, no LDS bank conflicts.
+// latency.
 namespace {
 
 struct ShareArgs {
@@ -66,6 +65,25 @@ __global__ __launch_bounds__(256, 2) void k_share(ShareArgs, unsigned prefix_tok
     block -= prefix_tile;
     if (block < own_tile) return paged_tile<DT, 1, BF, kOwn>(kernel_args<ShareArgs>().a, block, tile);
     paged_tok<DT, NW, BF, SCORED ? kScored : kOwn>(kernel_args<ShareArgs>().a, block - own_tile, tok);
+}
+
+// k_share_tiles
+// Tiles of 128 rows, of lists and of sequences: the sequences' short ones fill the end of
+// the prefix's (12 times up to 130 rows behind 16001, 32 heads over 8 of 128: 404 us in a
+// launch each, 388 so).  With the tokens beside them a register spills.
+//
+// Bound by the vector unit (softmax, widening), which is busy for 64 % of that time beside
+// the matrix units' 33 %; no LDS bank conflicts; 270 GFLOP, some 700 TFLOP/s.
+template <int DT>
+__global__ __launch_bounds__(256, 2) void k_share_tiles(ShareArgs, unsigned prefix_tile)
+{
+    constexpr int kK = 2 * 4 * (2 * ((DT + 3) / 4)) * 64, kV = 2 * DT * 2 * 64;  // fragments of k and v
+    __shared__ __align__(16) uint8_t s[16 * (kK + kV) + 4 * (2 * 64 + 2 * 64 + 2)];
+    uint8_t* const sf = s + 16 * (kK + kV);
+    const TileLds<DT> tile = {(h8(*)[4][2 * ((DT + 3) / 4)][64])s, (h8(*)[DT][2][64])(s + 16 * kK), (float(*)[64])sf,
+                              (float(*)[64])(sf + 512), (float*)(sf + 1024)};
+    if (blockIdx.x < prefix_tile) return paged_tile<DT, 2, true, kPrefix>(kernel_args<ShareArgs>().p, blockIdx.x, tile);
+    paged_tile<DT, 2, true, kOwn>(kernel_args<ShareArgs>().a, blockIdx.x - prefix_tile, tile);
 }
 
 // ---------------------------------------------------------------------------
@@ -535,8 +553,8 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
         } else {
             // Chunks so that there are about 256 workgroups, one a CU beside the sequences' own (64
             // tokens behind 8192 positions: 42.4 us, 48.5 with 192, 48.9 with 512, 58.9 with 1024);
-            // of many tiles 2048, as long as a chunk has 2048 positions (12 questions behind 16001:
-            // 406 us, 433 with 1024, 626 with one chunk).
+            // of many tiles 2048, as long as a chunk has 2048 positions (12 times up to 130 rows behind
+            // 16001: 388 us; chunks of 1024 470, of 8192 495).
             const int64_t per = (per_list + r.tile_rows - 1) / r.tile_rows;
             r.tiles = (int)std::min<int64_t>((int64_t)g.n_seqs * per, (int64_t)g.rows * group / r.tile_rows + g.n_seqs);
             const int64_t base = (int64_t)r.tiles * g.nkv;
@@ -578,8 +596,8 @@ static hipError_t launch_share(const PagedShare& a, hipStream_t st)
     args.p.p = a.gp;
     if constexpr (BF) {
         if (a.p.tile_rows == 128) {
-            if (prefix_tile) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kPrefix>), dim3(prefix_tile), dim3(256), 0, st, args.p);
-            if (own_tile) hipLaunchKernelGGL((k_paged_tile<DT, 2, BF, kOwn>), dim3(own_tile), dim3(256), 0, st, a);
+            if (prefix_tile + own_tile)
+                hipLaunchKernelGGL((k_share_tiles<DT>), dim3(prefix_tile + own_tile), dim3(256), 0, st, args, prefix_tile);
             prefix_tile = own_tile = 0;
         }
     }
