@@ -478,10 +478,17 @@ __device__ __forceinline__ void account_sum(const PagedShare& a, unsigned block)
             }
         }
     } else {
-        for (int x = 0; x < a.splits; ++x) {
-            const f4 y = *(const f4*)(a.sums + ((int64_t)x * c.n_seqs * c.nkv + head) * a.score_ld + key);
+        constexpr int V = 8;  // shares at a time
+        const float* from = a.sums + head * a.score_ld + key;
+        const int64_t step = (int64_t)c.n_seqs * c.nkv * a.score_ld;
+        for (int x0 = 0; x0 < a.splits; x0 += V) {
+            f4 y[V];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = __fadd_rn(w[e], y[e]);
+            for (int u = 0; u < V; ++u) y[u] = *(const f4*)(from + min(x0 + u, a.splits - 1) * step);
+#pragma unroll
+            for (int u = 0; u < V; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = x0 + u < a.splits ? __fadd_rn(w[e], y[u][e]) : w[e];
         }
     }
     if (four && key + 4 <= seen) {
