@@ -5,6 +5,7 @@
 // beside it and for scores that are kept, and
 //   k_share, k_share_tiles      these forms side by side in one launch.
 //   k_share_merge               a row's parts joined.
+//   k_share_ml                  their maxima and sums alone.
 //   k_account_tile              the weights of 256 positions from many rows.
 //   k_account_sum               the weights from the token form's scores, or from the shares of rows.
 //   k_share_finish              the merge and the weights from scores in one launch.
@@ -98,7 +99,26 @@ __global__ __launch_bounds__(256, 2) void k_share_tiles(ShareArgs, unsigned pref
 // 4 KB a row and head: 1025 rows of 32 heads 24 us.
 namespace {
 
-template <int N, int U, bool BF>
+// The maximum and the sum of row r from its n parts, at most U of them.
+template <int U>
+__device__ __forceinline__ float2 joined(const PagedShare& a, int64_t r, int n, const Behind& p)
+{
+    float2 part[U ? U : 1];
+    float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (int y = 0; y < U; ++y)
+        if (y < n) {
+            part[y] = *(const float2*)(a.part_ml + 2 * (r * a.parts + (y < p.parts ? y : a.own0 - p.parts + y)));
+            top = fmaxf(top, part[y].x);
+        }
+#pragma unroll
+    for (int y = 0; y < U; ++y)
+        if (y < n) sum = __fmaf_rn(__builtin_amdgcn_exp2f(__fsub_rn(part[y].x, top)), part[y].y, sum);
+    return make_float2(top, p.lost ? __builtin_nanf("") : sum);
+}
+
+// ML: the row's maximum and sum are put out where they are wanted
+template <int N, int U, bool BF, bool ML = true>
 __device__ __forceinline__ void share_merge(const PagedShare& a, int t, int block)
 {
     const Paged& c = a.c;
@@ -149,7 +169,7 @@ __device__ __forceinline__ void share_merge(const PagedShare& a, int t, int bloc
                 for (int e = 0; e < 4; ++e) v[e] = __fmaf_rn(b, o[y][e], v[e]);
             }
         if (p.lost) sum = __builtin_nanf("");
-        if (a.ml && d == 0) *(float2*)(a.ml + 2 * r) = make_float2(top, sum);
+        if (ML && a.ml && d == 0) *(float2*)(a.ml + 2 * r) = make_float2(top, sum);
         if (d < hd) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], sum);
@@ -164,6 +184,36 @@ template <int N, int U, bool BF>
 __global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
 {
     share_merge<N, U, BF>(a, blockIdx.x, blockIdx.y);
+}
+
+// ---------------------------------------------------------------------------
+// k_share_ml
+// ---------------------------------------------------------------------------
+// The rows' maxima and sums alone, as k_share_merge forms them, so that k_account_tile need
+// not wait for their outputs, which are joined in its launch.  A wave a row, a head a lane.
+// grid ceil(rows / 4), block 256.
+//
+// Bound by latency: 4.7 us for 1000 rows of 32 heads, where the whole merge takes 11.4.  With
+// the weights 169.0 us in all before, 166.2 so; 14 sequences of few or 201 rows 44.6 and 43.3.
+template <int U>
+__global__ __launch_bounds__(256) void k_share_ml(PagedShare a)
+{
+    const Paged& c = a.c;
+    const int lane = threadIdx.x & 63, t = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (t >= c.rows) return;
+    const int s = find_seq(c, t, lane);
+    if (s < 0 || s >= c.n_seqs) return;
+    const Seq q = seq_at(c, s);
+    const Behind p = behind(a, t, lane);
+    const int i = t - q.a;
+    if (i < 0 || i >= q.n || !q.ok) return;
+    const int C = (int64_t)q.n * a.group > a.p.lo ? a.p.tile_c : a.p.tok_c;
+    if (whole_of<kOwn>(a, q.p0 + q.n, C)) return;  // put out by its one chunk
+    const int nc = p.parts + (q.p0 + i) / C + 1;
+    for (int head = lane; head < a.nh; head += 64) {
+        const int64_t r = (int64_t)t * a.nh + head;
+        *(float2*)(a.ml + 2 * r) = joined<U>(a, r, nc, p);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -185,7 +235,8 @@ __global__ __launch_bounds__(256) void k_share_merge(PagedShare a)
 // in a row some 45 us so, 61 with rows read when they are wanted, 78 at two workgroups.  Keys
 // in LDS and rows in registers would need the sums across rows at every step, not at the end.
 //
-// grid nkv * ceil(cap / 256) * splits * n_seqs, block 256.
+// grid nkv * ceil(cap / 256) * splits * n_seqs, block 256; behind them, where k_share_ml has
+// put out the rows' maxima and sums, the merges of rows of at most 8 parts.
 namespace {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -227,7 +278,7 @@ __device__ __forceinline__ void put_weight(const PagedShare& a, const Seq& q, in
 }  // namespace
 
 template <int DT, bool BF>
-__global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a)
+__global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a, unsigned blocks_of_keys)
 {
     constexpr int NJ = (DT + 3) / 4;
     constexpr int PARTS = BF ? 1 : 2;
@@ -236,6 +287,10 @@ __global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a)
     __shared__ float s_unit[2][4][BF ? 1 : 16];  // the unit of its products
     __shared__ int s_bad[2][4];       // a tile has rows that came back as NaN
     const Paged& c = a.c;
+    if (blockIdx.x >= blocks_of_keys) {
+        const unsigned block = blockIdx.x - blocks_of_keys;
+        return share_merge<1, 8, BF, false>(a, (int)(block % (unsigned)c.rows), (int)(block / (unsigned)c.rows));
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15, hd = c.hd, ndt = hd >> 4;
     // workgroup -> head, block of 256 positions, share of the rows, sequence
@@ -433,19 +488,7 @@ __device__ __forceinline__ void account_sum(const PagedShare& a, unsigned block)
             if (whole) {
                 ml = *(const float2*)(a.ml + 2 * r);
             } else {
-                const int n = p.parts + (q.p0 + i) / a.p.tok_c + 1;
-                float2 part[U ? U : 1];
-                float top = -__builtin_inff(), sum = 0.0f;
-#pragma unroll
-                for (int y = 0; y < U; ++y)
-                    if (y < n) {
-                        part[y] = *(const float2*)(a.part_ml + 2 * (r * a.parts + (y < p.parts ? y : a.own0 - p.parts + y)));
-                        top = fmaxf(top, part[y].x);
-                    }
-#pragma unroll
-                for (int y = 0; y < U; ++y)
-                    if (y < n) sum = __fmaf_rn(__builtin_amdgcn_exp2f(__fsub_rn(part[y].x, top)), part[y].y, sum);
-                ml = make_float2(top, p.lost ? __builtin_nanf("") : sum);
+                ml = joined<U>(a, r, p.parts + (q.p0 + i) / a.p.tok_c + 1, p);
             }
             // a row that came back as NaN adds nothing
             const bool good = ml.y > 0.0f && ml.y < __builtin_inff();
@@ -626,7 +669,11 @@ static hipError_t launch_share(const PagedShare& a, hipStream_t st)
         else hipLaunchKernelGGL((k_share_finish<8, BF>), dim3(merge + sums), dim3(256), 0, st, a, merge);
         return hipGetLastError();
     }
-    if (a.parts > 16)
+    const int64_t keys = (int64_t)heads * ((a.c.cap + 255) / 256) * a.splits, merges = (int64_t)one.x * one.y;
+    const bool beside = account && tiles && a.parts > 1 && a.parts <= 8 && keys + merges < (int64_t)1 << 24;
+    if (beside)
+        hipLaunchKernelGGL(k_share_ml<8>, dim3((unsigned)(a.c.rows + 3) / 4), dim3(256), 0, st, a);
+    else if (a.parts > 16)
         hipLaunchKernelGGL((k_paged_merge<4, BF, kOwn>), dim3((unsigned)a.c.rows, (unsigned)a.nh), dim3(256), 0, st, a);
     else if (a.parts > 8)
         hipLaunchKernelGGL((k_share_merge<1, 16, BF>), one, dim3(256), 0, st, a);
@@ -636,7 +683,8 @@ static hipError_t launch_share(const PagedShare& a, hipStream_t st)
         hipLaunchKernelGGL((k_share_merge<1, 8, BF>), one, dim3(256), 0, st, a);
     if (account) {
         if (tiles)
-            hipLaunchKernelGGL((k_account_tile<DT, BF>), dim3(heads * ((a.c.cap + 255) / 256) * a.splits), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((k_account_tile<DT, BF>), dim3((unsigned)(keys + (beside ? merges : 0))), dim3(256), 0, st, a,
+                               (unsigned)keys);
         if (a.scored || a.splits > 1) hipLaunchKernelGGL(k_account_sum, dim3(sums), dim3(256), 0, st, a);
     }
     return hipGetLastError();

@@ -165,6 +165,11 @@ ACCOUNTS = [
     (4, 2, 32, 64, [(2, 3100), (1, 7)], []),                   # of two rows, and of some
     (32, 8, 128, 64, [(390, 300), (20, 0)], [(0, 390, 150)]),  # tiles of 128 rows in bf16
     (15, 1, 112, 16, [(1, 200), (1, 0), (3, 64)], [(0, 2, 100)]),  # groups of 15
+    # many rows, whose merges wait for nothing: of up to 8 chunks, up to 16, more
+    (8, 2, 64, 64, [(40, 1500), (1, 33)], []),
+    (8, 2, 64, 64, [(40, 2400), (1, 33)], []),
+    (8, 2, 64, 64, [(40, 5000), (1, 33)], []),
+    (80, 5, 16, 16, [(2, 700), (3, 10), (0, 9), (1, 600)], [(0, 5, 20)]),  # more heads than a wave has lanes
 ]
 
 
