@@ -622,3 +622,68 @@ def test_calls_on_a_stream_and_in_two_graphs_of_one_workspace():
                     within(host(a.weight[s, :, :at + 1]), w[s], wb[s] + cref.U * w[s])
                 assert (a.weight[:, :, at + 1:] == 0).all()
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_captured_step_whose_rows_change_hands(dtype):
+    """Attention with weights behind a prefix and the eviction after it in one graph: between its
+    replays rows go from one sequence to another, so that each is once of many rows, of few and of
+    none, and lists end elsewhere."""
+    nh, nkv, hd, ps, rows, keep = 8, 2, 64, 32, 60, 150
+    rng = np.random.default_rng(77)
+    table, n_own = ref.pages_for([(60, 400)] * 3, ps, rng, wide_extra=0)
+    ptable = np.arange(n_own, n_own + 16, dtype=np.int32).reshape(2, 8)
+    cache = ref.rand_cache(rng, n_own + 16, nkv, ps, hd)
+    gpu, fresh = on_gpu(cache), [dev(x) for x in cache]
+    q = dev(rng.standard_normal((rows, nh * hd)).astype(np.float32), DT[dtype])
+    start, pos = dev(np.array([0, 20, 40, 60], np.int32)), dev(np.zeros(3, np.int32))
+    p_start, p_pos = dev(np.array([0, 30, 60], np.int32)), dev(np.zeros(2, np.int32))
+    batch = bl.PagedBatch(start, pos, dev(table), rows, 60, 460)
+    prefix = bl.PagedBatch(p_start, p_pos, dev(ptable), rows, 60, 250)
+    account, left = bl.KVAccount(3, nkv, 460, DEV), bl.KVAccount(3, nkv, 460, DEV)
+    out, held = torch.empty_like(q), dev(np.zeros(3, np.int32))
+    recent = dev(np.full(3, 10, np.int32))
+    keeps = dev(np.full(3, keep, np.int32))
+    space = bl.paged_attention_account_workspace(gpu, batch, nh, prefix=prefix)
+    more = bl.paged_evict_workspace(gpu, batch)
+
+    def step():
+        bl.paged_attention_account(q, gpu, batch, account, prefix=prefix, out=out, workspace=space)
+        bl.paged_evict(gpu, batch, account, keeps, recent=recent, max_keep=keep, out=left, held=held, workspace=more)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for starts, at, p_starts, p_at in (([0, 20, 40, 60], [0, 100, 400], [0, 30, 60], [250, 3]),
+                                       ([0, 57, 58, 60], [300, 400, 0], [0, 1, 59], [64, 250]),
+                                       ([0, 0, 1, 60], [222, 399, 90], [0, 0, 60], [250, 100]),
+                                       ([0, 60, 60, 60], [400, 149, 151], [10, 20, 50], [0, 250]),
+                                       ([0, 20, 40, 60], [0, 100, 400], [0, 30, 60], [250, 3])):
+        for x, y in zip((start, pos, p_start, p_pos), (starts, at, p_starts, p_at)):
+            x.copy_(dev(np.array(y, np.int32)))
+        for x, y in zip((gpu.k, gpu.v, gpu.k_scale, gpu.v_scale), fresh):
+            x.copy_(y)
+        account.weight.fill_(0.25)
+        graph.replay()
+        sizes = [(b - a, p) for a, b, p in zip(starts, starts[1:], at)]
+        lists = [(a, b - a, p) for a, b, p in zip(p_starts, p_starts[1:], p_at)]
+        want, bound, w, wb = cref.attention(host(q).reshape(rows, nh, hd), cache, table, sizes, starts, dtype == "bf16", lists,
+                                            ptable)
+        within(host(out).reshape(rows, nh, hd), want, bound)
+        for s, (r, p) in enumerate(sizes):
+            if r:
+                w[s][:, :p] += 0.25
+                within(host(account.weight[s, :, :r + p]), w[s], wb[s] + cref.U * w[s])
+                assert (account.weight[s, :, r + p:] == 0.25).all()
+            else:
+                assert (account.weight[s] == 0.25).all()
+        arrays = [x.cpu().numpy() for x in (account.weight, account.token, account.filled, account.shift)]
+        want_cache, kept, want_held = cref.evict(cache, table, [r + p for r, p in sizes], arrays, [keep] * 3, [0] * 3, [10] * 3)
+        assert held.tolist() == want_held
+        for name, g, x in zip(("k", "v", "k scale", "v scale"), (gpu.k, gpu.v, gpu.k_scale, gpu.v_scale), want_cache):
+            same_bits(g.cpu().numpy(), x, name)
+        for s, n in enumerate(want_held):
+            same_bits(left.weight[s, :, :n].cpu().numpy(), kept[0][s, :, :n], "weights")
+            same_bits(left.token[s, :, :n].cpu().numpy(), kept[1][s, :, :n], "tokens")
