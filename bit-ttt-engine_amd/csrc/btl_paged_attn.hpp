@@ -865,7 +865,11 @@ __device__ __forceinline__ void paged_tile(const PagedArgs<MODE>& a, unsigned bl
     const bool whole = whole_of<MODE>(z, sees<MODE>(q, q.n - 1), C);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        const float l = xor16_sum(r[u].l), unit = r[u].unit();
+        float l = xor16_sum(r[u].l);
+        const float unit = r[u].unit();
+        // a value scale that is not finite makes all of a row's values NaN, but is in no score:
+        // its sum says so too, to whoever adds up its weights
+        if (MODE != kPlain && r[u].o[0].x != r[u].o[0].x) l = __builtin_nanf("");
         int m = m_wave + 16 * u + n;
         asm("" : "+v"(m));
         const int i = row_of(a, m);
