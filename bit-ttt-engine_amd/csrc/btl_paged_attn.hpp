@@ -556,10 +556,12 @@ __device__ __forceinline__ void paged_tok(const PagedArgs<MODE>& a, unsigned blo
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const h8 k0 = widen8(kw[t][j].x, kw[t][j].y), k1 = widen8(kw[t][j].z, kw[t][j].w);
+                // Where k_account_tile may make these scores again, they are added up in its order:
+                // sums of another would be apart by roundings, which of large scores are any number.
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qs.v[p][0][2 * j], sc[t], 0, 0, 0);
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qs.v[p][0][2 * j + 1], sc[t], 0, 0, 0);
+                for (int x = 0; x < 2 * PARTS; ++x) {
+                    const int p = MODE == kPlain ? x >> 1 : x % PARTS, half = MODE == kPlain ? x & 1 : x / PARTS;
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(half ? k1 : k0, qs.v[p][0][2 * j + half], sc[t], 0, 0, 0);
                 }
             }
             // NaN where the page is outside the pool or a scale is not finite: an infinite one

@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a, 
     __syncthreads();
     for (int step = step0, b = 0; step < step1; ++step, b ^= 1) {
         if (step + 1 < step1) fetch(step + 1);
-        // the scores of tile u, less the row's largest, in the roundings of the attention
+        // the scores of tile u, less the row's largest, in the order and the roundings of the attention
         auto scores = [&](int u, float top, f4* sc) {
             const float unit = BF ? 1.0f / kCodeDown : s_unit[b][u][BF ? 0 : n];
 #pragma unroll
