@@ -127,7 +127,7 @@ int btl_paged_read(const btl_kv_paged_t* cache, const btl_paged_batch_t* batch, 
  * reads KV head h / (n_heads / n_kv), n_heads / n_kv <= 16.
  * Arithmetic: the codes are exact in the matrix instructions' f16; queries and
  * softmax weights are taken in two f16 parts (22 bits) for BTL_F32; for BTL_BF16
- * queries in one (exact), weights in two for sequences of at most 16 rows times
+ * queries in one (exact down to 2^-31 of the row's largest), weights in two for sequences of at most 16 rows times
  * heads of a group and in one (11 bits) for longer ones (for a single sequence
  * max_rows decides it); products are summed in f32, the softmax's maxima, sums and
  * outputs are f32.  Powers of two keep the parts in f16's range: one a row, by its
@@ -199,6 +199,9 @@ typedef struct btl_kv_account {
  * call's rows begins with it).  Only account->weight is used.  Nothing is done for
  * positions that no row sees, for sequences without rows and for refused ones; a row
  * that comes back as NaN adds nothing.  Sums are f32, in an order that the sizes fix.
+ * The scores are the attention's, or made again from the same numbers in the same order,
+ * for BTL_BF16 from the queries as they are: of a row whose scores come from queries below
+ * 2^-31 of its largest alone, and are above some 2^6, the weights are then no softmax's.
  * ws: btl_paged_attention_account_workspace_bytes (or NULL: the library's).
  */
 size_t btl_paged_attention_account_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,

@@ -40,3 +40,25 @@ def test_scores_of_any_size_that_are_not_kept(size, dtype, hd, sizes):
         assert np.abs(w.sum(axis=1) - n).max() <= n * (2 * (p + r) + n + 8) * cref.U
         if size >= 1e12:  # every softmax is one key's
             assert (np.abs(w - np.rint(w)) <= n * 8 * cref.U).all()
+
+
+@pytest.mark.parametrize("rows,far,dtype", [(1, 0, "f32"), (4, FAR, "f32"), (40, 0, "f32"), (400, 0, "f32"), (1, 0, "bf16")])
+def test_queries_far_below_one_that_meets_only_zeros(rows, far, dtype):
+    """The attention scales a row by its largest query and loses bits of those far below it.  Where that one
+    meets zeros alone, the scores are what is lost: weights then are some softmax's, each at most 1."""
+    nh, nkv, hd, ps, pos = 16, 4, 64, 16, 100
+    rng = np.random.default_rng(43)
+    table, n_pages = ref.pages_for([(rows, pos)], ps, rng)
+    table = np.concatenate([table, np.full((1, max(1, far // ps - table.shape[1])), -1, np.int32)], axis=1)
+    cache = ref.rand_cache(rng, n_pages, nkv, ps, hd)
+    cache[0][..., 5] = 128
+    batch, _ = batch_of(table, [(rows, pos)], max_len=far or None)
+    q = (rng.standard_normal((rows, nh, hd)) * 2.0 ** 40).astype(np.float32)
+    q[..., 5] = 2.0 ** 90
+    ld = far or rows + pos
+    account = bl.KVAccount.of(torch.zeros((1, nkv, ld), device=DEV))
+    out = host(bl.paged_attention_account(dev(q.reshape(rows, -1), DT[dtype]), on_gpu(cache), batch, account))
+    assert np.isfinite(out).all()
+    w = host(account.weight[0, :, :pos + rows])
+    n = rows * nh // nkv
+    assert np.isfinite(w).all() and (w >= 0).all() and (w <= n * (1 + n * cref.U)).all()
