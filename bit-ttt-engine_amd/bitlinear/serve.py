@@ -16,11 +16,13 @@ layers/attention.rs:149-239, model/llama.rs:496-530 (the pick at a temperature).
 
 Behind a prompt that all of them share, and within a budget of positions:
 
-    prefix = PagedBatch([0, rows], [prompt], prompt_pages, rows, rows, prompt)   # lists of rows and their pages
+    # lists of rows, what they share and its pages: here one list of all rows (int32 tensors, as row_start, pos and pages)
+    prefix = PagedBatch(list_start, prompt_len, prompt_pages, rows, rows, prompt)
     account = KVAccount(n_seqs, n_kv_heads, max_len, "cuda", shift=prompt)       # one a layer
     q = paged_rope_append(q, k, v, cache, batch, rope_cos, rope_sin, rope_shift=account.shift)
     o = paged_attention_account(q, cache, batch, account, prefix=prefix)
-    held = paged_evict(cache, batch, account, keep=2048, recent=256)             # pos of the next rows
+    held = paged_evict(cache, batch, account, keep=2048, recent=256)
+    pos.copy_(held)                                                              # of the next rows
 """
 import ctypes
 import functools

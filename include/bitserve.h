@@ -223,7 +223,8 @@ int btl_paged_attention_account(const void* q, int dtype, int64_t n_heads, const
  * recent may be NULL (0).  max_keep: the host's bound on what a sequence is cut down to.
  * account_out (NULL: account itself): weight and token of the positions that are held,
  * filled = held, shift = shift + len - held; its arrays are account's, or overlap
- * nothing.  held [n_seqs] int32: min(keep, len), the pos of the sequence's next rows; -1
+ * nothing.  held [n_seqs] int32: min(keep, len), the pos of the sequence's next rows, in an
+ * array of its own (the batch's pos is read as long as it is written); -1
  * for a refused sequence (its pos, rows or len out of the batch's bounds, or to be cut down
  * to more than max_keep), whose pages and account stay as they are.  A moved position whose page is
  * outside the pool gets NaN scales; one that would go to such a page is lost.
