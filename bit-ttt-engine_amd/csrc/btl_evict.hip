@@ -81,15 +81,17 @@ struct Head {
     int32_t* token_out;
     int32_t* from;  // [keep]: -1 where a position stays
     int len, keep, filled, shift;
-    int sink, late;  // tokens below and from there on are protected
+    int sink, last;  // tokens below the first and above the second are protected
 
     __device__ __forceinline__ Head(const PagedEvict& a, const Cut& cut, int64_t head)
         : weight(a.weight + head * a.ld), token(a.token + head * a.ld), weight_out(a.weight_out + head * a.ld_out),
           token_out(a.token_out + head * a.ld_out), from(a.from + head * a.c.cap), len(cut.len), keep(cut.keep),
           filled(cut.filled), shift(cut.shift), sink(cut.sink)
     {
-        // tokens are int32, so a bound past them is the bound
-        late = (int)max(min((int64_t)len + shift - cut.recent, (int64_t)INT_MAX), (int64_t)INT_MIN);
+        // the recent ones: a bound past every token leaves none, one at or below the least all
+        const int64_t bound = (int64_t)len + shift - cut.recent;
+        last = bound <= INT_MIN ? INT_MAX - 1 : (int)min(bound - 1, (int64_t)INT_MAX);
+        if (bound <= INT_MIN) sink = INT_MAX;
     }
     __device__ __forceinline__ int in_order(int j) const { return (int)((uint32_t)j + (uint32_t)shift); }
     __device__ __forceinline__ int token_at(int j) const { return j < filled ? token[j] : in_order(j); }
@@ -136,7 +138,7 @@ struct Each {
     // protected positions are above every weight
     __device__ __forceinline__ uint32_t key(const Head& h, int e) const
     {
-        return t[e] < h.sink || t[e] >= h.late ? 0xFFFFFFFFu : order_of(w[e]);
+        return t[e] < h.sink || t[e] > h.last ? 0xFFFFFFFFu : order_of(w[e]);
     }
 };
 

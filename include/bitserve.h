@@ -181,6 +181,7 @@ int btl_paged_attention_prefix(const void* q, int dtype, int64_t n_heads, const 
  *   (its RoPE position) lies at position j: token[s][h][j] for j < filled[s], else
  *   j + shift[s].  A sequence begins with filled = 0 and shift = 0 (the prefix's length
  *   where it has one); btl_paged_evict keeps them.  shift is the rope_shift of its rows.
+ *   Tokens are int32: pos + rows + shift[s] is at most 2^31.
  * ld: positions of a head, at least min(max_len, max_pages * page_size, 2^23).
  */
 typedef struct btl_kv_account {
