@@ -366,6 +366,12 @@ __global__ __launch_bounds__(T) void k_evict_choose(PagedEvict a)
 // head, which goes through its head span by span, took 101 for all three).  A launch between
 // them is the cheapest way to have all spans' counts; a wait inside one kernel would need all
 // its workgroups to be resident.
+//
+// Every workgroup goes through all spans' counts, and through all keys that share the sought
+// one's first digit, up to three times: where many do, the work grows with the square of the
+// head's length.  With the move, weights spread; 95 % of them zero and the cut among those; all
+// of one first digit: 8 heads of 100001 55, 228 and 126 us; 8 of 10^6 0.33, 7.0 and 2.2 ms; one of
+// 2^23 1.1, 62 and 28 ms.
 namespace {
 
 struct Span {

@@ -658,7 +658,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged_tok(PagedArgs<MODE> a)
 // code is widened once a workgroup instead of once a wave.
 //
 // 512 rows over 8192 positions, 32 heads over 8 of 128: 66.6 GFLOP in 114 us in bf16
-// (584 TFLOP/s; a large library product reaches 1116), 192 us in f32, whose two parts
+// (584 TFLOP/s; a large library product reaches 1116 to 1232), 192 us in f32, whose two parts
 // are two products.  Per wave and 64 keys of 32 rows the matrix instructions take 1024
 // cycles, the softmax and the widening some 1900 of the vector unit, on which two waves
 // a SIMD take turns: that, and what is left of LDS latency between them, is the bound.

@@ -34,8 +34,8 @@ namespace btl {
 // Times by trace, 32 heads over 8 of 128.  64 tokens behind 8192 positions, own ones up to
 // 700, bf16: 34.7 us, vector unit busy 51 %, matrix units 15 %: one prefix tile a CU waits
 // for its keys and for LDS, the tokens use its other half.  32 tokens over up to 8192
-// positions, scores kept, bf16: 87.3 us where the form without scores takes 75.4; with 4
-// heads a KV head the scores are 16 bytes a position beside the cache's 272, put out a step
+// positions, scores kept, bf16: 88.0 us where the form without scores takes 75.4; with 4
+// heads a KV head the scores are 16 bytes a position beside the cache's 264, put out a step
 // late, behind the next step's loads (without that 98).  4 tokens behind 515, f32: 8.1 us,
 // latency.
 namespace {
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, 2) void k_share(ShareArgs, unsigned prefix_tok
 // the prefix's (12 times up to 130 rows behind 16001, 32 heads over 8 of 128: 404 us in a
 // launch each, 388 so).  With the tokens beside them a register spills.
 //
-// Bound by the vector unit (softmax, widening), which is busy for 64 % of that time beside
+// Bound by the vector unit (softmax, widening), which is busy for 65 % of that time beside
 // the matrix units' 33 %; no LDS bank conflicts; 270 GFLOP, some 700 TFLOP/s.
 template <int DT>
 __global__ __launch_bounds__(256, 2) void k_share_tiles(ShareArgs, unsigned prefix_tile)
@@ -229,9 +229,9 @@ __global__ __launch_bounds__(256) void k_share_ml(PagedShare a)
 // that no product overflows; of f32 in two f16 parts as the attention takes them.
 //
 // Half the attention's products, no value, and no reference to follow: a fused operation,
-// an exponential and another fused one a score.  Bound by the vector unit (busy 71 %, the
-// matrix units 27 %): 1000 rows over 4099 positions, 32 heads over 8 of 128, bf16, 59 us,
-// 500 TFLOP/s, by trace.  Three workgroups a CU, and rows asked for a step ahead: in passes
+// an exponential and another fused one a score.  Bound by the vector unit (busy 75 %, the
+// matrix units 23 %): 1000 rows over 4099 positions, 32 heads over 8 of 128, bf16, 63 us by
+// trace with the rows' merges beside it, 59 and 500 TFLOP/s without.  Three workgroups a CU, and rows asked for a step ahead: in passes
 // in a row some 45 us so, 61 with rows read when they are wanted, 78 at two workgroups.  Keys
 // in LDS and rows in registers would need the sums across rows at every step, not at the end.
 //
@@ -573,8 +573,9 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
                heads * std::min<int64_t>(kTokRows, c.max_rows * group) * up(longest, 64) <= ((int64_t)1 << 28);
     // Sequences of at most 512 positions, their scores kept and nothing beside them, in one
     // launch of eight waves.  Else four waves.  Beside a prefix, whose tiles fill the chip as
-    // well, chunks for 512 workgroups: 64 sequences of up to 700 52.5 us where btl_serve.hip's
-    // rule takes 59.8, 32 of up to 4000 75.4 and 83.6 (with 256: 52.8 and 80.2; 1024: 60.3 and 77.3).
+    // well, chunks for 512 workgroups: behind 8192 positions 64 sequences of up to 700 40.2 us where
+    // btl_serve.hip's 4096 take 46.8, 32 of up to 4000 60.3 and 72.9 (256: 37.8 and 61.6; 1024: 45.6
+    // and 63.1).
     const bool apart = p.tok_w == 8 && p.tok_n && a.scored && !a.split && !p.tile_n;
     if (!apart) p.tok_w = 4;
     if (!apart && p.tok_n) {
@@ -586,9 +587,10 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
     a.gp = AttnPlan{};
     if (a.split) {
         // One form for all lists: the token form, in tiles of 16 rows, where every list is of at most
-        // two (8 rows of 4 heads behind 4000 positions: 15.7 us, 16.5 in the tile form, in f32 14.8
-        // and 17.2; of three 19.1 and 16.7), in chunks for 256 workgroups (8 sequences behind 16000:
-        // 21.6 us, 24.4 with 192 or 512).
+        // two (8 rows of 4 heads behind 4000 positions: 15.8 us, 16.8 in the tile form, in f32 15.0 and
+        // 17.2).  Of three it would be 16.3 and 17.4, of four 16.4 and 17.9, of five 21.4 and 19.9: the
+        // rule could go up to four.  In chunks for 256 workgroups (8 sequences behind 16000: 21.9 us,
+        // 24.3 with 192, 24.8 with 512).
         AttnPlan& r = a.gp;
         const int64_t far = std::max(g.cap, 1), all = up(far, 256);
         r.tok_w = 4;
@@ -602,9 +604,9 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
             r.tok_n = (int)((far + r.tok_c - 1) / r.tok_c);
         } else {
             // Chunks so that there are about 256 workgroups, one a CU beside the sequences' own (64
-            // tokens behind 8192 positions: 42.4 us, 48.5 with 192, 48.9 with 512, 58.9 with 1024);
+            // tokens behind 8192 positions: 39.9 us, 45.0 with 192, 46.4 with 512, 55.4 with 1024);
             // of many tiles 2048, as long as a chunk has 2048 positions (12 times up to 130 rows behind
-            // 16001: 388 us; chunks of 1024 470, of 8192 495).
+            // 16001: 389 us; chunks of some 1100 430, of 4000 413, of 8000 495).
             const int64_t per = (per_list + r.tile_rows - 1) / r.tile_rows;
             r.tiles = (int)std::min<int64_t>((int64_t)g.n_seqs * per, (int64_t)g.rows * group / r.tile_rows + g.n_seqs);
             const int64_t base = (int64_t)r.tiles * g.nkv;
@@ -625,7 +627,7 @@ bool plan_paged_share(int64_t n_heads, PagedShare& a, bool bf, bool account)
     a.score_rows = (int)std::min<int64_t>(kTokRows, (int64_t)c.max_rows * group);
     a.score_ld = (int)up(c.cap, 64);
     // k_account_tile's rows in shares of at least 256, for some 2048 workgroups: of the sequences
-    // that the bounds allow to be long, few may be (two of 14: 39.8 us, 49.7 for 768).
+    // that the bounds allow to be long, few may be (two of 14: 44.4 us, 49.0 for 768).
     const bool tiles = p.lo != INT_MAX || !a.scored;
     const int64_t seqs = !tiles ? 0 : (a.scored ? std::min<int64_t>(c.n_seqs, (int64_t)c.rows * group / 16 + 1) : c.n_seqs);
     const int64_t keys = (c.cap + 255) / 256, have = std::max<int64_t>(1, seqs * c.nkv * keys);

@@ -229,6 +229,8 @@ int btl_paged_attention_account(const void* q, int dtype, int64_t n_heads, const
  * for a refused sequence (its pos, rows or len out of the batch's bounds, or to be cut down
  * to more than max_keep), whose pages and account stay as they are.  A moved position whose page is
  * outside the pool gets NaN scales; one that would go to such a page is lost.
+ * Heads of far more than 8192 positions that mostly have equal weights take longest, with
+ * the square of their length (2^23 positions, 95 % of them 0: 62 ms, else 1.1).
  * Pages that two sequences share, and in which one has a position below keep that goes,
  * would be written for both: share prefixes by btl_paged_attention_prefix, or keep
  * shared first tokens by sink.
