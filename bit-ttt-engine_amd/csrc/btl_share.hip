@@ -231,9 +231,10 @@ __global__ __launch_bounds__(256) void k_share_ml(PagedShare a)
 // Half the attention's products, no value, and no reference to follow: a fused operation,
 // an exponential and another fused one a score.  Bound by the vector unit (busy 75 %, the
 // matrix units 23 %): 1000 rows over 4099 positions, 32 heads over 8 of 128, bf16, 63 us by
-// trace with the rows' merges beside it, 59 and 500 TFLOP/s without.  Three workgroups a CU, and rows asked for a step ahead: in passes
-// in a row some 45 us so, 61 with rows read when they are wanted, 78 at two workgroups.  Keys
-// in LDS and rows in registers would need the sums across rows at every step, not at the end.
+// trace with the rows' merges beside it, 59 and 500 TFLOP/s without.  Three workgroups a CU, and
+// rows asked for a step ahead: in passes in a row some 45 us so, 61 with rows read when they are
+// wanted, 78 at two workgroups.  Keys in LDS and rows in registers would need the sums across
+// rows at every step, not at the end.
 //
 // grid nkv * ceil(cap / 256) * splits * n_seqs, block 256; behind them, where k_share_ml has
 // put out the rows' maxima and sums, the merges of rows of at most 8 parts.
@@ -449,6 +450,9 @@ __global__ __launch_bounds__(256, BF ? 3 : 2) void k_account_tile(PagedShare a, 
         w = n == x ? v : w;
     }
     if (kb + lane >= seen) return;
+    // at most 1 a row, also where the products hold what the attention's scaled queries lost (bf16 ones
+    // below 2^-31 of their row's largest) and a score is far above all that the row's sum is of
+    w = fminf(w, (float)max(min(64 * (step1 - step0), (int)M - first - 64 * step0), 0));
     if (a.splits == 1) put_weight(a, q, s, h, kb + lane, w);
     else a.sums[(((int64_t)share * c.n_seqs + s) * c.nkv + h) * a.score_ld + kb + lane] = w;
 }

@@ -202,7 +202,8 @@ typedef struct btl_kv_account {
  * that comes back as NaN adds nothing.  Sums are f32, in an order that the sizes fix.
  * The scores are the attention's, or made again from the same numbers in the same order,
  * for BTL_BF16 from the queries as they are: of a row whose scores come from queries below
- * 2^-31 of its largest alone, and are above some 2^6, the weights are then no softmax's.
+ * 2^-31 of its largest alone, and are above some 2^6, the weights are then no softmax's,
+ * but a position's sum is at most 1 for each row and head.
  * ws: btl_paged_attention_account_workspace_bytes (or NULL: the library's).
  */
 size_t btl_paged_attention_account_workspace_bytes(int64_t n_heads, const btl_kv_paged_t* cache,

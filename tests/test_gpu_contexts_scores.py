@@ -42,10 +42,11 @@ def test_scores_of_any_size_that_are_not_kept(size, dtype, hd, sizes):
             assert (np.abs(w - np.rint(w)) <= n * 8 * cref.U).all()
 
 
-@pytest.mark.parametrize("rows,far,dtype", [(1, 0, "f32"), (4, FAR, "f32"), (40, 0, "f32"), (400, 0, "f32"), (1, 0, "bf16")])
-def test_queries_far_below_one_that_meets_only_zeros(rows, far, dtype):
+@pytest.mark.parametrize("rows,far", [(1, 0), (4, FAR), (40, 0), (400, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_queries_far_below_one_that_meets_only_zeros(dtype, rows, far):
     """The attention scales a row by its largest query and loses bits of those far below it.  Where that one
-    meets zeros alone, the scores are what is lost: weights then are some softmax's, each at most 1."""
+    meets zeros alone, the scores are what is lost: a position's weight is still at most 1 a row and head."""
     nh, nkv, hd, ps, pos = 16, 4, 64, 16, 100
     rng = np.random.default_rng(43)
     table, n_pages = ref.pages_for([(rows, pos)], ps, rng)
